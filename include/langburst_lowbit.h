@@ -230,6 +230,94 @@ int lb_marlin_gemm_noalloc(const uint16_t* A, const int32_t* B, uint16_t* C, con
 int lb_marlin_dequant(const int32_t* B, const uint16_t* s, uint16_t* w_nk,
                       int64_t prob_n, int64_t prob_k, int64_t groupsize, lb_stream_t stream);
 
+/* ---------------- Attention between the QKV and the O projection ----------------
+ * No counterpart in the reference's projection path: the operators that a layer
+ * needs between lb_marlin_gemm of QKV and lb_marlin_gemm of O.
+ *
+ * Rows: fp16 [tokens, heads, head_dim]; the token and head strides are given in
+ * elements and the last axis is contiguous, so a row may be a part of the fused
+ * projection's output.  Base addresses 16-byte aligned, strides multiples of 8.
+ * head_dim 64, 128 or 256; heads_q a multiple of heads_kv (query head h reads
+ * key/value head h / (heads_q / heads_kv)).
+ *
+ * Cache: pages of page_size (16, 32, 64 or 128) tokens, codes in [-127, 127]:
+ *   k_cache int8 [num_pages, heads_kv, page_size, head_dim]
+ *   v_cache int8 [num_pages, heads_kv, head_dim, page_size]
+ *   k_scale, v_scale fp32 [num_pages, heads_kv]; a value is code * scale
+ * page_table int32 [batch, max_pages], rows table_stride apart: sequence b's
+ * token t is slot t % page_size of page page_table[b][t / page_size].  A page
+ * number outside [0, num_pages) has no page: nothing is stored there and its
+ * tokens are not attended; numbers past a sequence's length are not read.
+ * seq_lens int32 [batch]: tokens of each sequence, the new ones included;
+ * at most max_pages * page_size are read.
+ * cu_seqlens int32 [batch + 1]: the packed tokens cu_seqlens[b] to
+ * cu_seqlens[b + 1] - 1 are sequence b's (its newest, in order); NULL: every
+ * sequence has tokens / batch.  Tokens that belong to no sequence are skipped. */
+
+/* Rotates queries and keys and stores keys and values, in one launch.
+ * cos_sin fp32 [positions, rot_dim]: cos of the rot_dim / 2 angles of a
+ * position, then sin; a token's position is its place in the sequence, and one
+ * outside the table gives NaN.  rot_dim % 16 == 0, 0 to head_dim: the first rot_dim values of a
+ * head are rotated, as halves (i, i + rot_dim / 2) or, interleaved, as pairs
+ * (2 i, 2 i + 1); cos_sin may be NULL when it is 0.
+ * A page's scale is max |x| / 127 over its tokens when they enter.  A page that
+ * holds earlier tokens of the sequence keeps its scale unless the new tokens
+ * need a larger one, and then its codes are rescaled.  A non-finite key or
+ * value makes the scale non-finite.
+ * q and q_out may be NULL together (no queries); q_out may be q.  k_out, when
+ * given, receives the rotated keys and must not be k.  A token before position
+ * 0 (seq_lens[b] below the sequence's new tokens) is padding: its q_out row is
+ * zero and nothing is stored.  Two sequences of one call must not append to the
+ * same page. */
+int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                  const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                  const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride,
+                  uint16_t* q_out, int64_t qo_token_stride, int64_t qo_head_stride,
+                  uint16_t* k_out, int64_t ko_token_stride, int64_t ko_head_stride,
+                  int8_t* k_cache, int8_t* v_cache, float* k_scale, float* v_scale,
+                  int64_t num_pages, int64_t page_size,
+                  const int32_t* page_table, int64_t max_pages, int64_t table_stride,
+                  const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t batch, int64_t tokens,
+                  int64_t heads_q, int64_t heads_kv, int64_t head_dim,
+                  const float* cos_sin, int64_t positions, int64_t rot_dim, int32_t interleaved,
+                  lb_stream_t stream);
+
+/* out = softmax(softmax_scale * q k^T) v over the cache, one launch.  The
+ * tokens / batch newest tokens of every sequence are the queries; token i of n
+ * sees the keys 0 to seq_lens[b] - n + i, and a row that sees none is zero.
+ * Scores, softmax and sums are fp32; a weight times its value scale is rounded
+ * to fp16 for the second product, relative to the largest scale met.
+ * workspace: int32, zero on entry, left zero, at least
+ * batch * heads_kv * ceil(tokens / batch * heads_q / heads_kv / 16) entries
+ * (tokens * heads_q always suffice).  scratch: lb_kv8_attention_scratch_bytes()
+ * bytes, no initialisation.  Calls that share either must not overlap.
+ * softmax_scale positive and finite. */
+size_t lb_kv8_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv,
+                                      int64_t head_dim, int64_t page_size, int64_t max_pages);
+int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                     const int8_t* k_cache, const int8_t* v_cache, const float* k_scale, const float* v_scale,
+                     int64_t num_pages, int64_t page_size,
+                     const int32_t* page_table, int64_t max_pages, int64_t table_stride,
+                     const int32_t* seq_lens, int64_t batch, int64_t tokens,
+                     int64_t heads_q, int64_t heads_kv, int64_t head_dim,
+                     uint16_t* out, int64_t o_token_stride, int64_t o_head_stride, float softmax_scale,
+                     int32_t* workspace, int64_t workspace_len, void* scratch, size_t scratch_bytes,
+                     lb_stream_t stream);
+
+/* Causal attention of whole prompts: token i of a sequence sees the keys 0 to
+ * i of the same sequence.  cu_seqlens NULL: one sequence (batch 1) of all
+ * tokens.  Scores, softmax and sums are fp32, weights fp16 for the second
+ * product.  Rows of tokens that belong to no sequence are left as they are.
+ * A non-finite value may reach every row of its sequence from up to 63 tokens
+ * before it on, but no other sequence.  softmax_scale positive and finite. */
+int lb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                        const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                        const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride,
+                        const int32_t* cu_seqlens, int64_t batch, int64_t tokens,
+                        int64_t heads_q, int64_t heads_kv, int64_t head_dim,
+                        uint16_t* out, int64_t o_token_stride, int64_t o_head_stride, float softmax_scale,
+                        lb_stream_t stream);
+
 /* ---------------- Measurement probe (no reference counterpart) ----------------
  * Reads `bytes` (a multiple of 16) of device memory at `src` with 16-byte
  * non-temporal loads over `workgroups` workgroups of 256 threads, each a

@@ -39,6 +39,10 @@ ARCH = "gfx950"
 # (source, object name, extra definitions); the rowwise matrix-core product is
 # compiled once per bit width
 HIP_SOURCES = [(f"{n}.hip", n, []) for n in ("lb_rowwise", "lb_marlin", "lb_probe", "lb_noalloc")]
+# fp contraction follows the pragmas in the attention sources: the cache's writer
+# rounds each operation of the rotation and the codes by itself
+HIP_SOURCES += [(f"{n}.hip", n, ["-ffp-contract=fast-honor-pragmas"])
+                for n in ("lb_kv8_append", "lb_kv8_attention", "lb_prompt_attention")]
 HIP_SOURCES += [("lb_rowwise_mm.hip", f"lb_rowwise_mm{b}", [f"-DLB_RW_BITS={b}"]) for b in range(2, 9)]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",

@@ -29,6 +29,7 @@ LB_ERR_NOALLOC_LIMIT = 9
 P = ctypes.c_void_p
 I64 = ctypes.c_int64
 I32 = ctypes.c_int32
+F32 = ctypes.c_float
 SZ = ctypes.c_size_t
 
 _SIGNATURES = {
@@ -51,6 +52,12 @@ _SIGNATURES = {
     "lb_marlin_gemm_noalloc": ([P, P, P, P, I64, I64, I64, P, I64, I64, P], ctypes.c_int),
     "lb_marlin_mlp_fused_scratch_bytes": ([I64, I64, I64], SZ),
     "lb_marlin_mlp_fused_workspace_len": ([I64, I64, I64], I64),
+    "lb_kv8_append": ([P, I64, I64] * 5 + [P, P, P, P, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, P, I64, I64, I32, P],
+                      ctypes.c_int),
+    "lb_kv8_attention_scratch_bytes": ([I64] * 7, SZ),
+    "lb_kv8_attention": ([P, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P, I64, I64, I64, I64, I64, P, I64, I64, F32, P,
+                          I64, P, SZ, P], ctypes.c_int),
+    "lb_prompt_attention": ([P, I64, I64] * 3 + [P, I64, I64, I64, I64, I64, P, I64, I64, F32, P], ctypes.c_int),
     "lb_marlin_mlp_fused": ([P, P, P, P, P, P, I64, I64, I64, I64, I64, P, I64, P, SZ, P], ctypes.c_int),
 }
 
@@ -206,3 +213,40 @@ def marlin_gemm_noalloc(a, b, c, s, workspace, group_size) -> int:
     n = b.shape[1] // 2
     return lib().lb_marlin_gemm_noalloc(_ptr(a), _ptr(b), _ptr(c), _ptr(s), m, n, k, _ptr(workspace),
                                         workspace.numel(), group_size, _stream(a))
+
+
+def _rows(t) -> tuple:
+    """Address, token stride and head stride of fp16 rows [tokens, heads, head_dim]."""
+    return (None, 0, 0) if t is None else (_ptr(t), t.stride(0), t.stride(1))
+
+
+def kv8_append(q, k, v, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cu_seqlens, cos_sin, q_out, k_out,
+               interleaved=False) -> int:
+    pages, heads_kv, page_size, head_dim = k_cache.shape
+    positions, rot = (0, 0) if cos_sin is None else cos_sin.shape
+    return lib().lb_kv8_append(*_rows(q), *_rows(k), *_rows(v), *_rows(q_out), *_rows(k_out), _ptr(k_cache),
+                               _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), pages, page_size, _ptr(page_table),
+                               page_table.shape[1], page_table.stride(0), _ptr(seq_lens), _ptr(cu_seqlens),
+                               seq_lens.shape[0], k.shape[0], 0 if q is None else q.shape[1], heads_kv, head_dim,
+                               _ptr(cos_sin), positions, rot, int(interleaved), _stream(k))
+
+
+def kv8_attention_scratch_bytes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages) -> int:
+    return int(lib().lb_kv8_attention_scratch_bytes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages))
+
+
+def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, out, workspace, scratch,
+                  softmax_scale) -> int:
+    pages, heads_kv, page_size, head_dim = k_cache.shape
+    nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    return lib().lb_kv8_attention(*_rows(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), pages,
+                                  page_size, _ptr(page_table), page_table.shape[1], page_table.stride(0),
+                                  _ptr(seq_lens), seq_lens.shape[0], q.shape[0], q.shape[1], heads_kv, head_dim,
+                                  *_rows(out), softmax_scale, _ptr(workspace), workspace.numel(), _ptr(scratch), nbytes,
+                                  _stream(q))
+
+
+def prompt_attention(q, k, v, cu_seqlens, out, softmax_scale) -> int:
+    batch = 1 if cu_seqlens is None else cu_seqlens.numel() - 1
+    return lib().lb_prompt_attention(*_rows(q), *_rows(k), *_rows(v), _ptr(cu_seqlens), batch, q.shape[0], q.shape[1],
+                                     k.shape[1], q.shape[2], *_rows(out), softmax_scale, _stream(q))

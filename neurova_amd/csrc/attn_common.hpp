@@ -1,0 +1,38 @@
+// Device helpers shared by the attention kernels: the 8-bit cache's writer and
+// reader, and the prompt attention.
+#pragma once
+
+#include "lb_common.hpp"
+
+namespace lb {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ int lane_id() { return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, int lane) {
+  return (uint32_t)__builtin_amdgcn_ds_bpermute(lane << 2, (int)v);
+}
+__device__ __forceinline__ float from_lane(float v, int lane) {
+  return __builtin_bit_cast(float, from_lane(__builtin_bit_cast(uint32_t, v), lane));
+}
+
+// The packed sequence that holds work item `item`, where sequence b's items
+// start at starts[b] * per / span + slack * b (monotone in b for sorted starts):
+// the last b whose first item is <= item, -1 if there is none.  The whole wave
+// searches together, 64 sequences a load; `item` is wave-uniform.
+__device__ __forceinline__ int sequence_of_item(const int32_t* starts, int batch, int per, int span, int slack,
+                                                int item) {
+  const int lane = lane_id();
+  int count = 0;
+  for (int c = 0; c < batch; c += kWave) {
+    const int b = c + lane;
+    const bool le = b < batch && starts[b] * per / span + slack * b <= item;
+    const uint64_t m = __ballot(le);
+    count += __popcll(m);
+    if (m != ~0ull) break;
+  }
+  return __builtin_amdgcn_readfirstlane(count) - 1;
+}
+
+}  // namespace lb

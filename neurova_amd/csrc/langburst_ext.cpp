@@ -5,8 +5,9 @@
 // include/langburst_lowbit.h.  Tensors are launched on the caller's current
 // HIP stream; nothing here synchronises.
 //
-// Only the low-bit projection ops are provided; the reference module's other
-// ops (RMSNorm, GDN, attention, sampling) are outside this library.
+// Of the reference module's ops only the low-bit projections are provided; its
+// RMSNorm, GDN, attention and sampling ops are outside this library.  The
+// attention ops here (8-bit cache, prompts) are this library's own.
 
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
@@ -428,6 +429,169 @@ torch::Tensor lowbit_marlin_dequant(torch::Tensor qweight, torch::Tensor scales,
   return w;
 }
 
+// -------------------------------------------------------------- attention ---
+
+#define LB_CHECK_I32(x) TORCH_CHECK((x).scalar_type() == at::kInt, #x " must be int32")
+
+// fp16 rows [tokens, heads, head_dim] as the C ABI takes them.  The stride of an
+// axis of one entry means nothing and may be any number: the packed one instead.
+struct RowsView {
+  uint16_t* p = nullptr;
+  int64_t token = 0, head = 0;
+};
+
+RowsView rows_of(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
+  TORCH_CHECK(t.is_cuda(), name, " must be CUDA");
+  TORCH_CHECK(t.device() == like.device(), name, " must be on the same device as the other tensors");
+  TORCH_CHECK(t.scalar_type() == at::kHalf, name, " must be fp16");
+  TORCH_CHECK(t.dim() == 3, name, " must be [tokens, heads, head_dim]");
+  TORCH_CHECK(t.stride(2) == 1 || t.size(2) == 1, name, " must be contiguous along head_dim");
+  RowsView r;
+  r.p = h16m(t);
+  r.head = t.size(1) == 1 ? t.size(2) : t.stride(1);
+  r.token = t.size(0) == 1 ? t.size(1) * t.size(2) : t.stride(0);
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.head % 8 == 0 && r.token % 8 == 0, name,
+              " must have 16-byte aligned rows");
+  return r;
+}
+
+// The cache's tensors and tables; returns (num_pages, heads_kv, page_size, head_dim).
+struct CacheShape {
+  int64_t pages, heads, page_size, head_dim, batch, max_pages, table_stride;
+};
+
+CacheShape check_kv8_cache(const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& k_scale,
+                           const torch::Tensor& v_scale, const torch::Tensor& page_table,
+                           const torch::Tensor& seq_lens) {
+  LB_CHECK_DEV(k_cache); LB_CHECK_DEV(v_cache); LB_CHECK_DEV(k_scale); LB_CHECK_DEV(v_scale);
+  LB_CHECK_DEV(page_table); LB_CHECK_DEV(seq_lens);
+  for (const torch::Tensor* t : {&v_cache, &k_scale, &v_scale, &page_table, &seq_lens})
+    TORCH_CHECK(t->device() == k_cache.device(), "the cache's tensors must be on the same device");
+  LB_CHECK_CONTIG(k_cache); LB_CHECK_CONTIG(v_cache); LB_CHECK_CONTIG(k_scale); LB_CHECK_CONTIG(v_scale);
+  LB_CHECK_CONTIG(seq_lens);
+  TORCH_CHECK(k_cache.scalar_type() == at::kChar && v_cache.scalar_type() == at::kChar,
+              "k_cache and v_cache must be int8");
+  LB_CHECK_FLOAT(k_scale); LB_CHECK_FLOAT(v_scale); LB_CHECK_I32(page_table); LB_CHECK_I32(seq_lens);
+  TORCH_CHECK(k_cache.dim() == 4, "k_cache must be [pages, heads, page_size, head_dim]");
+  CacheShape c;
+  c.pages = k_cache.size(0), c.heads = k_cache.size(1), c.page_size = k_cache.size(2), c.head_dim = k_cache.size(3);
+  TORCH_CHECK(v_cache.dim() == 4 && v_cache.size(0) == c.pages && v_cache.size(1) == c.heads &&
+                  v_cache.size(2) == c.head_dim && v_cache.size(3) == c.page_size,
+              "v_cache must be [pages, heads, head_dim, page_size]");
+  TORCH_CHECK(k_scale.dim() == 2 && k_scale.size(0) == c.pages && k_scale.size(1) == c.heads,
+              "k_scale must be [pages, heads]");
+  TORCH_CHECK(v_scale.sizes() == k_scale.sizes(), "v_scale must be [pages, heads]");
+  TORCH_CHECK(c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256, "head_dim must be 64, 128 or 256");
+  TORCH_CHECK(c.page_size == 16 || c.page_size == 32 || c.page_size == 64 || c.page_size == 128,
+              "page_size must be 16, 32, 64 or 128");
+  TORCH_CHECK(seq_lens.dim() == 1, "seq_lens must be [batch]");
+  c.batch = seq_lens.size(0);
+  TORCH_CHECK(page_table.dim() == 2 && page_table.size(0) == c.batch, "page_table must be [batch, max_pages]");
+  c.max_pages = page_table.size(1);
+  TORCH_CHECK(page_table.stride(1) == 1 || c.max_pages <= 1, "page_table must be contiguous along the pages");
+  c.table_stride = c.batch <= 1 ? c.max_pages : page_table.stride(0);
+  TORCH_CHECK(c.table_stride >= c.max_pages, "page_table rows must not overlap");
+  return c;
+}
+
+const int32_t* check_cu_seqlens(const c10::optional<torch::Tensor>& cu, int64_t batch, const torch::Tensor& like) {
+  if (!cu.has_value()) return nullptr;
+  const torch::Tensor& cu_seqlens = *cu;
+  LB_CHECK_DEV(cu_seqlens); LB_CHECK_CONTIG(cu_seqlens); LB_CHECK_I32(cu_seqlens);
+  TORCH_CHECK(cu_seqlens.device() == like.device(), "cu_seqlens must be on the same device as the other tensors");
+  TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.size(0) == batch + 1, "cu_seqlens must be [batch + 1]");
+  return cu_seqlens.data_ptr<int32_t>();
+}
+
+void kv8_append_out(c10::optional<torch::Tensor> q, torch::Tensor k, torch::Tensor v, torch::Tensor k_cache,
+                    torch::Tensor v_cache, torch::Tensor k_scale, torch::Tensor v_scale, torch::Tensor page_table,
+                    torch::Tensor seq_lens, c10::optional<torch::Tensor> cu_seqlens,
+                    c10::optional<torch::Tensor> cos_sin, c10::optional<torch::Tensor> q_out,
+                    c10::optional<torch::Tensor> k_out, bool interleaved) {
+  const CacheShape c = check_kv8_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens);
+  const RowsView kr = rows_of(k, "k", k_cache), vr = rows_of(v, "v", k_cache);
+  const int64_t tokens = k.size(0);
+  TORCH_CHECK(k.size(1) == c.heads && k.size(2) == c.head_dim, "k must be [tokens, heads, head_dim] of the cache");
+  TORCH_CHECK(v.sizes() == k.sizes(), "v must have k's shape");
+  TORCH_CHECK(q.has_value() == q_out.has_value(), "q and q_out must be given together");
+  RowsView qr, qo, ko;
+  if (q.has_value()) {
+    qr = rows_of(*q, "q", k_cache), qo = rows_of(*q_out, "q_out", k_cache);
+    TORCH_CHECK(q->size(0) == tokens && q->size(2) == c.head_dim, "q must be [tokens, heads_q, head_dim]");
+    TORCH_CHECK(q_out->sizes() == q->sizes(), "q_out must have q's shape");
+  }
+  if (k_out.has_value()) {
+    ko = rows_of(*k_out, "k_out", k_cache);
+    TORCH_CHECK(k_out->sizes() == k.sizes(), "k_out must have k's shape");
+    TORCH_CHECK(ko.p != kr.p || tokens == 0, "k_out must not be k");
+  }
+  const int32_t* cu = check_cu_seqlens(cu_seqlens, c.batch, k_cache);
+  TORCH_CHECK(cu != nullptr || (c.batch == 0 ? tokens == 0 : tokens % c.batch == 0),
+              "without cu_seqlens every sequence needs the same number of tokens");
+  int64_t positions = 0, rot = 0;
+  const float* table = nullptr;
+  if (cos_sin.has_value()) {
+    const torch::Tensor& t = *cos_sin;
+    TORCH_CHECK(t.is_cuda() && t.device() == k_cache.device(), "cos_sin must be on the same device as the cache");
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous() && t.dim() == 2,
+                "cos_sin must be contiguous fp32 [positions, rot_dim]");
+    positions = t.size(0), rot = t.size(1), table = t.data_ptr<float>();
+    TORCH_CHECK(rot % 16 == 0 && rot <= c.head_dim, "rot_dim must be a multiple of 16, at most head_dim");
+  }
+  const c10::DeviceGuard guard(k_cache.device());
+  lb_ok(lb_kv8_append(qr.p, qr.token, qr.head, kr.p, kr.token, kr.head, vr.p, vr.token, vr.head, qo.p, qo.token,
+                      qo.head, ko.p, ko.token, ko.head, k_cache.data_ptr<int8_t>(), v_cache.data_ptr<int8_t>(),
+                      k_scale.data_ptr<float>(), v_scale.data_ptr<float>(), c.pages, c.page_size,
+                      page_table.data_ptr<int32_t>(), c.max_pages, c.table_stride, seq_lens.data_ptr<int32_t>(), cu,
+                      c.batch, tokens, q.has_value() ? q->size(1) : 0, c.heads, c.head_dim, table, positions, rot,
+                      interleaved ? 1 : 0, stream_of(k_cache)),
+        "kv8_append_out");
+}
+
+void kv8_attention_out(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
+                       torch::Tensor v_scale, torch::Tensor page_table, torch::Tensor seq_lens, torch::Tensor out,
+                       torch::Tensor workspace, double softmax_scale) {
+  const CacheShape c = check_kv8_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens);
+  const RowsView qr = rows_of(q, "q", k_cache), ov = rows_of(out, "out", k_cache);
+  const int64_t tokens = q.size(0), heads_q = q.size(1);
+  TORCH_CHECK(q.size(2) == c.head_dim, "q must be [tokens, heads_q, head_dim]");
+  TORCH_CHECK(heads_q > 0 && heads_q % c.heads == 0, "heads_q must be a multiple of the cache's heads");
+  TORCH_CHECK(c.batch == 0 ? tokens == 0 : tokens % c.batch == 0, "q must hold the same number of tokens for every sequence");
+  TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
+  LB_CHECK_DEV(workspace); LB_CHECK_CONTIG(workspace); LB_CHECK_I32(workspace);
+  TORCH_CHECK(workspace.device() == k_cache.device(), "workspace must be on the same device as the cache");
+  TORCH_CHECK(softmax_scale > 0 && softmax_scale < 3e38, "softmax_scale must be positive and finite");
+  const c10::DeviceGuard guard(k_cache.device());
+  auto scratch = op_scratch(
+      lb_kv8_attention_scratch_bytes(c.batch, tokens, heads_q, c.heads, c.head_dim, c.page_size, c.max_pages), q);
+  lb_ok(lb_kv8_attention(qr.p, qr.token, qr.head, k_cache.data_ptr<int8_t>(), v_cache.data_ptr<int8_t>(),
+                         k_scale.data_ptr<float>(), v_scale.data_ptr<float>(), c.pages, c.page_size,
+                         page_table.data_ptr<int32_t>(), c.max_pages, c.table_stride, seq_lens.data_ptr<int32_t>(),
+                         c.batch, tokens, heads_q, c.heads, c.head_dim, ov.p, ov.token, ov.head, (float)softmax_scale,
+                         workspace.data_ptr<int32_t>(), workspace.numel(), scratch.ptr, scratch.bytes,
+                         stream_of(k_cache)),
+        "kv8_attention_out");
+}
+
+void prompt_attention_out(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> cu_seqlens,
+                          torch::Tensor out, double softmax_scale) {
+  const RowsView qr = rows_of(q, "q", q), kr = rows_of(k, "k", q), vr = rows_of(v, "v", q), ov = rows_of(out, "out", q);
+  const int64_t tokens = q.size(0), heads_q = q.size(1), head_dim = q.size(2);
+  TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim must be 64, 128 or 256");
+  TORCH_CHECK(k.size(0) == tokens && k.size(2) == head_dim, "k must be [tokens, heads_kv, head_dim]");
+  TORCH_CHECK(v.sizes() == k.sizes(), "v must have k's shape");
+  TORCH_CHECK(heads_q > 0 && k.size(1) > 0 && heads_q % k.size(1) == 0, "heads_q must be a multiple of k's heads");
+  TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
+  TORCH_CHECK(softmax_scale > 0 && softmax_scale < 3e38, "softmax_scale must be positive and finite");
+  const int64_t batch = cu_seqlens.has_value() ? cu_seqlens->numel() - 1 : 1;
+  const int32_t* cu = check_cu_seqlens(cu_seqlens, batch, q);
+  const c10::DeviceGuard guard(q.device());
+  lb_ok(lb_prompt_attention(qr.p, qr.token, qr.head, kr.p, kr.token, kr.head, vr.p, vr.token, vr.head, cu, batch,
+                            tokens, heads_q, k.size(1), head_dim, ov.p, ov.token, ov.head, (float)softmax_scale,
+                            stream_of(q)),
+        "prompt_attention_out");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(langburst_cuda, m) {
@@ -475,6 +639,18 @@ PYBIND11_MODULE(langburst_cuda, m) {
         },
         "int32 elements of the workspace lowbit_marlin_mlp_fused_out needs", py::arg("batch"), py::arg("hidden"),
         py::arg("intermediate"));
+  m.def("kv8_append_out", &kv8_append_out,
+        "Rotates queries and keys to their positions and stores keys and values in the paged 8-bit cache",
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("page_table"), py::arg("seq_lens"), py::arg("cu_seqlens"), py::arg("cos_sin"),
+        py::arg("q_out"), py::arg("k_out"), py::arg("interleaved") = false);
+  m.def("kv8_attention_out", &kv8_attention_out,
+        "Attention of each sequence's newest tokens over its pages of the 8-bit cache", py::arg("q"),
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("page_table"),
+        py::arg("seq_lens"), py::arg("out"), py::arg("workspace"), py::arg("softmax_scale"));
+  m.def("prompt_attention_out", &prompt_attention_out,
+        "Causal attention inside each of the packed sequences of a batch of prompts", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("cu_seqlens"), py::arg("out"), py::arg("softmax_scale"));
   m.def("abi_version", []() { return lb_abi_version(); });
   m.attr("__provides__") = py::make_tuple("lowbit_gemv", "lowbit_row_dequant", "lowbit_gemv_pair", "lowbit_gemm",
                                           "lowbit_marlin_gemm", "lowbit_marlin_gemm_out",

@@ -1,0 +1,431 @@
+// Writer of the paged 8-bit cache: rotates queries and keys to their positions
+// and stores keys and values as codes, one launch for both.
+//
+//   q'  = R(pos) q,  k' = R(pos) k    R(pos): pairs (a, b) of the first rot values of a
+//                                     head become (a cos - b sin, b cos + a sin)
+//   s   = max(s_old if the page holds earlier tokens, max |x| / 127)   per page, head; K and V apart
+//   old = rint(old * s_old / s) where s grew
+//   c   = rint(x / s)
+//
+// The rotation and the codes are computed with each product and sum rounded to
+// fp32 by itself (no contraction), so a program that repeats the definition in
+// 32 bits gets the same codes.
+#include "attn_common.hpp"
+
+namespace lb {
+namespace {
+
+struct Rows {  // fp16 [tokens][heads][head_dim], the last axis contiguous
+  uint16_t* p;
+  int64_t token, head;  // strides in elements
+};
+
+struct AppendArgs {
+  Rows q, k, v, q_out, k_out;
+  int8_t *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  const int32_t *page_table, *seq_lens, *starts;
+  const float* cos_sin;
+  int64_t table_stride;
+  int num_pages, page_shift, max_pages;
+  int batch, tokens, heads_q, heads_kv, d8;  // d8: head_dim / 8
+  int positions, rot, interleaved;
+  int per_seq;    // tokens of each sequence where starts is null
+  int kv_blocks;  // workgroups of the keys and values, before those of the queries
+  int page_bound;  // pages a sequence can touch (starts null)
+  int q_heads_per_thread;
+};
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x8 load8(const uint16_t* p) {
+  const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+  f32x8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f16x2 h = as_h2(w[i]);
+    r[2 * i] = (float)h[0];
+    r[2 * i + 1] = (float)h[1];
+  }
+  return r;
+}
+
+__device__ __forceinline__ void store8(uint16_t* p, f32x8 v) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = as_u32((f16x2){(f16)v[2 * i], (f16)v[2 * i + 1]});
+  *reinterpret_cast<u32x4*>(p) = w;
+}
+
+// cos and sin of eight consecutive frequencies at `pos`.  A position outside
+// the table has none: NaN, which the outputs then show.
+__device__ __forceinline__ void angles(const AppendArgs& a, int pos, int f, f32x8& c, f32x8& s) {
+  if ((unsigned)pos >= (unsigned)a.positions) {
+    c = s = (f32x8)(__builtin_nanf(""));
+    return;
+  }
+  const float* row = a.cos_sin + (int64_t)pos * a.rot + f;
+  c = *reinterpret_cast<const f32x8*>(__builtin_assume_aligned(row, 16));
+  s = *reinterpret_cast<const f32x8*>(__builtin_assume_aligned(row + a.rot / 2, 16));
+}
+
+// The same of four.
+__device__ __forceinline__ void angles4(const AppendArgs& a, int pos, int f, f32x8& c, f32x8& s) {
+  if ((unsigned)pos >= (unsigned)a.positions) {
+    c = s = (f32x8)(__builtin_nanf(""));
+    return;
+  }
+  const float* row = a.cos_sin + (int64_t)pos * a.rot + f;
+  const f32x4 c4 = *reinterpret_cast<const f32x4*>(row), s4 = *reinterpret_cast<const f32x4*>(row + a.rot / 2);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c[j] = c4[j], s[j] = s4[j];
+}
+
+// (x, y) -> (x cos - y sin, y cos + x sin), every operation rounded by itself.
+__device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
+#pragma clang fp contract(off)
+  const float xc = x * c, ys = y * s, yc = y * c, xs = x * s;
+  x = xc - ys;
+  y = yc + xs;
+}
+
+// The two vectors of eight that rotate together: halves pair value i with
+// i + rot/2, interleaved pairs are neighbours.  Pair j of a head is vectors
+// (j, j + rot/16) or (2j, 2j + 1); past the rotated part it is (2j, 2j + 1).
+struct Pair {
+  int v0, v1;
+  bool rotated;
+};
+__device__ __forceinline__ Pair pair_of(const AppendArgs& a, int j) {
+  const int n = a.rot / 16;
+  if (j < n && !a.interleaved) return {j, j + n, true};
+  return {2 * j, 2 * j + 1, j < n};
+}
+
+__device__ __forceinline__ void rotate_pair(f32x8& x, f32x8& y, const f32x8& c, const f32x8& s, bool interleaved) {
+  if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float u = x[2 * i], w = x[2 * i + 1];
+      turn(u, w, c[i], s[i]);
+      x[2 * i] = u, x[2 * i + 1] = w;
+      u = y[2 * i], w = y[2 * i + 1];
+      turn(u, w, c[4 + i], s[4 + i]);
+      y[2 * i] = u, y[2 * i + 1] = w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float u = x[i], w = y[i];
+      turn(u, w, c[i], s[i]);
+      x[i] = u, y[i] = w;
+    }
+  }
+}
+
+__device__ __forceinline__ int code_of(float x, float inverse) {
+  const float r = __builtin_rintf(x * inverse);
+  return (int)__builtin_fminf(__builtin_fmaxf(r, -127.0f), 127.0f);
+}
+
+__device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
+
+// Largest bit pattern of |x| over the workgroup: above the infinity's pattern
+// if any is NaN, so a non-finite value shows in the page's scale.
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* lds) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int x = 1; x < kWave; x *= 2) {
+    const uint32_t o = from_lane(v, lane ^ x);
+    v = o > v ? o : v;
+  }
+  const int waves = blockDim.x / kWave;
+  if (waves == 1) return v;
+  if (lane == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  for (int i = 0; i < waves; ++i) v = lds[i] > v ? lds[i] : v;
+  return v;
+}
+
+// Keys (or values) of one head in one page.  A thread holds four neighbouring
+// tokens at eight neighbouring channels: eight codes of a token are one store
+// of the key layout [page][token][channel], four of a channel one of the value
+// layout [page][channel][token], and nothing has to change threads.
+template <bool KEYS>
+__device__ __forceinline__ void append_page(const AppendArgs& a, int b, int first_token, int start, int len, int page,
+                                            int head, uint32_t* lds) {
+  const int p = 1 << a.page_shift;
+  const int page_lo = page << a.page_shift;
+  const int lo = max(max(start, 0), page_lo), hi = min(len, page_lo + p);
+  if (lo >= hi || page >= a.max_pages) return;
+  const int id = a.page_table[(int64_t)b * a.table_stride + page];
+  if ((unsigned)id >= (unsigned)a.num_pages) return;
+  const int64_t cell = (int64_t)id * a.heads_kv + head;
+  float* scale_at = (KEYS ? a.k_scale : a.v_scale) + cell;
+  const bool kept = page_lo < start;
+  const float old_scale = kept ? *scale_at : 0.0f;
+
+  const int t4 = p / 4;
+  const int tid = threadIdx.x;
+  const bool active = tid < t4 * a.d8;
+  const int d8 = KEYS ? tid % a.d8 : tid / t4;
+  const int tg = KEYS ? tid / a.d8 : tid % t4;
+  // loads of the group's four tokens together; a slot that is not new reads a
+  // new one's row instead and drops it
+  f32x8 x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = (f32x8)(0.0f);
+  const int pos0 = page_lo + 4 * tg;
+  uint32_t peak = 0;
+  if (active && pos0 + 4 > lo && pos0 < hi) {
+    const Rows& src = KEYS ? a.k : a.v;
+    const int pairs = a.rot / 16;
+    const bool rotated = KEYS && 8 * d8 < a.rot;
+    const bool low = d8 < pairs;  // halves: which of the pair this thread stores
+    f32x8 y[4], c[4], s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = min(max(pos0 + i, lo), hi - 1);
+      const uint16_t* row = src.p + (int64_t)(first_token + (pos - start)) * src.token + (int64_t)head * src.head;
+      x[i] = load8(row + 8 * d8);
+      if (rotated && a.interleaved) {
+        angles4(a, pos, 4 * d8, c[i], s[i]);
+      } else if (rotated) {
+        y[i] = load8(row + 8 * (low ? d8 + pairs : d8 - pairs));
+        angles(a, pos, 8 * (low ? d8 : d8 - pairs), c[i], s[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = pos0 + i;
+      if (rotated && a.interleaved) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float u = x[i][2 * j], w = x[i][2 * j + 1];
+          turn(u, w, c[i][j], s[i][j]);
+          x[i][2 * j] = u, x[i][2 * j + 1] = w;
+        }
+      } else if (rotated) {
+        f32x8 u = low ? x[i] : y[i], w = low ? y[i] : x[i];
+        rotate_pair(u, w, c[i], s[i], false);
+        x[i] = low ? u : w;
+      }
+      if (pos < lo || pos >= hi) {
+        x[i] = (f32x8)(0.0f);
+        continue;
+      }
+      if (KEYS && a.k_out.p)
+        store8(a.k_out.p + (int64_t)(first_token + (pos - start)) * a.k_out.token + (int64_t)head * a.k_out.head + 8 * d8,
+               x[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = x[i][j];
+        const uint32_t m = __builtin_bit_cast(uint32_t, e) & 0x7fffffffu;
+        peak = m > peak ? m : peak;
+      }
+    }
+  }
+  peak = block_max(peak, lds);
+  const float need = __builtin_bit_cast(float, peak) * (1.0f / 127.0f);
+  // `need` may be NaN: then it is taken
+  const float scale = need <= old_scale ? old_scale : need;
+  const bool grew = kept && scale != old_scale;
+  if (tid == 0 && scale != old_scale) *scale_at = scale;
+  if (tid == 0 && !kept && scale == 0.0f) *scale_at = 0.0f;
+  const float inverse = scale > 0.0f ? 1.0f / scale : 0.0f;
+  const float shrink = grew ? old_scale / scale : 1.0f;
+  if (!active) return;
+
+  const int old_slots = kept ? start - page_lo : 0;  // slots before the new tokens
+  const int off0 = 4 * tg;
+  if (KEYS) {
+    int8_t* base = a.k_cache + ((cell << a.page_shift) + off0) * (8 * a.d8) + 8 * d8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = page_lo + off0 + i;
+      u32x2* at = reinterpret_cast<u32x2*>(base + i * 8 * a.d8);
+      if (pos >= lo && pos < hi) {
+        u32x2 w = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j / 4] |= (uint32_t)(code_of(x[i][j], inverse) & 255) << (8 * (j % 4));
+        *at = w;
+      } else if (grew && off0 + i < old_slots) {
+        const u32x2 old = *at;
+        u32x2 w = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          w[j / 4] |= (uint32_t)(code_of((float)byte_of(old[j / 4], j % 4), shrink) & 255) << (8 * (j % 4));
+        *at = w;
+      }
+    }
+  } else {
+    int8_t* base = a.v_cache + ((cell * (8 * a.d8) + 8 * d8) << a.page_shift) + off0;
+    const bool full = page_lo + off0 >= lo && page_lo + off0 + 4 <= hi;
+    const bool olds = grew && off0 < old_slots;
+    const bool any_new = page_lo + off0 + 4 > lo && page_lo + off0 < hi;
+    if (!any_new && !olds) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      int8_t* at = base + ((int64_t)j << a.page_shift);
+      uint32_t w = 0;
+      if (full) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= (uint32_t)(code_of(x[i][j], inverse) & 255) << (8 * i);
+        *reinterpret_cast<uint32_t*>(at) = w;
+      } else if (olds) {
+        const uint32_t old = *reinterpret_cast<const uint32_t*>(at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int pos = page_lo + off0 + i;
+          int c = byte_of(old, i);
+          if (pos >= lo && pos < hi) c = code_of(x[i][j], inverse);
+          else if (off0 + i < old_slots) c = code_of((float)c, shrink);
+          w |= (uint32_t)(c & 255) << (8 * i);
+        }
+        *reinterpret_cast<uint32_t*>(at) = w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int pos = page_lo + off0 + i;
+          if (pos >= lo && pos < hi) at[i] = (int8_t)code_of(x[i][j], inverse);
+        }
+      }
+    }
+  }
+}
+
+// Rows of padding (a token before position 0) come out as zeros.
+__device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t job) {
+  const int pairs = a.d8 / 2;
+  const int j = (int)(job % pairs);
+  const int64_t rest = job / pairs;
+  const int chunks = (a.heads_q + a.q_heads_per_thread - 1) / a.q_heads_per_thread;
+  const int chunk = (int)(rest % chunks);
+  const int64_t t64 = rest / chunks;
+  if (t64 >= a.tokens) return;
+  const int t = (int)t64;
+  int b, first, n;
+  if (a.starts == nullptr) {
+    b = t / a.per_seq, first = b * a.per_seq, n = a.per_seq;
+  } else {
+    int lo = 0, hi = a.batch;  // the last b in [0, batch] with starts[b] <= t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (a.starts[mid] <= t) lo = mid; else hi = mid;
+    }
+    b = lo, first = a.starts[b], n = a.starts[b + 1] - first;
+    if (t < first || t >= first + n) return;  // outside every sequence
+  }
+  const int pos = a.seq_lens[b] - n + (t - first);
+  const Pair pr = pair_of(a, j);
+  f32x8 c, s;
+  if (pr.rotated) angles(a, pos, 8 * j, c, s);
+  const int h0 = chunk * a.q_heads_per_thread, h1 = min(h0 + a.q_heads_per_thread, a.heads_q);
+#pragma unroll 4
+  for (int h = h0; h < h1; ++h) {
+    const uint16_t* row = a.q.p + (int64_t)t * a.q.token + (int64_t)h * a.q.head;
+    uint16_t* out = a.q_out.p + (int64_t)t * a.q_out.token + (int64_t)h * a.q_out.head;
+    f32x8 x = load8(row + 8 * pr.v0), y = load8(row + 8 * pr.v1);
+    if (pr.rotated) rotate_pair(x, y, c, s, a.interleaved);
+    if (pos < 0) x = y = (f32x8)(0.0f);
+    store8(out + 8 * pr.v0, x);
+    store8(out + 8 * pr.v1, y);
+  }
+}
+
+__global__ __launch_bounds__(1024) void kv8_append_kernel(AppendArgs a) {
+  __shared__ uint32_t lds[16];
+  if ((int)blockIdx.x >= a.kv_blocks) {
+    rotate_queries(a, (int64_t)(blockIdx.x - a.kv_blocks) * blockDim.x + threadIdx.x);
+    return;
+  }
+  // workgroup -> (page item, head, keys or values)
+  const int kind = blockIdx.x & 1;
+  const int rest = blockIdx.x >> 1;
+  const int head = rest % a.heads_kv, item = rest / a.heads_kv;
+  int b, first, n, page;
+  if (a.starts == nullptr) {
+    b = item / a.page_bound, page = item % a.page_bound;
+    first = b * a.per_seq, n = a.per_seq;
+  } else {
+    b = sequence_of_item(a.starts, a.batch, 1, 1 << a.page_shift, 2, item);
+    if (b < 0) return;
+    first = max(a.starts[b], 0), n = min(a.starts[b + 1], a.tokens) - first;
+    page = item - (a.starts[b] / (1 << a.page_shift) + 2 * b);
+    if (n <= 0) return;
+  }
+  const int len = a.seq_lens[b];
+  const int start = len - n;
+  page += max(start, 0) >> a.page_shift;
+  if (kind == 0) append_page<true>(a, b, first, start, len, page, head, lds);
+  else append_page<false>(a, b, first, start, len, page, head, lds);
+}
+
+}  // namespace
+}  // namespace lb
+
+extern "C" int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
+                             int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v, int64_t v_token_stride,
+                             int64_t v_head_stride, uint16_t* q_out, int64_t qo_token_stride, int64_t qo_head_stride,
+                             uint16_t* k_out, int64_t ko_token_stride, int64_t ko_head_stride, int8_t* k_cache,
+                             int8_t* v_cache, float* k_scale, float* v_scale, int64_t num_pages, int64_t page_size,
+                             const int32_t* page_table, int64_t max_pages, int64_t table_stride,
+                             const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t batch, int64_t tokens,
+                             int64_t heads_q, int64_t heads_kv, int64_t head_dim, const float* cos_sin,
+                             int64_t positions, int64_t rot_dim, int32_t interleaved, lb_stream_t stream) {
+  using namespace lb;
+  constexpr int64_t kIntMax = 0x7fffffff;
+  if (batch < 0 || tokens < 0 || heads_q < 0 || heads_kv <= 0 || num_pages < 0 || max_pages < 0 || rot_dim < 0 ||
+      positions < 0)
+    return LB_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return LB_ERR_PROB_SHAPE;
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return LB_ERR_PROB_SHAPE;
+  if (rot_dim > head_dim || rot_dim % 16 != 0) return LB_ERR_PROB_SHAPE;
+  if (heads_q > 4096 || heads_kv > 4096 || batch > (1 << 20) || tokens > (1 << 26) || num_pages > kIntMax ||
+      max_pages > kIntMax / page_size || positions > kIntMax || table_stride < max_pages)
+    return LB_ERR_ARG;
+  if (tokens == 0 || batch == 0) return LB_OK;
+  if (cu_seqlens == nullptr && tokens % batch != 0) return LB_ERR_ARG;
+  const bool queries = q_out != nullptr && heads_q > 0;
+  if (!k || !v || !k_cache || !v_cache || !k_scale || !v_scale || !page_table || !seq_lens || (queries && !q) ||
+      (rot_dim > 0 && !cos_sin))
+    return LB_ERR_ARG;
+  if (k_out == k) return LB_ERR_ARG;  // a thread reads both halves of a pair and writes one
+  const void* ptrs[] = {k, v, queries ? q : nullptr, q_out, k_out, k_cache, v_cache, cos_sin};
+  for (const void* p : ptrs)
+    if (!lbh::aligned(p, 16)) return LB_ERR_ALIGN;
+  int64_t strides = k_token_stride | k_head_stride | v_token_stride | v_head_stride;
+  if (queries) strides |= q_token_stride | q_head_stride | qo_token_stride | qo_head_stride;
+  if (k_out) strides |= ko_token_stride | ko_head_stride;
+  if (strides % 8 != 0) return LB_ERR_ALIGN;
+
+  AppendArgs a;
+  a.q = {const_cast<uint16_t*>(q), q_token_stride, q_head_stride};
+  a.k = {const_cast<uint16_t*>(k), k_token_stride, k_head_stride};
+  a.v = {const_cast<uint16_t*>(v), v_token_stride, v_head_stride};
+  a.q_out = {q_out, qo_token_stride, qo_head_stride};
+  a.k_out = {k_out, ko_token_stride, ko_head_stride};
+  a.k_cache = k_cache, a.v_cache = v_cache, a.k_scale = k_scale, a.v_scale = v_scale;
+  a.page_table = page_table, a.seq_lens = seq_lens, a.starts = cu_seqlens, a.cos_sin = cos_sin;
+  a.table_stride = table_stride, a.num_pages = (int)num_pages, a.max_pages = (int)max_pages;
+  a.page_shift = __builtin_ctzll((unsigned long long)page_size);
+  a.batch = (int)batch, a.tokens = (int)tokens, a.heads_q = (int)heads_q, a.heads_kv = (int)heads_kv;
+  a.d8 = (int)head_dim / 8, a.positions = (int)positions, a.rot = (int)rot_dim, a.interleaved = interleaved != 0;
+  a.per_seq = cu_seqlens ? 0 : (int)(tokens / batch);
+  // pages that n tokens can touch: floor((n - 2) / P) + 2 for n >= 1
+  a.page_bound = cu_seqlens ? 0 : (int)((a.per_seq - 2 + page_size) / page_size + 1);
+  // packed: sequence b's pages are numbered from cu_seqlens[b] / P + 2 b, which leaves room for all of them
+  const int64_t items = cu_seqlens ? tokens / page_size + 2 * batch : batch * a.page_bound;
+  const int64_t kv_blocks = items * heads_kv * 2;
+  const int threads = (int)(page_size * head_dim / 32 < kWave ? kWave : page_size * head_dim / 32);
+  // a thread's angles serve several heads once there are threads enough for the chip
+  const int64_t lanes = tokens * (head_dim / 16);
+  a.q_heads_per_thread = lanes * heads_q >= (int64_t)8 * lbh::device_cus() * 2048 ? 8 : 1;
+  const int64_t chunks = (heads_q + a.q_heads_per_thread - 1) / a.q_heads_per_thread;
+  const int64_t q_blocks = queries ? (lanes * chunks + threads - 1) / threads : 0;
+  if (kv_blocks + q_blocks > kIntMax) return LB_ERR_ARG;
+  a.kv_blocks = (int)kv_blocks;
+  kv8_append_kernel<<<dim3((unsigned)(kv_blocks + q_blocks)), dim3(threads), 0,
+                      reinterpret_cast<hipStream_t>(stream)>>>(a);
+  return lbh::launch_status();
+}

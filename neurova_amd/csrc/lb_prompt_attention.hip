@@ -1,0 +1,275 @@
+// Causal attention inside each of the packed sequences of a batch of prompts.
+//
+//   o[i] = sum_{j <= i} softmax_j(scale q[i] . k[j]) v[j]      per sequence and query head
+//
+// Bound by the matrix cores: 4 head_dim flop a query, key and head.  The rows of
+// a tile are (token, query head of the group) pairs of one key/value head, so a
+// tile of 256 rows spans few tokens: its waves end at the same keys and little
+// work falls past the diagonal.
+//
+//   S^T = K Q^T    32x32x16: a lane holds 16 keys of one row, so a row's maximum
+//                  and sum stay in the lane but for one exchange with lane ^ 32
+//   O^T = V^T P^T  the weights of a lane are already the second product's operand
+#include "attn_common.hpp"
+
+namespace lb {
+namespace {
+
+struct PromptArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t* out;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
+  const int32_t* starts;
+  int batch, tokens, group, heads_kv, tiles;
+  float scale;  // softmax scale * log2(e)
+};
+
+constexpr int kWaves = 4;
+constexpr int kKeys = 64;  // keys of a tile
+constexpr float kNoMax = -1e30f;
+// The running maximum moves only when a score exceeds it by 2^kSlack, and the
+// weights (and their sum) carry 2^kLift more: at most 2^15, inside fp16, and 2^7
+// farther from its subnormals.
+constexpr float kSlack = 8.0f, kLift = 7.0f;
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __fp16 fp16x4 __attribute__((__vector_size__(8)));
+
+// Sixteen-byte chunks of a key (value) row change places so that the 16-byte
+// reads of 16 rows at one column, and the transposing reads of 8 rows at one
+// 64-byte column, use every bank.
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) {
+  return D == 64 ? (row >> 1) & 7 : row & 15;
+}
+template <int D>
+__device__ __forceinline__ int v_swizzle(int row) {
+  return D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+}
+
+// A tile of 64 rows of keys (values) into LDS, 16 bytes a lane and load; rows
+// past `rows` come out as zeros (the descriptor ends there).
+template <int D, bool KEYS>
+__device__ __forceinline__ void stage(const uint16_t* base, int64_t token_stride, int rows, uint16_t* lds, int wave,
+                                      int lane) {
+  constexpr int C = D / 8;
+  const __amdgpu_buffer_rsrc_t r =
+      buffer_of(base, (uint32_t)(((int64_t)(min(rows, kKeys) - 1) * token_stride + D) * 2));
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    const int c = (j * kWaves + wave) * kWave + lane;
+    const int row = c / C, col = (c % C) ^ (KEYS ? k_swizzle<D>(row) : v_swizzle<D>(row));
+    const uint32_t off = (uint32_t)(row * (int)token_stride * 2 + col * 16);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + (j * kWaves + wave) * kWave * 8), 16, off, 0, 0, 0);
+  }
+}
+
+template <int D, int RB>
+__global__ __launch_bounds__(kWave * kWaves, 1) void prompt_attention_kernel(PromptArgs a) {
+  constexpr int ROWS = kWaves * RB * 32, DT = D / 32, KK = D / 16;
+  __shared__ __align__(16) uint16_t kbuf[2][kKeys * D];
+  __shared__ __align__(16) uint16_t vbuf[2][kKeys * D];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 31, h = lane >> 5;
+  // the last tiles, which see the most keys, come first
+  const int kvh = blockIdx.x % a.heads_kv, item = a.tiles - 1 - blockIdx.x / a.heads_kv;
+  int first = 0, len = a.tokens, tile = item;
+  if (a.starts != nullptr) {
+    const int b = sequence_of_item(a.starts, a.batch, a.group, ROWS, 1, item);
+    if (b < 0) return;
+    first = a.starts[b];
+    tile = item - (first * a.group / ROWS + b);
+    first = max(first, 0);
+    len = min(a.starts[b + 1], a.tokens) - first;
+  }
+  first = __builtin_amdgcn_readfirstlane(first), len = __builtin_amdgcn_readfirstlane(len);
+  const int rows = len * a.group, row0 = tile * ROWS;
+  if (row0 >= rows) return;
+  const int last_token = (min(rows, row0 + ROWS) - 1) / a.group;
+  const int tiles = last_token / kKeys + 1;
+  const int wave_row = row0 + wave * RB * 32;
+  const int wave_first = wave_row / a.group;  // tokens of the wave's first and last row
+  const int wave_last = wave_row < rows ? (min(rows, wave_row + RB * 32) - 1) / a.group : -1;
+
+  f16x8 qf[RB][KK];
+  int seen[RB];  // the last key of the lane's row
+#pragma unroll
+  for (int n = 0; n < RB; ++n) {
+    const int row = wave_row + 32 * n + r;
+    const int t = row / a.group;
+    seen[n] = row < rows ? t : -1;
+    const uint16_t* p = a.q + (int64_t)(first + t) * a.q_token + (int64_t)(kvh * a.group + row - t * a.group) * a.q_head;
+#pragma unroll
+    for (int k = 0; k < KK; ++k) {
+      qf[n][k] = (f16x8)((f16)0.0f);
+      if (row < rows) qf[n][k] = *reinterpret_cast<const f16x8*>(p + 16 * k + 8 * h);
+    }
+  }
+  const uint16_t* kbase = a.k + (int64_t)first * a.k_token + (int64_t)kvh * a.k_head;
+  const uint16_t* vbase = a.v + (int64_t)first * a.v_token + (int64_t)kvh * a.v_head;
+
+  typedef float f32x16_t __attribute__((ext_vector_type(16)));
+  f32x16_t o[RB][DT];
+  float m[RB], l[RB];
+#pragma unroll
+  for (int n = 0; n < RB; ++n) {
+    m[n] = kNoMax, l[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[n][d] = (f32x16_t)(0.0f);
+  }
+
+  stage<D, true>(kbase, a.k_token, len, kbuf[0], wave, lane);
+  stage<D, false>(vbase, a.v_token, len, vbuf[0], wave, lane);
+  for (int kt = 0; kt < tiles; ++kt) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    const int cur = kt & 1;
+    if (kt + 1 < tiles) {
+      const int64_t at = (int64_t)(kt + 1) * kKeys;
+      const int left = len - (kt + 1) * kKeys;
+      stage<D, true>(kbase + at * a.k_token, a.k_token, left, kbuf[cur ^ 1], wave, lane);
+      stage<D, false>(vbase + at * a.v_token, a.v_token, left, vbuf[cur ^ 1], wave, lane);
+    }
+    if (kt * kKeys > wave_last) continue;
+    const uint16_t* kl = kbuf[cur];
+    const uint16_t* vl = vbuf[cur];
+
+    f32x16_t s[RB][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int n = 0; n < RB; ++n) s[n][t] = (f32x16_t)(0.0f);
+#pragma unroll
+      for (int k = 0; k < KK; ++k) {
+        const int row = 32 * t + r;
+        const f16x8 kf =
+            *reinterpret_cast<const f16x8*>(kl + row * D + 8 * ((2 * k + h) ^ k_swizzle<D>(row)));
+#pragma unroll
+        for (int n = 0; n < RB; ++n) s[n][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[n][k], s[n][t], 0, 0, 0);
+      }
+    }
+    f16x8 pf[RB][4];
+#pragma unroll
+    for (int n = 0; n < RB; ++n) {
+      if (kt * kKeys + kKeys - 1 > wave_first) {
+        const int past = seen[n] - kt * kKeys - 4 * h;  // keys of the lane up to here are seen
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * t + 8 * (i >> 2) + (i & 3) > past) s[n][t][i] = -__builtin_inff();
+      }
+      float peak = kNoMax;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) peak = __builtin_fmaxf(peak, s[n][t][i]);
+      peak *= a.scale;
+      if (__any(peak > m[n] + kSlack)) {
+        const float up = __builtin_fmaxf(__builtin_fmaxf(peak, from_lane(peak, lane ^ 32)), m[n]);
+        const float f = __builtin_amdgcn_exp2f(m[n] - up);
+        m[n] = up;
+        l[n] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[n][d] *= f;
+      }
+      const float lift = kLift - m[n];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f(s[n][t][i] * a.scale + lift);
+          l[n] += p;
+          pf[n][2 * t + i / 8][i % 8] = (f16)p;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        f16x8 vf;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int token = 16 * c + 8 * u + 4 * h + ((lane & 15) >> 2);
+          const int chunk = (4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_swizzle<D>(token);
+          const f16x4 x = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+              (__attribute__((address_space(3))) fp16x4*)(vl + token * D + 8 * chunk + 4 * (lane & 1))));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vf[4 * u + i] = x[i];
+        }
+#pragma unroll
+        for (int n = 0; n < RB; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[n][c], o[n][d], 0, 0, 0);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int n = 0; n < RB; ++n) {
+    l[n] += from_lane(l[n], lane ^ 32);
+    const float inv = 1.0f / l[n];
+    const int row = wave_row + 32 * n + r;
+    if (row >= rows) continue;
+    const int t = row / a.group;
+    uint16_t* p = a.out + (int64_t)(first + t) * a.o_token + (int64_t)(kvh * a.group + row - t * a.group) * a.o_head;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        u32x2 w;
+        w[0] = as_u32((f16x2){(f16)(o[n][d][i] * inv), (f16)(o[n][d][i + 1] * inv)});
+        w[1] = as_u32((f16x2){(f16)(o[n][d][i + 2] * inv), (f16)(o[n][d][i + 3] * inv)});
+        *reinterpret_cast<u32x2*>(p + 32 * d + 2 * i + 4 * h) = w;
+      }
+  }
+}
+
+template <int D, int RB>
+int launch(PromptArgs a, hipStream_t st) {
+  constexpr int ROWS = kWaves * RB * 32;
+  const int64_t rows = (int64_t)a.tokens * a.group;
+  // sequence b's tiles are numbered from starts[b] * group / ROWS + b, which leaves room for all of them
+  const int64_t tiles = a.starts ? rows / ROWS + a.batch : (rows + ROWS - 1) / ROWS;
+  if (tiles * a.heads_kv > 0x7fffffff) return LB_ERR_PROB_SHAPE;
+  a.tiles = (int)tiles;
+  prompt_attention_kernel<D, RB><<<dim3((unsigned)(tiles * a.heads_kv)), dim3(kWave * kWaves), 0, st>>>(a);
+  return lbh::launch_status();
+}
+
+}  // namespace
+}  // namespace lb
+
+extern "C" int lb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
+                                   int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v,
+                                   int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens,
+                                   int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv, int64_t head_dim,
+                                   uint16_t* out, int64_t o_token_stride, int64_t o_head_stride, float softmax_scale,
+                                   lb_stream_t stream) {
+  using namespace lb;
+  if (batch < 0 || tokens < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0) return LB_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return LB_ERR_PROB_SHAPE;
+  if (heads_q > 4096 || batch > (1 << 20) || tokens > (1 << 26) || tokens * (heads_q / heads_kv) >= (1ll << 31) - 4096)
+    return LB_ERR_ARG;
+  if (!(softmax_scale > 0.0f) || softmax_scale > 3e38f) return LB_ERR_ARG;
+  if (tokens == 0 || batch == 0) return LB_OK;
+  if (cu_seqlens == nullptr && batch != 1) return LB_ERR_ARG;
+  if (!q || !k || !v || !out) return LB_ERR_ARG;
+  const void* ptrs[] = {q, k, v, out};
+  for (const void* p : ptrs)
+    if (!lbh::aligned(p, 16)) return LB_ERR_ALIGN;
+  if ((q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride | v_head_stride |
+       o_token_stride | o_head_stride) % 8 != 0)
+    return LB_ERR_ALIGN;
+  // a tile's offsets from its first key are 32-bit
+  if (k_token_stride < 0 || v_token_stride < 0 || k_token_stride > (1 << 23) || v_token_stride > (1 << 23))
+    return LB_ERR_ARG;
+  PromptArgs a;
+  a.q = q, a.k = k, a.v = v, a.out = out;
+  a.q_token = q_token_stride, a.q_head = q_head_stride, a.k_token = k_token_stride, a.k_head = k_head_stride;
+  a.v_token = v_token_stride, a.v_head = v_head_stride, a.o_token = o_token_stride, a.o_head = o_head_stride;
+  a.starts = cu_seqlens, a.batch = (int)batch, a.tokens = (int)tokens, a.group = (int)(heads_q / heads_kv);
+  a.heads_kv = (int)heads_kv, a.scale = softmax_scale * kLog2e;
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (head_dim == 64) return launch<64, 2>(a, st);
+  if (head_dim == 128) return launch<128, 2>(a, st);
+  return launch<256, 1>(a, st);
+}

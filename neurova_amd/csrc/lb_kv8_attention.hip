@@ -7,8 +7,8 @@
 // key/value head.  The query heads of a group and the n tokens are the columns
 // of both products, 16 or 32 at a time:
 //
-//   S^T = K Q^T   rows = tokens: the key layout [token][channel] gives a lane
-//                 16 channels of one token in a 16-byte load
+//   S^T = K Q^T   rows = tokens: the key layout [token][channel] holds a lane's
+//                 16 channels of one token together
 //   O^T = V^T P^T rows = channels: the value layout [channel][token] gives a
 //                 lane 16 tokens of one channel in a 16-byte load
 //
@@ -18,6 +18,8 @@
 // weights go from the first product to the second without leaving the lane, and
 // a lane's tokens share a page (pages hold 16 tokens or more), so both scales
 // are one number a lane and step.
+#include <type_traits>
+
 #include "attn_common.hpp"
 
 namespace lb {
@@ -37,18 +39,23 @@ struct AttnArgs {
   int num_pages, page_shift, max_tokens;
   int batch, new_tokens, heads_kv, group;
   int col_blocks;
+  int workers, joined;  // joined: a second launch joins the parts
   float scale;  // softmax scale * log2(e)
 };
 
 constexpr int kStep = 64;           // tokens a wave takes at a time
-constexpr int kWaves = 4;
-constexpr int kUnit = kStep * kWaves;  // tokens of a unit of work
+constexpr int kStreams = 4;            // streams of tokens in a workgroup
+constexpr int kUnit = kStep * kStreams;  // tokens of a unit of work
 constexpr float kNoMax = -1e30f;
 // The running maximum moves only when a score exceeds it by 2^kSlack, and the
 // weights carry 2^kLift more: at most 2^15, inside fp16, and 2^7 farther from its
 // subnormals.
 constexpr float kSlack = 8.0f;
 constexpr int kLift = 7;
+constexpr int kNoExp = -1000;
+constexpr int kMinUnits = 2;
+constexpr int kParts = 4;     // parts whose loads the joining workgroup has in flight
+constexpr int kFewParts = 16;  // up to here the last worker of a pair joins its parts, above a second launch
 
 // Sixteen signed bytes -> two MFMA fragments of eight fp16 (exact): the byte
 // with its sign flipped under the exponent of 1024 is 1024 + 128 + c.
@@ -69,149 +76,396 @@ __device__ __forceinline__ void codes_to_half(u32x4 w, f16x8& a, f16x8& b) {
 
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnit - 1) / kUnit : 1; }
 
-__device__ __forceinline__ int wave_sum_int(int v) {
-  const int lane = lane_id();
-#pragma unroll
-  for (int x = 1; x < kWave; x *= 2) v += (int)from_lane((uint32_t)v, lane ^ x);
-  return v;
-}
+// Head dimension 256 is two waves of 128 channels for each stream of tokens (the
+// registers of all 256 would leave one wave a SIMD): each sums the scores over
+// its half, the halves are exchanged through LDS, and both carry the same
+// softmax for their half of the output.
+template <int D>
+constexpr int kHalves = D == 256 ? 2 : 1;
+template <int D>
+constexpr int kThreads = kWave * kStreams * kHalves<D>;
+
+// Workgroups of a compute unit: two waves a SIMD where the registers allow it.
+template <int D, int NQ>
+constexpr int kPerCu = D * NQ <= 128 ? 2 : 1;
 
 template <int D, int NQ>
 struct Shared {
   static constexpr int kCols = 16 * NQ;
-  float o[kWaves][kCols][D + 4];
-  float m[kWaves][kCols], l[kWaves][kCols];
+  union {
+    float o[kStreams][kCols][D + 4];
+    f32x4 s[kHalves<D>][kStreams][kHalves<D>][NQ * 4][kHalves<D> == 2 ? kWave : 1];  // partial scores, two steps of them
+  };
+  float m[kStreams][kCols], l[kStreams][kCols];
   int last;
 };
+
+// How a launch's work is cut.  A pair (sequence, key/value head, column block)
+// has `nu` units.  With many pairs the workgroups take equal contiguous ranges
+// of all units, numbered pair by pair, so one may end a pair and begin the
+// next.  With few pairs each is cut into slots of its own, `per` units or a
+// little less, one a workgroup: the fixed time of a segment (its first loads,
+// the join) is then paid once.
+struct Work {
+  int units, per;
+  bool slots;
+};
+
+__device__ __forceinline__ int len_at(const AttnArgs& a, int b) {
+  return b < a.batch ? max(min(a.seq_lens[b], a.max_tokens), 0) : -1;
+}
+// Units of a sequence's pairs; 0 past the batch (length -1).
+__device__ __forceinline__ int units_or_none(int len) { return len < 0 ? 0 : units_of(len); }
+
+__device__ __forceinline__ Work work_of(const AttnArgs& a, int first_len) {
+  int total = __builtin_amdgcn_readlane(wave_scan(units_or_none(first_len)), kWave - 1);
+  for (int c = kWave; c < a.batch; c += kWave)
+    total += __builtin_amdgcn_readlane(wave_scan(units_or_none(len_at(a, c + lane_id()))), kWave - 1);
+  const int pairs = a.batch * a.heads_kv * a.col_blocks;
+  Work w;
+  w.units = total * a.heads_kv * a.col_blocks;
+  w.slots = 4 * pairs <= a.workers;
+  // slots of `per` units: at most units / per + pairs of them, which is no more than the workers
+  const int among = w.slots ? a.workers - pairs : a.workers;
+  w.per = max((w.units + among - 1) / among, kMinUnits);
+  return w;
+}
 
 // One (sequence, key/value head, column block) over units [u0, u1) of its nu.
 struct Segment {
   int b, head, cb, u0, u1, nu, len;
-  int first_unit;  // of the whole pair, in the launch's numbering
+  int w_first, w_last;  // the workers of the whole pair
   int pair;
 };
 
-template <int D, int NQ>
-__device__ __forceinline__ void run_segment(const AttnArgs& a, const Segment& sg, int worker, int per_worker,
-                                            Shared<D, NQ>& sh) {
-  constexpr int KI = D / 64, VT = D / 16, COLS = 16 * NQ;
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int r = lane & 15, g = lane >> 4;
-  const int len = sg.len, cols = a.new_tokens * a.group;
-  const int t_begin = sg.u0 * kUnit, t_end = min(len, sg.u1 * kUnit);
-  const int32_t* table = a.page_table + (int64_t)sg.b * a.table_stride;
-  const int page_tokens = 1 << a.page_shift;
+// Four channels of an output row, divided by the sum of the weights (a row that
+// saw no key is zero).
+__device__ __forceinline__ void store_out(const AttnArgs& a, int b, int head, int col, int d, f32x4 x, float sum) {
+  const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+  const int i = col / a.group;
+  uint16_t* row = a.out + ((int64_t)b * a.new_tokens + i) * a.o_token +
+                  (int64_t)(head * a.group + (col - i * a.group)) * a.o_head + d;
+  u32x2 w;
+  w[0] = as_u32((f16x2){(f16)(x[0] * inv), (f16)(x[1] * inv)});
+  w[1] = as_u32((f16x2){(f16)(x[2] * inv), (f16)(x[3] * inv)});
+  *reinterpret_cast<u32x2*>(row) = w;
+}
 
-  // the query fragments, in the channel order of the key loads
+// A part: the columns' maxima, their sums, then o [column][channel].
+template <int D, int NQ>
+constexpr int kPartFloats = 16 * NQ * (D + 2);
+
+// Worker w's part of a pair that begins with worker w_first: its first if the
+// pair began before it, else its second (a pair that ends after it).
+template <int D, int NQ>
+__device__ __forceinline__ int64_t part_at(int w, int w_first) {
+  return ((int64_t)w * 2 + (w > w_first ? 0 : 1)) * kPartFloats<D, NQ>;
+}
+
+// The segments of a worker, in order.
+struct Segments {
+  Work work;
+  int worker, pairs;  // pairs of a sequence
+  int u, u_end;       // position: in units, or with slots in slots
+  int chunk, at, base;  // sequence chunk + at, which begins at position base
+  int lens;             // lengths of the 64 sequences from chunk on
+
+  __device__ __forceinline__ bool begin(const AttnArgs& a) {
+    const int lane = lane_id();
+    pairs = a.heads_kv * a.col_blocks;
+    lens = len_at(a, lane);
+    work = work_of(a, lens);
+    worker = blockIdx.x;
+    u = work.slots ? worker : worker * work.per;
+    u_end = 0, chunk = 0, base = 0;
+    int size, upto;
+    for (;;) {
+      const int nu = units_or_none(lens);
+      size = (work.slots ? (nu + work.per - 1) / work.per : nu) * pairs;
+      upto = wave_scan(size);
+      const int all = __builtin_amdgcn_readlane(upto, kWave - 1);
+      if (base + all > u) break;
+      base += all, chunk += kWave;
+      if (chunk >= a.batch) return false;
+      lens = len_at(a, chunk + lane);
+    }
+    at = __builtin_ctzll(__ballot(base + upto > u));  // the sequence that holds u
+    base += __builtin_amdgcn_readlane(upto - size, at);
+    u_end = work.slots ? u + 1 : min(work.units, u + work.per);
+    return true;
+  }
+
+  __device__ __forceinline__ bool next(const AttnArgs& a, Segment& sg) {
+    if (u >= u_end) return false;
+    const int len = __builtin_amdgcn_readlane(lens, at), nu = units_of(len);
+    const int slots = work.slots ? (nu + work.per - 1) / work.per : nu;
+    const int x = (u - base) / slots, first = base + x * slots;
+    sg.b = chunk + at, sg.nu = nu, sg.len = len;
+    sg.head = x / a.col_blocks, sg.cb = x - sg.head * a.col_blocks;
+    sg.pair = sg.b * pairs + x;
+    if (work.slots) {
+      const int i = u - first;
+      sg.u0 = nu * i / slots, sg.u1 = nu * (i + 1) / slots;  // nu <= 2^20, slots <= workers
+      sg.w_first = first, sg.w_last = first + slots - 1;
+      u = u_end;
+    } else {
+      sg.u0 = u - first, sg.u1 = min(nu, u_end - first);
+      sg.w_first = first / work.per, sg.w_last = (first + nu - 1) / work.per;
+      u = first + sg.u1;
+      if (u < u_end && x == pairs - 1 && sg.u1 == nu) {  // on to the next sequence
+        base += nu * pairs;
+        if (++at == kWave) at = 0, chunk += kWave, lens = len_at(a, chunk + lane_id());
+      }
+    }
+    return true;
+  }
+};
+
+// A wave's walk over the steps of its worker's segments, with the loads of one
+// step ahead: the registers that a product has read are loaded for the next
+// step at once, also across the end of a segment, so that its join runs while
+// the next segment's first keys and values are on their way.  ONCE: the pair has
+// one column block, so its keys and values are read once and need no place in
+// the caches (64 sequences of 2000 to 4000 tokens, 8 heads of 128: 84 us against
+// 77; with two column blocks the second one's reads would miss: 27 against 30).
+template <int D, int NQ, bool ONCE>
+struct Walk {
+  static constexpr int H = kHalves<D>, DW = D / H, KI = DW / 64, VT = DW / 16, COLS = 16 * NQ;
+  const AttnArgs& a;
+  Shared<D, NQ>& sh;
+  int lane, r, g, stream, half;
+  // the step whose keys and values are loaded, or on their way
+  const int8_t* vp;
+  int cell;  // page and head of the lane's own 16 tokens
+  float ks, vs;
+  bool held;
+  u32x4 vw[VT];
+  uint8_t* keys;        // this wave's keys of a step in LDS
+  uint32_t k_off[4];    // the lane's place in a load of 16-token group i
+  const int8_t* k_base[4];  // where the groups' keys are
+  int pv;               // page number of the lane's own 16 tokens in the step after
+  bool loaded, pages_known;
   f16x8 qf[NQ][2 * KI];
-  int limit[NQ];  // tokens the lane's column sees
+  int limit[NQ];  // keys that the lane's columns see
+  int flip;       // which of the two score buffers
+
+  __device__ __forceinline__ Walk(const AttnArgs& args, Shared<D, NQ>& shared, uint8_t* lds) : a(args), sh(shared) {
+    lane = lane_id(), r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    stream = wave % kStreams, half = H == 1 ? 0 : wave / kStreams;
+    loaded = pages_known = false, flip = 0, pv = -1;
+    keys = lds + wave * kStep * DW;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int col = sg.cb * COLS + 16 * n + r;
-    const int i = col / a.group;
-    limit[n] = col < cols ? len - a.new_tokens + i + 1 : 0;
-    const uint16_t* row = a.q + ((int64_t)sg.b * a.new_tokens + i) * a.q_token +
-                          (int64_t)(sg.head * a.group + (col - i * a.group)) * a.q_head;
+    for (int i = 0; i < 4; ++i)
+      k_off[i] = DW == 64 ? (lane >> 2) * D + ((lane & 3) ^ i) * 16
+                          : (lane >> 3) * D + ((lane & 7) ^ (2 * i + ((lane >> 4) & 1))) * 16;
+  }
+  __device__ __forceinline__ int first_token(const Segment& sg) const { return sg.u0 * kUnit + stream * kStep; }
+  __device__ __forceinline__ static int end_token(const Segment& sg) { return min(sg.len, sg.u1 * kUnit); }
+
+  // Page numbers of the step of sequence b at token tb.  No branch around the
+  // load (a token past the end reads the last one's): the waits inside the loop
+  // over the steps count the loads between.
+  __device__ __forceinline__ void fetch_pages(int b, int len, int tb) {
+    pv = a.page_table[(int64_t)b * a.table_stride + (min(tb + 16 * g, len - 1) >> a.page_shift)];
+  }
+  __device__ __forceinline__ void resolve(const Segment& sg, int tb) {
+    const int tv = tb + 16 * g, mask = (1 << a.page_shift) - 1;
+    held = tv < sg.len && (unsigned)pv < (unsigned)a.num_pages;
+    const int page = held ? pv : 0;
+    cell = page * a.heads_kv + sg.head;
+    const int64_t cv = cell;
+    vp = a.v_cache + ((cv * D + half * DW + r) << a.page_shift) + (tv & mask);
 #pragma unroll
-    for (int k = 0; k < 2 * KI; ++k) {
-      qf[n][k] = (f16x8)((f16)0.0f);
-      if (col < cols) qf[n][k] = *reinterpret_cast<const f16x8*>(row + 64 * (k / 2) + 16 * g + 8 * (k & 1));
+    for (int i = 0; i < 4; ++i) {
+      const int64_t ck = (int64_t)__builtin_amdgcn_readlane(page, 16 * i) * a.heads_kv + sg.head;
+      k_base[i] = a.k_cache + ((ck << a.page_shift) + ((tb + 16 * i) & mask)) * D + half * DW;
     }
   }
-
-  // the largest value scale of the segment: the weights p * v_scale enter the
-  // second product relative to it, as the sum of two fp16 numbers (one alone
-  // would add as much error as the rounding of the output; the matrix cores are
-  // idle most of the time here)
-  float top = 0.0f;
-  for (int p = (t_begin >> a.page_shift) + lane; p < (t_end + page_tokens - 1) >> a.page_shift; p += kWave) {
-    const int id = table[p];
-    if ((unsigned)id < (unsigned)a.num_pages) top = __builtin_fmaxf(top, a.v_scale[(int64_t)id * a.heads_kv + sg.head]);
+  __device__ __forceinline__ void load_scales() { ks = a.k_scale[cell], vs = a.v_scale[cell]; }
+  // Keys of a step go through LDS: a load of 1 KB takes whole cache lines, which
+  // the first product's operand (one token a lane) would touch one lane at a
+  // time, a quarter of the first-level cache's rate.  Chunks of 16 bytes change
+  // places inside a row so that the reads of a product's 16 tokens use every bank.
+  __device__ __forceinline__ void load_k() {
+    typedef __attribute__((address_space(3))) void lds_void;
+    constexpr int N = DW / 64;  // loads of a group of 16 tokens
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) {
+      const __amdgpu_buffer_rsrc_t from = buffer_of(k_base[i / N], 16 * D - half * DW);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)(keys + i * 1024), 16, k_off[i / N], (i % N) * 8 * D, 0, ONCE ? kNonTemporal : 0);
+    }
   }
+  __device__ __forceinline__ u32x4 read_k(int t, int i) const {
+    const int token = 16 * (r >> 2) + 4 * t + (r & 3), chunk = g + 4 * i;
+    const int swz = DW == 64 ? token >> 4 : 2 * (token >> 4) + ((token >> 1) & 1);
+    return *reinterpret_cast<const u32x4*>(keys + token * DW + (chunk ^ swz) * 16);
+  }
+  __device__ __forceinline__ void load_v(int d) {
+    const u32x4* from = reinterpret_cast<const u32x4*>(vp + ((int64_t)(16 * d) << a.page_shift));
+    vw[d] = ONCE ? __builtin_nontemporal_load(from) : *from;
+  }
+  // The query fragments, in the channel order of the key loads.
+  __device__ __forceinline__ void load_q(const Segment& sg) {
+    const int cols = a.new_tokens * a.group;
 #pragma unroll
-  for (int x = 1; x < kWave; x *= 2) top = __builtin_fmaxf(top, from_lane(top, lane ^ x));
-  const int top_exp = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;
-
-  f32x4 o[NQ][VT];
-  float m[NQ], l[NQ];
+    for (int n = 0; n < NQ; ++n) {
+      const int col = sg.cb * COLS + 16 * n + r;
+      const int i = col / a.group;
+      limit[n] = col < cols ? sg.len - a.new_tokens + i + 1 : 0;
+      const uint16_t* row = a.q + ((int64_t)sg.b * a.new_tokens + i) * a.q_token +
+                            (int64_t)(sg.head * a.group + (col - i * a.group)) * a.q_head + half * DW + 16 * g;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    m[n] = kNoMax, l[n] = 0.0f;
+      for (int k = 0; k < 2 * KI; ++k) {
+        qf[n][k] = (f16x8)((f16)0.0f);
+        if (col < cols) qf[n][k] = *reinterpret_cast<const f16x8*>(row + 64 * (k / 2) + 8 * (k & 1));
+      }
+    }
+  }
+  __device__ __forceinline__ static int steps_from(int tb, int end) { return tb < end ? (end - tb + kUnit - 1) / kUnit : 0; }
+  // The pages of the step after the next one, at token tp of sg or past its end,
+  // where that is known by now: in `to`, if it follows.
+  __device__ __forceinline__ void fetch_after(const Segment& sg, int tp, bool ahead, const Segment& to) {
+    const bool inside = tp < end_token(sg);
+    const bool beyond = !inside && ahead && first_token(to) < end_token(to);
+    pages_known = inside || beyond;
+    fetch_pages(beyond ? to.b : sg.b, beyond ? to.len : sg.len, inside ? tp : beyond ? first_token(to) : 0);
+  }
+  // Loads of a step that nothing was loaded ahead of.
+  __device__ __forceinline__ void start(const Segment& sg, bool ahead, const Segment& to) {
+    const int tb = first_token(sg);
+    if (loaded || tb >= end_token(sg)) return;
+    if (!pages_known) fetch_pages(sg.b, sg.len, tb);
+    resolve(sg, tb);
+    fetch_after(sg, tb + kUnit, ahead, to);
+    load_k();
+    load_scales();
 #pragma unroll
-    for (int d = 0; d < VT; ++d) o[n][d] = (f32x4)(0.0f);
+    for (int d = 0; d < VT; ++d) load_v(d);
+    loaded = true;
   }
 
-  for (int tb = t_begin + wave * kStep; tb < t_end; tb += kUnit) {
-    // pages: the lane's own 16 tokens, and those of the key rows it loads
-    const int tv = tb + 16 * g, tk = tb + 16 * (r >> 2);
-    int pv = tv < len ? table[tv >> a.page_shift] : -1;
-    int pk = tk < len ? table[tk >> a.page_shift] : -1;
-    const bool held = (unsigned)pv < (unsigned)a.num_pages;
-    if (!held) pv = 0;
-    if ((unsigned)pk >= (unsigned)a.num_pages) pk = 0;
-    const int64_t cv = (int64_t)pv * a.heads_kv + sg.head, ck = (int64_t)pk * a.heads_kv + sg.head;
-    const float ks = held ? a.k_scale[cv] * a.scale : 0.0f;
-    const float vs = held ? __builtin_amdgcn_ldexpf(a.v_scale[cv], kLift - top_exp) : 0.0f;
-    const int8_t* kp = a.k_cache + ((ck << a.page_shift) + ((tk + (r & 3)) & (page_tokens - 1))) * D + 16 * g;
-    const int8_t* vp = a.v_cache + ((cv * D + r) << a.page_shift) + (tv & (page_tokens - 1));
-    u32x4 kw[4][KI], vw[VT];
+  // One step of segment sg at token tb: the last of the segment or (LAST false)
+  // not; with MORE another one follows, in sg or in `to`.
+  template <bool MORE, bool LAST>
+  __device__ __forceinline__ void step(const Segment& sg, int tb, f32x4 (&o)[NQ][VT], float (&m)[NQ], float (&l)[NQ],
+                                       int& e, bool ahead, const Segment& to) {
+    const bool held0 = held;
+    u32x4 kw[4][KI];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int i = 0; i < KI; ++i) kw[t][i] = *reinterpret_cast<const u32x4*>(kp + t * 4 * D + i * 64);
-#pragma unroll
-    for (int d = 0; d < VT; ++d) vw[d] = *reinterpret_cast<const u32x4*>(vp + ((int64_t)(16 * d) << a.page_shift));
-
-    f32x4 s[NQ][4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) s[n][t] = (f32x4)(0.0f);
-#pragma unroll
-      for (int i = 0; i < KI; ++i) {
-        f16x8 x, y;
-        codes_to_half(kw[t][i], x, y);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qf[n][2 * i], s[n][t], 0, 0, 0);
-          s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, qf[n][2 * i + 1], s[n][t], 0, 0, 0);
-        }
+      for (int i = 0; i < KI; ++i) kw[t][i] = read_k(t, i);
+    if (MORE) {
+      if (LAST) {
+        if (!pages_known) fetch_pages(to.b, to.len, first_token(to));
+        resolve(to, first_token(to));
+        fetch_after(to, first_token(to) + kUnit, false, to);
+      } else {
+        resolve(sg, tb + kUnit);
+        fetch_after(sg, tb + 2 * kUnit, ahead, to);
       }
+      // the reads above are done: the next keys may take their place
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      load_k();
     }
-    f16x8 pf[NQ][2], pl[NQ][2];
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 s[NQ][4];
+    // two products at a time, each in two sums: four independent chains of MFMAs
+#pragma unroll
+    for (int t = 0; t < 4; t += 2) {
+      f32x4 odd[NQ][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) s[n][t] = s[n][t + 1] = odd[n][0] = odd[n][1] = (f32x4)(0.0f);
+#pragma unroll
+      for (int i = 0; i < KI; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          f16x8 x, y;
+          codes_to_half(kw[t + u][i], x, y);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            s[n][t + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qf[n][2 * i], s[n][t + u], 0, 0, 0);
+            odd[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, qf[n][2 * i + 1], odd[n][u], 0, 0, 0);
+          }
+        }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) s[n][t] += odd[n][0], s[n][t + 1] += odd[n][1];
+    }
+    if (H == 2) {
+      // a step's buffer is written again two steps later, behind the barrier
+      // that the partner reaches after its reads
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sh.s[flip][stream][half][4 * n + t][lane] = s[n][t];
+      lds_barrier();
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[n][t] += sh.s[flip][stream][half ^ 1][4 * n + t][lane];
+      flip ^= 1;
+    }
+    const int tv = tb + 16 * g;
+    const float kscale = held0 ? ks * a.scale : 0.0f;
+    // the exponent of the value scale; a page of zeros, or none, has the lowest
+    const int ve = held0 && vs > 0.0f ? __builtin_amdgcn_frexp_expf(vs) : kNoExp;
+    const bool mask = tb + kStep > sg.len - a.new_tokens + 1 || __any(!held0);
+    float peak[NQ];
+    bool up = ve > e;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      float peak = kNoMax;
+      peak[n] = kNoMax;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float x = s[n][t][i] * ks;
-          if (!held || tv + 4 * t + i >= limit[n]) x = -__builtin_inff();
+          float x = s[n][t][i] * kscale;
+          if (mask && (!held0 || tv + 4 * t + i >= limit[n])) x = -__builtin_inff();
           s[n][t][i] = x;
-          peak = __builtin_fmaxf(peak, x);
+          peak[n] = __builtin_fmaxf(peak[n], x);
         }
-      if (__any(peak > m[n] + kSlack)) {
-        peak = __builtin_fmaxf(peak, from_lane(peak, lane ^ 16));
-        peak = __builtin_fmaxf(peak, from_lane(peak, lane ^ 32));
-        const float up = __builtin_fmaxf(peak, m[n]);
-        const float f = __builtin_amdgcn_exp2f(m[n] - up);
-        m[n] = up;
-        l[n] *= f;
+      up |= peak[n] > m[n] + kSlack;
+    }
+    if (__any(up)) {
+      int top = max(ve, e);
+      top = max(top, (int)from_lane((uint32_t)top, lane ^ 16));
+      top = max(top, (int)from_lane((uint32_t)top, lane ^ 32));
+      const int down = max(e - top, -300);
+      e = top;
 #pragma unroll
-        for (int d = 0; d < VT; ++d) o[n][d] *= f;
+      for (int n = 0; n < NQ; ++n) {
+        float x = __builtin_fmaxf(peak[n], m[n]);
+        x = __builtin_fmaxf(x, from_lane(x, lane ^ 16));
+        x = __builtin_fmaxf(x, from_lane(x, lane ^ 32));
+        const float f = __builtin_amdgcn_exp2f(m[n] - x);
+        m[n] = x;
+        l[n] *= f;
+        const float fo = __builtin_amdgcn_ldexpf(f, down);
+#pragma unroll
+        for (int d = 0; d < VT; ++d) o[n][d] *= fo;
       }
+    }
+    // the weights p * v_scale enter the second product relative to the largest
+    // scale, as the sum of two fp16 numbers (one alone would add as much error
+    // as the rounding of the output; the matrix cores are mostly idle here)
+    const float vscale = held0 ? __builtin_amdgcn_ldexpf(vs, kLift - e) : 0.0f;
+    f16x8 pf[NQ][2], pl[NQ][2];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float p = __builtin_amdgcn_exp2f(s[n][2 * f + j / 4][j % 4] - m[n]);
           l[n] += p;
-          const float w = p * vs;
+          const float w = p * vscale;
           pf[n][f][j] = (f16)w;
           pl[n][f][j] = (f16)(w - (float)(f16)w);
         }
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (MORE) load_scales();
 #pragma unroll
     for (int d = 0; d < VT; ++d) {
       f16x8 x, y;
@@ -223,163 +477,220 @@ __device__ __forceinline__ void run_segment(const AttnArgs& a, const Segment& sg
         o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[n][0], o[n][d], 0, 0, 0);
         o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl[n][1], o[n][d], 0, 0, 0);
       }
+      if (MORE) load_v(d);
+      if ((d & 3) == 3) __builtin_amdgcn_sched_barrier(0);
     }
+    loaded = MORE;
   }
 
-  // the four waves' states -> one
+  // All steps of segment sg, and its join; `ahead`: segment `to` follows.
+  __device__ __forceinline__ void run(const Segment& sg, bool ahead, const Segment& to, int worker) {
+    f32x4 o[NQ][VT];
+    float m[NQ], l[NQ];
+    int e = kNoExp;  // o is relative to 2^(e - kLift), the largest value scale met
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    l[n] += from_lane(l[n], lane ^ 16);
-    l[n] += from_lane(l[n], lane ^ 32);
-    if (g == 0) sh.m[wave][16 * n + r] = m[n], sh.l[wave][16 * n + r] = l[n];
-  }
-  __syncthreads();
+    for (int n = 0; n < NQ; ++n) {
+      m[n] = kNoMax, l[n] = 0.0f;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int c = 16 * n + r;
-    float up = kNoMax;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) up = __builtin_fmaxf(up, sh.m[w][c]);
-    const float f = __builtin_amdgcn_exp2f(m[n] - up);
-#pragma unroll
-    for (int d = 0; d < VT; ++d) *reinterpret_cast<f32x4*>(&sh.o[wave][c][16 * d + 4 * g]) = o[n][d] * f;
-  }
-  __syncthreads();
-
-  const bool whole = sg.u0 == 0 && sg.u1 == sg.nu;
-  const int live = min(COLS, cols - sg.cb * COLS);  // columns of this block that exist
-  // a worker's part of a pair that starts before its range, or of one that ends after it
-  const int part_floats = COLS * (D + 2);
-  float* part = a.parts + ((int64_t)worker * 2 + (sg.u0 > 0 ? 0 : 1)) * part_floats;
-  for (int e = threadIdx.x; e < live * (D / 4); e += kWave * kWaves) {
-    const int c = e / (D / 4), d = 4 * (e % (D / 4));
-    float up = kNoMax, sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) up = __builtin_fmaxf(up, sh.m[w][c]);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += sh.l[w][c] * __builtin_amdgcn_exp2f(sh.m[w][c] - up);
-    f32x4 x = (f32x4)(0.0f);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) x += *reinterpret_cast<const f32x4*>(&sh.o[w][c][d]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], top_exp - kLift);
-    if (whole) {
-      const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-      const int col = sg.cb * COLS + c, i = col / a.group;
-      uint16_t* row = a.out + ((int64_t)sg.b * a.new_tokens + i) * a.o_token +
-                      (int64_t)(sg.head * a.group + (col - i * a.group)) * a.o_head + d;
-      u32x2 w;
-      w[0] = as_u32((f16x2){(f16)(x[0] * inv), (f16)(x[1] * inv)});
-      w[1] = as_u32((f16x2){(f16)(x[2] * inv), (f16)(x[3] * inv)});
-      *reinterpret_cast<u32x2*>(row) = w;
-    } else {
-      if (d == 0) publish(part + c, up), publish(part + COLS + c, sum);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) publish(part + 2 * COLS + c * D + d + i, x[i]);
+      for (int d = 0; d < VT; ++d) o[n][d] = (f32x4)(0.0f);
     }
-  }
-  if (whole) {
-    __syncthreads();  // the next segment writes the shared states again
-    return;
-  }
-  // the last of the pair's workers to arrive joins the parts, in worker order
-  const int w_first = sg.first_unit / per_worker, w_last = (sg.first_unit + sg.nu - 1) / per_worker;
-  wait_published();
-  __syncthreads();
-  if (threadIdx.x == 0) sh.last = arrive(a.counters + sg.pair) == w_last - w_first;
-  __syncthreads();
-  if (sh.last) {
-    after_last_arrival();
-    for (int e = threadIdx.x; e < live * (D / 4); e += kWave * kWaves) {
-      const int c = e / (D / 4), d = 4 * (e % (D / 4));
+    start(sg, ahead, to);
+    const int end = end_token(sg);
+    int tb = first_token(sg);
+    for (; tb + kUnit < end; tb += kUnit) step<true, false>(sg, tb, o, m, l, e, ahead, to);
+    if (tb < end) {
+      if (ahead && first_token(to) < end_token(to)) step<true, true>(sg, tb, o, m, l, e, ahead, to);
+      else step<false, true>(sg, tb, o, m, l, e, ahead, to);
+    }
+    // a round of steps in which this stream has none: its barrier all the same
+    if (H == 2 && end > sg.u0 * kUnit && steps_from(first_token(sg), end) < steps_from(sg.u0 * kUnit, end)) lds_barrier();
+    if (ahead) load_q(to);
+
+    // the streams' states -> one
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      l[n] += from_lane(l[n], lane ^ 16);
+      l[n] += from_lane(l[n], lane ^ 32);
+      if (g == 0 && half == 0) sh.m[stream][16 * n + r] = m[n], sh.l[stream][16 * n + r] = l[n];
+    }
+    lds_barrier();
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int c = 16 * n + r;
+      float up = kNoMax;
+#pragma unroll
+      for (int w = 0; w < kStreams; ++w) up = __builtin_fmaxf(up, sh.m[w][c]);
+      const float f = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(m[n] - up), max(e, -300) - kLift);
+#pragma unroll
+      for (int d = 0; d < VT; ++d)
+        *reinterpret_cast<f32x4*>(&sh.o[stream][c][half * DW + 16 * d + 4 * g]) = o[n][d] * f;
+    }
+    lds_barrier();
+
+    const bool whole = sg.u0 == 0 && sg.u1 == sg.nu;
+    const int cols = a.new_tokens * a.group;
+    const int live = min(COLS, cols - sg.cb * COLS);  // columns of this block that exist
+    float* part = a.parts + part_at<D, NQ>(worker, sg.w_first);
+    const __amdgpu_buffer_rsrc_t dst = buffer_of(part, kPartFloats<D, NQ> * 4);
+    for (int x = threadIdx.x; x < live * (D / 4); x += kThreads<D>) {
+      const int c = x / (D / 4), d = 4 * (x % (D / 4));
       float up = kNoMax, sum = 0.0f;
-      f32x4 x = (f32x4)(0.0f);
-      for (int w = w_first; w <= w_last; ++w) {
-        const bool starts_before = w * per_worker > sg.first_unit;
-        const float* src = a.parts + ((int64_t)w * 2 + (starts_before ? 0 : 1)) * part_floats;
-        const float pm = collect(src + c), pl = collect(src + COLS + c);
-        f32x4 y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = collect(src + 2 * COLS + c * D + d + i);
-        const float to = __builtin_fmaxf(up, pm);
-        const float fx = __builtin_amdgcn_exp2f(up - to), fy = __builtin_amdgcn_exp2f(pm - to);
-        up = to;
-        sum = sum * fx + pl * fy;
-        x = x * fx + y * fy;
+      for (int w = 0; w < kStreams; ++w) up = __builtin_fmaxf(up, sh.m[w][c]);
+#pragma unroll
+      for (int w = 0; w < kStreams; ++w) sum += sh.l[w][c] * __builtin_amdgcn_exp2f(sh.m[w][c] - up);
+      f32x4 v = (f32x4)(0.0f);
+#pragma unroll
+      for (int w = 0; w < kStreams; ++w) v += *reinterpret_cast<const f32x4*>(&sh.o[w][c][d]);
+      if (whole) {
+        store_out(a, sg.b, sg.head, sg.cb * COLS + c, d, v, sum);
+      } else {
+        if (d == 0) publish(part + c, up), publish(part + COLS + c, sum);
+        publish16(dst, (2 * COLS + c * D + d) * 4, v);
       }
-      const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-      const int col = sg.cb * COLS + c, i = col / a.group;
-      uint16_t* row = a.out + ((int64_t)sg.b * a.new_tokens + i) * a.o_token +
-                      (int64_t)(sg.head * a.group + (col - i * a.group)) * a.o_head + d;
-      u32x2 wd;
-      wd[0] = as_u32((f16x2){(f16)(x[0] * inv), (f16)(x[1] * inv)});
-      wd[1] = as_u32((f16x2){(f16)(x[2] * inv), (f16)(x[3] * inv)});
-      *reinterpret_cast<u32x2*>(row) = wd;
+    }
+    if (whole || a.joined) {
+      lds_barrier();  // the next segment writes the shared states again
+      return;
+    }
+    // the last of the pair's workers to arrive joins the parts, in worker order
+    wait_published();
+    __syncthreads();
+    if (threadIdx.x == 0) sh.last = arrive(a.counters + sg.pair) == sg.w_last - sg.w_first;
+    __syncthreads();
+    if (sh.last) join(sg, live);
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ void join(const Segment& sg, int live) {
+    after_last_arrival();
+    for (int x0 = threadIdx.x; x0 < live * (D / 4); x0 += 2 * kThreads<D>) {
+      // two columns and channels a thread, kParts parts each: all their loads in flight
+      float up[2] = {kNoMax, kNoMax}, sum[2] = {0.0f, 0.0f};
+      f32x4 v[2] = {(f32x4)(0.0f), (f32x4)(0.0f)};
+      const bool both = x0 + kThreads<D> < live * (D / 4);
+      for (int w0 = sg.w_first; w0 <= sg.w_last; w0 += kParts) {
+        float pm[2][kParts], pl[2][kParts];
+        f32x4 po[2][kParts];
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            pm[j][i] = kNoMax, pl[j][i] = 0.0f, po[j][i] = (f32x4)(0.0f);
+            if (w0 + i <= sg.w_last) {
+              const int x = both ? x0 + j * kThreads<D> : x0;
+              const int c = x / (D / 4), d = 4 * (x % (D / 4));
+              const __amdgpu_buffer_rsrc_t from =
+                  buffer_of(a.parts + part_at<D, NQ>(w0 + i, sg.w_first), kPartFloats<D, NQ> * 4);
+              pm[j][i] = collect4(from, c * 4);
+              pl[j][i] = collect4(from, (COLS + c) * 4);
+              po[j][i] = collect16(from, (2 * COLS + c * D + d) * 4);
+            }
+          }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = up[j];
+#pragma unroll
+          for (int i = 0; i < kParts; ++i) top = __builtin_fmaxf(top, pm[j][i]);
+          const float f0 = __builtin_amdgcn_exp2f(up[j] - top);
+          up[j] = top, sum[j] *= f0, v[j] *= f0;
+#pragma unroll
+          for (int i = 0; i < kParts; ++i) {
+            const float f = __builtin_amdgcn_exp2f(pm[j][i] - top);
+            sum[j] += pl[j][i] * f, v[j] += po[j][i] * f;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int x = x0 + j * kThreads<D>;
+        if (j == 0 || both) store_out(a, sg.b, sg.head, sg.cb * COLS + x / (D / 4), 4 * (x % (D / 4)), v[j], sum[j]);
+      }
     }
     if (threadIdx.x == 0) reset_counter(a.counters + sg.pair);
   }
-  __syncthreads();
+};
+
+template <int D, int NQ, bool ONCE>
+__global__ __launch_bounds__(kThreads<D>, (kPerCu<D, NQ>)) void kv8_attention_kernel(AttnArgs a) {
+  __shared__ Shared<D, NQ> sh;
+  __shared__ __align__(16) uint8_t keys[kStreams * kStep * D];
+  Segments segments;
+  if (!segments.begin(a)) return;
+  Segment cur, to;
+  bool have = segments.next(a, cur);
+  Walk<D, NQ, ONCE> walk(a, sh, keys);
+  if (have) {
+    walk.start(cur, false, cur);
+    walk.load_q(cur);
+  }
+  while (have) {
+    have = segments.next(a, to);
+    walk.run(cur, have, to, segments.worker);
+    cur = to;
+  }
 }
 
-// The launch's units, 256 tokens each, are numbered sequence by sequence, head
-// by head, column block by column block; each workgroup takes an equal
-// contiguous range of them, so ragged batches and single long sequences fill
-// the chip alike.
+// Joins the parts of the pairs that several workers share, one column of one
+// pair a workgroup: D / 4 threads a part, the parts dealt to the thread groups
+// in turn and their sums added in group order.
 template <int D, int NQ>
-__global__ __launch_bounds__(kWave * kWaves) void kv8_attention_kernel(AttnArgs a) {
-  __shared__ Shared<D, NQ> sh;
-  const int lane = lane_id();
+__global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs a) {
+  constexpr int COLS = 16 * NQ, T = D / 4, GROUPS = 256 / T;
+  __shared__ float sm[GROUPS], sl[GROUPS];
+  __shared__ f32x4 so[GROUPS][T];
   const int pairs = a.heads_kv * a.col_blocks;
-  int total = 0;
-  for (int c = 0; c < a.batch; c += kWave)
-    if (c + lane < a.batch) total += units_of(min(a.seq_lens[c + lane], a.max_tokens));
-  total = __builtin_amdgcn_readfirstlane(wave_sum_int(total));
-  const int units = total * pairs;
-  const int per_worker = (units + gridDim.x - 1) / gridDim.x;
-  const int worker = blockIdx.x;
-  int u = worker * per_worker;
-  const int u_end = min(units, u + per_worker);
-  if (u >= u_end) return;
-  // the sequence that holds unit u
-  int b = 0, base = 0;
-  for (int c = 0; c < a.batch; c += kWave) {
-    const int mine = c + lane < a.batch ? units_of(min(a.seq_lens[c + lane], a.max_tokens)) * pairs : 0;
-    int upto = mine;  // inclusive prefix sum
+  const int c = blockIdx.x % COLS, pair = blockIdx.x / COLS;
+  const int b = pair / pairs, x = pair % pairs, cb = x % a.col_blocks, head = x / a.col_blocks;
+  if (cb * COLS + c >= a.new_tokens * a.group) return;
+  const int first_lens = len_at(a, lane_id());
+  const Work work = work_of(a, first_lens);
+  int base = 0, len = 0;
+  for (int i = 0; i <= b; i += kWave) {
+    const int lens = i ? len_at(a, i + lane_id()) : first_lens;
+    const int nu = units_or_none(lens);
+    const int size = work.slots ? (nu + work.per - 1) / work.per : nu;
+    const int upto = wave_scan(size);
+    const bool here = b < i + kWave;
+    base += __builtin_amdgcn_readlane(here ? upto - size : upto, here ? b - i : kWave - 1);
+    if (here) len = __builtin_amdgcn_readlane(lens, b - i);
+  }
+  const int nu = units_of(len);
+  const int slots = work.slots ? (nu + work.per - 1) / work.per : nu;
+  const int first = base * pairs + x * slots;
+  const int w_first = work.slots ? first : first / work.per;
+  const int w_last = work.slots ? first + slots - 1 : (first + nu - 1) / work.per;
+  if (w_first == w_last) return;  // one worker held the whole pair and stored its rows
+  const int grp = threadIdx.x / T, d = 4 * (threadIdx.x % T);
+  float m = kNoMax, l = 0.0f;
+  f32x4 o = (f32x4)(0.0f);
+#pragma unroll 4
+  for (int w = w_first + grp; w <= w_last; w += GROUPS) {
+    const float* p = a.parts + part_at<D, NQ>(w, w_first);
+    const float pm = p[c], pl = p[COLS + c];
+    const f32x4 po = *reinterpret_cast<const f32x4*>(p + 2 * COLS + c * D + d);
+    const float up = __builtin_fmaxf(m, pm);
+    const float f = __builtin_amdgcn_exp2f(m - up), fp = __builtin_amdgcn_exp2f(pm - up);
+    m = up, l = l * f + pl * fp, o = o * f + po * fp;
+  }
+  if (d == 0) sm[grp] = m, sl[grp] = l;
+  so[grp][threadIdx.x % T] = o;
+  __syncthreads();
+  if (grp != 0) return;
+  float up = kNoMax, sum = 0.0f;
+  f32x4 v = (f32x4)(0.0f);
 #pragma unroll
-    for (int x = 1; x < kWave; x *= 2) {
-      const int o = (int)from_lane((uint32_t)upto, lane - x);
-      if (lane >= x) upto += o;
-    }
-    const uint64_t past = __ballot(base + upto > u);
-    if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      b = c + at;
-      base += __builtin_amdgcn_readlane(upto - mine, at);
-      break;
-    }
-    base += __builtin_amdgcn_readlane(upto, kWave - 1);
+  for (int i = 0; i < GROUPS; ++i) up = __builtin_fmaxf(up, sm[i]);
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const float f = __builtin_amdgcn_exp2f(sm[i] - up);
+    sum += sl[i] * f, v += so[i][threadIdx.x] * f;
   }
-  while (u < u_end) {
-    const int len = __builtin_amdgcn_readfirstlane(min(a.seq_lens[b], a.max_tokens));
-    const int nu = units_of(len);
-    const int seq_end = base + nu * pairs;
-    while (u < min(u_end, seq_end)) {
-      const int x = (u - base) / nu;
-      Segment sg;
-      sg.b = b, sg.head = x / a.col_blocks, sg.cb = x % a.col_blocks;
-      sg.nu = nu, sg.len = max(len, 0), sg.first_unit = base + x * nu;
-      sg.u0 = u - sg.first_unit, sg.u1 = min(nu, u_end - sg.first_unit);
-      sg.pair = b * pairs + x;
-      run_segment<D, NQ>(a, sg, worker, per_worker, sh);
-      u = sg.first_unit + sg.u1;
-    }
-    base = seq_end;
-    ++b;
-  }
+  store_out(a, b, head, cb * COLS + c, d, v, sum);
 }
 
 struct Plan {
-  int nq, col_blocks;
+  int nq, col_blocks, joined;
   int64_t workers, counters;
   size_t scratch;
 };
@@ -390,12 +701,17 @@ Plan plan_of(int64_t batch, int64_t new_tokens, int64_t heads_q, int64_t heads_k
              int64_t max_tokens) {
   Plan p;
   const int64_t cols = new_tokens * (heads_q / heads_kv);
-  p.nq = cols > 16 ? 2 : 1;
+  p.nq = cols > 16 && head_dim < 256 ? 2 : 1;
   p.col_blocks = (int)((cols + 16 * p.nq - 1) / (16 * p.nq));
   const int64_t units = max_tokens > 0 ? (max_tokens + kUnit - 1) / kUnit : 1;
   p.counters = batch * heads_kv * p.col_blocks;
-  const int64_t most = 2 * (int64_t)lbh::device_cus();
+  const int64_t most = (head_dim * p.nq <= 128 ? 2 : 1) * (int64_t)lbh::device_cus();
   p.workers = p.counters * units < most ? p.counters * units : most;
+  if (4 * p.counters > p.workers && p.workers < most) p.workers = 4 * p.counters < most ? 4 * p.counters : most;
+  // parts of a pair where all sequences fill the table (with one long sequence
+  // among short ones it may have more; the last worker then joins those too)
+  const int64_t per = (p.counters * units + p.workers - 1) / p.workers;
+  p.joined = units / (per > kMinUnits ? per : kMinUnits) + 1 > kFewParts;
   p.scratch = ((size_t)p.workers * 2 * 16 * p.nq * (head_dim + 2) * 4 + 255) & ~(size_t)255;
   return p;
 }
@@ -416,11 +732,13 @@ int check_sizes(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv
   return LB_OK;
 }
 
-template <int D>
+template <int D, int NQ>
 void launch(const AttnArgs& a, const Plan& p, hipStream_t st) {
-  const dim3 grid((unsigned)p.workers), block(kWave * kWaves);
-  if (p.nq == 1) kv8_attention_kernel<D, 1><<<grid, block, 0, st>>>(a);
-  else kv8_attention_kernel<D, 2><<<grid, block, 0, st>>>(a);
+  const dim3 grid((unsigned)p.workers), block(kThreads<D>);
+  // 64 and 128 channels: up to 16 columns are always one block
+  if (p.col_blocks == 1) kv8_attention_kernel<D, NQ, true><<<grid, block, 0, st>>>(a);
+  else if constexpr (D == 256 || NQ == 2) kv8_attention_kernel<D, NQ, false><<<grid, block, 0, st>>>(a);
+  if (p.joined) kv8_join_kernel<D, NQ><<<dim3((unsigned)(p.counters * 16 * NQ)), dim3(256), 0, st>>>(a);
 }
 
 }  // namespace
@@ -444,7 +762,7 @@ extern "C" int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64
   using namespace lb;
   const int err = check_sizes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages);
   if (err != LB_OK) return err;
-  if (num_pages < 0 || num_pages > 0x7fffffff || table_stride < max_pages) return LB_ERR_ARG;
+  if (num_pages < 0 || num_pages > 0x7fffffff / heads_kv || table_stride < max_pages) return LB_ERR_ARG;
   if (!(softmax_scale > 0.0f) || softmax_scale > 3e38f) return LB_ERR_ARG;
   if (batch == 0 || tokens == 0) return LB_OK;
   if (!q || !out || !seq_lens || !workspace) return LB_ERR_ARG;
@@ -469,10 +787,11 @@ extern "C" int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64
   a.max_tokens = num_pages > 0 ? (int)(max_pages * page_size) : 0;
   a.batch = (int)batch, a.new_tokens = (int)(tokens / batch), a.heads_kv = (int)heads_kv;
   a.group = (int)(heads_q / heads_kv), a.col_blocks = p.col_blocks;
+  a.workers = (int)p.workers, a.joined = p.joined;
   a.scale = softmax_scale * kLog2e;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (head_dim == 64) launch<64>(a, p, st);
-  else if (head_dim == 128) launch<128>(a, p, st);
-  else launch<256>(a, p, st);
+  if (head_dim == 256) launch<256, 1>(a, p, st);
+  else if (head_dim == 128) p.nq == 1 ? launch<128, 1>(a, p, st) : launch<128, 2>(a, p, st);
+  else p.nq == 1 ? launch<64, 1>(a, p, st) : launch<64, 2>(a, p, st);
   return lbh::launch_status();
 }

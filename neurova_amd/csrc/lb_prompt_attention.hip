@@ -24,8 +24,7 @@ struct PromptArgs {
   float scale;  // softmax scale * log2(e)
 };
 
-constexpr int kWaves = 4;
-constexpr int kKeys = 64;  // keys of a tile
+constexpr int kAhead = 7;  // LDS reads ahead of the products that take them
 constexpr float kNoMax = -1e30f;
 // The running maximum moves only when a score exceeds it by 2^kSlack, and the
 // weights (and their sum) carry 2^kLift more: at most 2^15, inside fp16, and 2^7
@@ -49,44 +48,99 @@ __device__ __forceinline__ int v_swizzle(int row) {
 
 // A tile of 64 rows of keys (values) into LDS, 16 bytes a lane and load; rows
 // past `rows` come out as zeros (the descriptor ends there).
-template <int D, bool KEYS>
+template <int D, int KT, int W, bool KEYS>
 __device__ __forceinline__ void stage(const uint16_t* base, int64_t token_stride, int rows, uint16_t* lds, int wave,
                                       int lane) {
   constexpr int C = D / 8;
   const __amdgpu_buffer_rsrc_t r =
-      buffer_of(base, (uint32_t)(((int64_t)(min(rows, kKeys) - 1) * token_stride + D) * 2));
+      buffer_of(base, (uint32_t)(((int64_t)(min(rows, KT) - 1) * token_stride + D) * 2));
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) {
-    const int c = (j * kWaves + wave) * kWave + lane;
+  for (int j = 0; j < KT * D / (W * kWave * 8); ++j) {
+    const int c = (j * W + wave) * kWave + lane;
     const int row = c / C, col = (c % C) ^ (KEYS ? k_swizzle<D>(row) : v_swizzle<D>(row));
     const uint32_t off = (uint32_t)(row * (int)token_stride * 2 + col * 16);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + (j * kWaves + wave) * kWave * 8), 16, off, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + (j * W + wave) * kWave * 8), 16, off, 0, 0, 0);
   }
 }
 
-template <int D, int RB>
-__global__ __launch_bounds__(kWave * kWaves, 1) void prompt_attention_kernel(PromptArgs a) {
-  constexpr int ROWS = kWaves * RB * 32, DT = D / 32, KK = D / 16;
-  __shared__ __align__(16) uint16_t kbuf[2][kKeys * D];
-  __shared__ __align__(16) uint16_t vbuf[2][kKeys * D];
+// The tiles with the most keys come first, whichever sequence they are of: a
+// workgroup's time is its number of keys, and short ones last fill the ends.
+struct Place {
+  int first, len, tile;  // of the sequence: its first token and length
+};
+
+struct Span {
+  int first, len;
+};
+__device__ __forceinline__ Span span_of(const PromptArgs& a, int b) {
+  if (b >= a.batch) return {0, 0};
+  const int first = max(a.starts[b], 0);
+  return {first, min(a.starts[b + 1], a.tokens) - first};
+}
+template <int ROWS>
+__device__ __forceinline__ int tiles_of(const PromptArgs& a, int len) {
+  return len > 0 ? (len * a.group + ROWS - 1) / ROWS : 0;
+}
+
+// Item i of all sequences' tiles in falling order of their place in the
+// sequence; an empty place past the last.  64 sequences stay in registers.
+template <int ROWS>
+__device__ __forceinline__ Place place_of(const PromptArgs& a, int i) {
+  const int lane = lane_id();
+  const Span own = span_of(a, lane);
+  const int own_tiles = tiles_of<ROWS>(a, own.len);
+  auto from = [&](int t) {  // tiles at place t or later
+    int n = __builtin_amdgcn_readlane(wave_scan(max(own_tiles - t, 0)), kWave - 1);
+    for (int c = kWave; c < a.batch; c += kWave)
+      n += __builtin_amdgcn_readlane(wave_scan(max(tiles_of<ROWS>(a, span_of(a, c + lane).len) - t, 0)), kWave - 1);
+    return n;
+  };
+  int rank = from(0);
+  if (rank <= i) return {0, 0, 0};
+  int lo = rank - 1 - i;  // where one sequence has all the tiles
+  if (a.batch > 1) {
+    lo = 0;
+    int hi = a.tiles;  // from(lo) > i >= from(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (from(mid) > i) lo = mid; else hi = mid;
+    }
+  }
+  rank = i - from(lo + 1);  // among the sequences that have a tile lo
+  for (int c = 0; c < a.batch; c += kWave) {
+    const Span s = c ? span_of(a, c + lane) : own;
+    const bool has = (c ? tiles_of<ROWS>(a, s.len) : own_tiles) > lo;
+    const uint64_t m = __ballot(has);
+    const int n = __popcll(m);
+    if (rank < n) {
+      const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+      const int at = __builtin_ctzll(__ballot(has && before == rank));
+      return {__builtin_amdgcn_readlane(s.first, at), __builtin_amdgcn_readlane(s.len, at), lo};
+    }
+    rank -= n;
+  }
+  return {0, 0, 0};
+}
+
+template <int D, int KT, int RB, int W, int PER_SIMD>
+__global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(PromptArgs a) {
+  constexpr int ROWS = W * RB * 32, DT = D / 32, KK = D / 16, ST = KT / 32;
+  // four arrays and not one: the compiler would make every read of a tile wait
+  // for the loads of the next into the same array
+  __shared__ __align__(16) uint16_t k0[KT * D], k1[KT * D], v0[KT * D], v1[KT * D];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 31, h = lane >> 5;
-  // the last tiles, which see the most keys, come first
-  const int kvh = blockIdx.x % a.heads_kv, item = a.tiles - 1 - blockIdx.x / a.heads_kv;
-  int first = 0, len = a.tokens, tile = item;
+  const int kvh = blockIdx.x % a.heads_kv, item = blockIdx.x / a.heads_kv;
+  int first = 0, len = a.tokens, tile = a.tiles - 1 - item;
   if (a.starts != nullptr) {
-    const int b = sequence_of_item(a.starts, a.batch, a.group, ROWS, 1, item);
-    if (b < 0) return;
-    first = a.starts[b];
-    tile = item - (first * a.group / ROWS + b);
-    first = max(first, 0);
-    len = min(a.starts[b + 1], a.tokens) - first;
+    const Place at = place_of<ROWS>(a, item);
+    first = at.first, len = at.len, tile = at.tile;
   }
   first = __builtin_amdgcn_readfirstlane(first), len = __builtin_amdgcn_readfirstlane(len);
   const int rows = len * a.group, row0 = tile * ROWS;
   if (row0 >= rows) return;
   const int last_token = (min(rows, row0 + ROWS) - 1) / a.group;
-  const int tiles = last_token / kKeys + 1;
+  const int tiles = last_token / KT + 1;
   const int wave_row = row0 + wave * RB * 32;
   const int wave_first = wave_row / a.group;  // tokens of the wave's first and last row
   const int wave_last = wave_row < rows ? (min(rows, wave_row + RB * 32) - 1) / a.group : -1;
@@ -118,50 +172,58 @@ __global__ __launch_bounds__(kWave * kWaves, 1) void prompt_attention_kernel(Pro
     for (int d = 0; d < DT; ++d) o[n][d] = (f32x16_t)(0.0f);
   }
 
-  stage<D, true>(kbase, a.k_token, len, kbuf[0], wave, lane);
-  stage<D, false>(vbase, a.v_token, len, vbuf[0], wave, lane);
-  for (int kt = 0; kt < tiles; ++kt) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  stage<D, KT, W, true>(kbase, a.k_token, len, k0, wave, lane);
+  stage<D, KT, W, false>(vbase, a.v_token, len, v0, wave, lane);
+  // tile kt from (kl, vl), and the loads of the next into (kn, vn)
+  auto take = [&](int kt, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), as a builtin: the compiler then knows that the tile is there
     lds_barrier();
-    const int cur = kt & 1;
     if (kt + 1 < tiles) {
-      const int64_t at = (int64_t)(kt + 1) * kKeys;
-      const int left = len - (kt + 1) * kKeys;
-      stage<D, true>(kbase + at * a.k_token, a.k_token, left, kbuf[cur ^ 1], wave, lane);
-      stage<D, false>(vbase + at * a.v_token, a.v_token, left, vbuf[cur ^ 1], wave, lane);
+      const int64_t at = (int64_t)(kt + 1) * KT;
+      const int left = len - (kt + 1) * KT;
+      stage<D, KT, W, true>(kbase + at * a.k_token, a.k_token, left, kn, wave, lane);
+      stage<D, KT, W, false>(vbase + at * a.v_token, a.v_token, left, vn, wave, lane);
     }
-    if (kt * kKeys > wave_last) continue;
-    const uint16_t* kl = kbuf[cur];
-    const uint16_t* vl = vbuf[cur];
+    if (kt * KT > wave_last) return;
 
-    f32x16_t s[RB][2];
+    f32x16_t s[RB][ST];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < ST; ++t)
 #pragma unroll
       for (int n = 0; n < RB; ++n) s[n][t] = (f32x16_t)(0.0f);
 #pragma unroll
-      for (int k = 0; k < KK; ++k) {
+    for (int k = 0; k < KK; ++k)
+#pragma unroll
+      for (int t = 0; t < ST; ++t) {
         const int row = 32 * t + r;
         const f16x8 kf =
             *reinterpret_cast<const f16x8*>(kl + row * D + 8 * ((2 * k + h) ^ k_swizzle<D>(row)));
 #pragma unroll
         for (int n = 0; n < RB; ++n) s[n][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[n][k], s[n][t], 0, 0, 0);
       }
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < ST * KK - kAhead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, RB, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
-    f16x8 pf[RB][4];
+    __builtin_amdgcn_sched_group_barrier(0x008, RB * kAhead, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    f16x8 pf[RB][2 * ST];
 #pragma unroll
     for (int n = 0; n < RB; ++n) {
-      if (kt * kKeys + kKeys - 1 > wave_first) {
-        const int past = seen[n] - kt * kKeys - 4 * h;  // keys of the lane up to here are seen
+      if (kt * KT + KT - 1 > wave_first) {
+        const int past = seen[n] - kt * KT - 4 * h;  // keys of the lane up to here are seen
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < ST; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (32 * t + 8 * (i >> 2) + (i & 3) > past) s[n][t][i] = -__builtin_inff();
       }
       float peak = kNoMax;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < ST; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) peak = __builtin_fmaxf(peak, s[n][t][i]);
       peak *= a.scale;
@@ -175,7 +237,7 @@ __global__ __launch_bounds__(kWave * kWaves, 1) void prompt_attention_kernel(Pro
       }
       const float lift = kLift - m[n];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < ST; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float p = __builtin_amdgcn_exp2f(s[n][t][i] * a.scale + lift);
@@ -184,9 +246,9 @@ __global__ __launch_bounds__(kWave * kWaves, 1) void prompt_attention_kernel(Pro
         }
     }
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
+    for (int c = 0; c < 2 * ST; ++c) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int d = 0; d < DT; ++d) {
         f16x8 vf;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -201,6 +263,10 @@ __global__ __launch_bounds__(kWave * kWaves, 1) void prompt_attention_kernel(Pro
         for (int n = 0; n < RB; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[n][c], o[n][d], 0, 0, 0);
       }
     }
+  };
+  for (int kt = 0; kt < tiles; kt += 2) {
+    take(kt, k0, v0, k1, v1);
+    if (kt + 1 < tiles) take(kt + 1, k1, v1, k0, v0);
   }
 
 #pragma unroll
@@ -223,15 +289,15 @@ __global__ __launch_bounds__(kWave * kWaves, 1) void prompt_attention_kernel(Pro
   }
 }
 
-template <int D, int RB>
+template <int D, int KT, int RB, int W, int PER_SIMD>
 int launch(PromptArgs a, hipStream_t st) {
-  constexpr int ROWS = kWaves * RB * 32;
+  constexpr int ROWS = W * RB * 32;
   const int64_t rows = (int64_t)a.tokens * a.group;
-  // sequence b's tiles are numbered from starts[b] * group / ROWS + b, which leaves room for all of them
+  // every sequence may end inside a tile
   const int64_t tiles = a.starts ? rows / ROWS + a.batch : (rows + ROWS - 1) / ROWS;
   if (tiles * a.heads_kv > 0x7fffffff) return LB_ERR_PROB_SHAPE;
   a.tiles = (int)tiles;
-  prompt_attention_kernel<D, RB><<<dim3((unsigned)(tiles * a.heads_kv)), dim3(kWave * kWaves), 0, st>>>(a);
+  prompt_attention_kernel<D, KT, RB, W, PER_SIMD><<<dim3((unsigned)(tiles * a.heads_kv)), dim3(kWave * W), 0, st>>>(a);
   return lbh::launch_status();
 }
 
@@ -269,7 +335,7 @@ extern "C" int lb_prompt_attention(const uint16_t* q, int64_t q_token_stride, in
   a.starts = cu_seqlens, a.batch = (int)batch, a.tokens = (int)tokens, a.group = (int)(heads_q / heads_kv);
   a.heads_kv = (int)heads_kv, a.scale = softmax_scale * kLog2e;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (head_dim == 64) return launch<64, 2>(a, st);
-  if (head_dim == 128) return launch<128, 2>(a, st);
-  return launch<256, 1>(a, st);
+  if (head_dim == 64) return launch<64, 64, 1, 4, 3>(a, st);
+  if (head_dim == 128) return launch<128, 64, 1, 4, 2>(a, st);
+  return launch<256, 64, 1, 4, 1>(a, st);
 }

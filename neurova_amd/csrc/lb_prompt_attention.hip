@@ -24,7 +24,6 @@ struct PromptArgs {
   float scale;  // softmax scale * log2(e)
 };
 
-constexpr int kAhead = 7;  // LDS reads ahead of the products that take them
 constexpr float kNoMax = -1e30f;
 // The running maximum moves only when a score exceeds it by 2^kSlack, and the
 // weights (and their sum) carry 2^kLift more: at most 2^15, inside fp16, and 2^7
@@ -46,22 +45,22 @@ __device__ __forceinline__ int v_swizzle(int row) {
   return D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
 }
 
-// A tile of 64 rows of keys (values) into LDS, 16 bytes a lane and load; rows
-// past `rows` come out as zeros (the descriptor ends there).
+// A tile of keys (values) on its way into LDS, 16 bytes a lane and load, N loads
+// a wave; rows past `rows` come out as zeros (the descriptor ends there).
 template <int D, int KT, int W, bool KEYS>
-__device__ __forceinline__ void stage(const uint16_t* base, int64_t token_stride, int rows, uint16_t* lds, int wave,
-                                      int lane) {
-  constexpr int C = D / 8;
-  const __amdgpu_buffer_rsrc_t r =
-      buffer_of(base, (uint32_t)(((int64_t)(min(rows, KT) - 1) * token_stride + D) * 2));
-#pragma unroll
-  for (int j = 0; j < KT * D / (W * kWave * 8); ++j) {
+struct Stage {
+  static constexpr int N = KT * D / (W * kWave * 8);
+  __amdgpu_buffer_rsrc_t from;
+  __device__ __forceinline__ Stage(const uint16_t* base, int64_t token_stride, int rows)
+      : from(buffer_of(base, rows > 0 ? (uint32_t)(((int64_t)(min(rows, KT) - 1) * token_stride + D) * 2) : 0u)) {}
+  __device__ __forceinline__ void load(int j, int token_stride, uint16_t* lds, int wave, int lane) const {
+    constexpr int C = D / 8;
     const int c = (j * W + wave) * kWave + lane;
     const int row = c / C, col = (c % C) ^ (KEYS ? k_swizzle<D>(row) : v_swizzle<D>(row));
-    const uint32_t off = (uint32_t)(row * (int)token_stride * 2 + col * 16);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + (j * W + wave) * kWave * 8), 16, off, 0, 0, 0);
+    const uint32_t off = (uint32_t)(row * token_stride * 2 + col * 16);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)(lds + (j * W + wave) * kWave * 8), 16, off, 0, 0, 0);
   }
-}
+};
 
 // The tiles with the most keys come first, whichever sequence they are of: a
 // workgroup's time is its number of keys, and short ones last fill the ends.
@@ -142,8 +141,7 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
   const int last_token = (min(rows, row0 + ROWS) - 1) / a.group;
   const int tiles = last_token / KT + 1;
   const int wave_row = row0 + wave * RB * 32;
-  const int wave_first = wave_row / a.group;  // tokens of the wave's first and last row
-  const int wave_last = wave_row < rows ? (min(rows, wave_row + RB * 32) - 1) / a.group : -1;
+  const int wave_first = wave_row / a.group;  // token of the wave's first row
 
   f16x8 qf[RB][KK];
   int seen[RB];  // the last key of the lane's row
@@ -172,44 +170,65 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
     for (int d = 0; d < DT; ++d) o[n][d] = (f32x16_t)(0.0f);
   }
 
-  stage<D, KT, W, true>(kbase, a.k_token, len, k0, wave, lane);
-  stage<D, KT, W, false>(vbase, a.v_token, len, v0, wave, lane);
-  // tile kt from (kl, vl), and the loads of the next into (kn, vn)
+  typedef Stage<D, KT, W, true> Keys;
+  typedef Stage<D, KT, W, false> Values;
+  static_assert(Keys::N + Values::N == KK * RB, "one load of the next tile for each channel step of the scores");
+  const int k_token = (int)a.k_token, v_token = (int)a.v_token;
+  {
+    const Keys keys(kbase, k_token, len);
+    const Values values(vbase, v_token, len);
+#pragma unroll
+    for (int j = 0; j < Keys::N; ++j) keys.load(j, k_token, k0, wave, lane), values.load(j, v_token, v0, wave, lane);
+  }
+  // Tile kt from (kl, vl).  The next tile's loads into (kn, vn) go out between
+  // the products of the scores: all at once they would hold up the wave (16
+  // loads of 1 KB from four waves take 1000 cycles and more to be accepted).
+  // After the last tile they have no rows: zeros, from nowhere.
   auto take = [&](int kt, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), as a builtin: the compiler then knows that the tile is there
     lds_barrier();
-    if (kt + 1 < tiles) {
-      const int64_t at = (int64_t)(kt + 1) * KT;
-      const int left = len - (kt + 1) * KT;
-      stage<D, KT, W, true>(kbase + at * a.k_token, a.k_token, left, kn, wave, lane);
-      stage<D, KT, W, false>(vbase + at * a.v_token, a.v_token, left, vn, wave, lane);
-    }
-    if (kt * KT > wave_last) return;
-
+    const int64_t at = (int64_t)(kt + 1) * KT;
+    const int left = kt + 1 < tiles ? len - (kt + 1) * KT : 0;
+    const Keys keys(kbase + at * k_token, k_token, left);
+    const Values values(vbase + at * v_token, v_token, left);
+    auto load_next = [&](int j) {
+      if (j < Keys::N) keys.load(j, k_token, kn, wave, lane);
+      else values.load(j - Keys::N, v_token, vn, wave, lane);
+    };
     f32x16_t s[RB][ST];
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
       for (int n = 0; n < RB; ++n) s[n][t] = (f32x16_t)(0.0f);
+    constexpr int CH = KK / 4;  // channel steps of a quarter
+    f16x8 kf[2][CH][ST];
+    auto read_k = [&](int q) {
 #pragma unroll
-    for (int k = 0; k < KK; ++k)
+      for (int k = 0; k < CH; ++k)
 #pragma unroll
-      for (int t = 0; t < ST; ++t) {
-        const int row = 32 * t + r;
-        const f16x8 kf =
-            *reinterpret_cast<const f16x8*>(kl + row * D + 8 * ((2 * k + h) ^ k_swizzle<D>(row)));
+        for (int t = 0; t < ST; ++t) {
+          const int row = 32 * t + r;
+          kf[q & 1][k][t] = *reinterpret_cast<const f16x8*>(
+              kl + row * D + 8 * ((2 * (q * CH + k) + h) ^ k_swizzle<D>(row)));
+        }
+    };
+    read_k(0);
 #pragma unroll
-        for (int n = 0; n < RB; ++n) s[n][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[n][k], s[n][t], 0, 0, 0);
-      }
-    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+    for (int q = 0; q < 4; ++q) {
+      if (q < 3) read_k(q + 1);
 #pragma unroll
-    for (int i = 0; i < ST * KK - kAhead; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, RB, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+          for (int n = 0; n < RB; ++n)
+            s[n][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[q & 1][k][t], qf[n][q * CH + k], s[n][t], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < CH; ++k) load_next(q * CH + k);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, RB * kAhead, 0);
-    __builtin_amdgcn_sched_barrier(0);
     f16x8 pf[RB][2 * ST];
 #pragma unroll
     for (int n = 0; n < RB; ++n) {
@@ -268,6 +287,7 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
     take(kt, k0, v0, k1, v1);
     if (kt + 1 < tiles) take(kt + 1, k1, v1, k0, v0);
   }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // no load may arrive in LDS after the workgroup
 
 #pragma unroll
   for (int n = 0; n < RB; ++n) {

@@ -289,14 +289,18 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);  // no load may arrive in LDS after the workgroup
 
+  // The rows leave through LDS (a wave's 32 x D in an array that no wave reads
+  // any more): a store then takes whole rows, where a lane's accumulators are
+  // four channels of a row each.  Chunks change places as in the tiles.
+  lds_barrier();
+  uint16_t* mine = wave < 2 ? (wave == 0 ? k0 : k1) : (wave == 2 ? v0 : v1);
+  static_assert(W == 4 && KT >= 32, "one array a wave");
 #pragma unroll
   for (int n = 0; n < RB; ++n) {
     l[n] += from_lane(l[n], lane ^ 32);
     const float inv = 1.0f / l[n];
-    const int row = wave_row + 32 * n + r;
-    if (row >= rows) continue;
-    const int t = row / a.group;
-    uint16_t* p = a.out + (int64_t)(first + t) * a.o_token + (int64_t)(kvh * a.group + row - t * a.group) * a.o_head;
+    const int row = wave_row + 32 * n + r, t = row / a.group;
+    const int64_t place = (int64_t)(first + t) * a.o_token + (int64_t)(kvh * a.group + row - t * a.group) * a.o_head;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -304,8 +308,17 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
         u32x2 w;
         w[0] = as_u32((f16x2){(f16)(o[n][d][i] * inv), (f16)(o[n][d][i + 1] * inv)});
         w[1] = as_u32((f16x2){(f16)(o[n][d][i + 2] * inv), (f16)(o[n][d][i + 3] * inv)});
-        *reinterpret_cast<u32x2*>(p + 32 * d + 2 * i + 4 * h) = w;
+        const int chunk = (4 * d + i / 4) ^ k_swizzle<D>(r);
+        *reinterpret_cast<u32x2*>(mine + r * D + 8 * chunk + 4 * h) = w;
       }
+#pragma unroll
+    for (int j = 0; j < 32 * D / 8 / kWave; ++j) {
+      const int x = j * kWave + lane, rr = x / (D / 8), chunk = x % (D / 8);
+      const uint32_t lo = from_lane((uint32_t)place, rr), hi = from_lane((uint32_t)(place >> 32), rr);
+      const u32x4 w = *reinterpret_cast<const u32x4*>(mine + rr * D + 8 * (chunk ^ k_swizzle<D>(rr)));
+      if (wave_row + 32 * n + rr < rows)
+        *reinterpret_cast<u32x4*>(a.out + (int64_t)(((uint64_t)hi << 32) | lo) + 8 * chunk) = w;
+    }
   }
 }
 

@@ -57,30 +57,6 @@ __device__ __forceinline__ void store8(uint16_t* p, f32x8 v) {
   *reinterpret_cast<u32x4*>(p) = w;
 }
 
-// cos and sin of eight consecutive frequencies at `pos`.  A position outside
-// the table has none: NaN, which the outputs then show.
-__device__ __forceinline__ void angles(const AppendArgs& a, int pos, int f, f32x8& c, f32x8& s) {
-  if ((unsigned)pos >= (unsigned)a.positions) {
-    c = s = (f32x8)(__builtin_nanf(""));
-    return;
-  }
-  const float* row = a.cos_sin + (int64_t)pos * a.rot + f;
-  c = *reinterpret_cast<const f32x8*>(__builtin_assume_aligned(row, 16));
-  s = *reinterpret_cast<const f32x8*>(__builtin_assume_aligned(row + a.rot / 2, 16));
-}
-
-// The same of four.
-__device__ __forceinline__ void angles4(const AppendArgs& a, int pos, int f, f32x8& c, f32x8& s) {
-  if ((unsigned)pos >= (unsigned)a.positions) {
-    c = s = (f32x8)(__builtin_nanf(""));
-    return;
-  }
-  const float* row = a.cos_sin + (int64_t)pos * a.rot + f;
-  const f32x4 c4 = *reinterpret_cast<const f32x4*>(row), s4 = *reinterpret_cast<const f32x4*>(row + a.rot / 2);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) c[j] = c4[j], s[j] = s4[j];
-}
-
 // (x, y) -> (x cos - y sin, y cos + x sin), every operation rounded by itself.
 __device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
 #pragma clang fp contract(off)
@@ -89,27 +65,52 @@ __device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
   y = yc + xs;
 }
 
-// The two vectors of eight that rotate together: halves pair value i with
-// i + rot/2, interleaved pairs are neighbours.  Pair j of a head is vectors
-// (j, j + rot/16) or (2j, 2j + 1); past the rotated part it is (2j, 2j + 1).
+// Two vectors of eight of a head and their angles.  Halves pair value i with
+// i + rot/2: vectors (j, j + rot/16), with eight angles.  Interleaved pairs are
+// neighbours inside a vector: (j, j + head_dim/16), with four angles each.  Either
+// way, and past the rotated part, neighbouring j take neighbouring vectors, so
+// that loads and stores cover whole lines.
 struct Pair {
   int v0, v1;
-  bool rotated;
+  bool r0, r1;  // rotated
 };
 __device__ __forceinline__ Pair pair_of(const AppendArgs& a, int j) {
-  const int n = a.rot / 16;
-  if (j < n && !a.interleaved) return {j, j + n, true};
-  return {2 * j, 2 * j + 1, j < n};
+  const int n = a.rot / 16, half = a.d8 / 2;
+  if (a.interleaved) return {j, j + half, j < 2 * n, j + half < 2 * n};
+  if (j < n) return {j, j + n, true, true};
+  return {n + j, half + j, false, false};
 }
 
-__device__ __forceinline__ void rotate_pair(f32x8& x, f32x8& y, const f32x8& c, const f32x8& s, bool interleaved) {
+// The pair's cos and sin at `pos` (interleaved: four of v0, then four of v1).  A
+// position outside the table has none: NaN, which the outputs then show.
+__device__ __forceinline__ void angles(const AppendArgs& a, int pos, const Pair& p, f32x8& c, f32x8& s) {
+  if ((unsigned)pos >= (unsigned)a.positions) {
+    c = s = (f32x8)(__builtin_nanf(""));
+    return;
+  }
+  const float* row = a.cos_sin + (int64_t)pos * a.rot;
+  const int f0 = a.interleaved ? 4 * p.v0 : 8 * p.v0, f1 = a.interleaved ? (p.r1 ? 4 * p.v1 : f0) : f0 + 4;
+  const f32x4 c0 = *reinterpret_cast<const f32x4*>(row + f0), c1 = *reinterpret_cast<const f32x4*>(row + f1);
+  const f32x4 s0 = *reinterpret_cast<const f32x4*>(row + a.rot / 2 + f0);
+  const f32x4 s1 = *reinterpret_cast<const f32x4*>(row + a.rot / 2 + f1);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = c0[i], c[4 + i] = c1[i], s[i] = s0[i], s[4 + i] = s1[i];
+}
+
+__device__ __forceinline__ void rotate_pair(const Pair& p, bool interleaved, f32x8& x, f32x8& y, const f32x8& c,
+                                            const f32x8& s) {
+  if (!p.r0) return;
   if (interleaved) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float u = x[2 * i], w = x[2 * i + 1];
       turn(u, w, c[i], s[i]);
       x[2 * i] = u, x[2 * i + 1] = w;
-      u = y[2 * i], w = y[2 * i + 1];
+    }
+    if (!p.r1) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float u = y[2 * i], w = y[2 * i + 1];
       turn(u, w, c[4 + i], s[4 + i]);
       y[2 * i] = u, y[2 * i + 1] = w;
     }
@@ -147,149 +148,158 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* lds) {
   return v;
 }
 
-// Keys (or values) of one head in one page.  A thread holds four neighbouring
-// tokens at eight neighbouring channels: eight codes of a token are one store
-// of the key layout [page][token][channel], four of a channel one of the value
-// layout [page][channel][token], and nothing has to change threads.
-template <bool KEYS>
-__device__ __forceinline__ void append_page(const AppendArgs& a, int b, int first_token, int start, int len, int page,
-                                            int head, uint32_t* lds) {
-  const int p = 1 << a.page_shift;
-  const int page_lo = page << a.page_shift;
-  const int lo = max(max(start, 0), page_lo), hi = min(len, page_lo + p);
-  if (lo >= hi || page >= a.max_pages) return;
-  const int id = a.page_table[(int64_t)b * a.table_stride + page];
-  if ((unsigned)id >= (unsigned)a.num_pages) return;
-  const int64_t cell = (int64_t)id * a.heads_kv + head;
-  float* scale_at = (KEYS ? a.k_scale : a.v_scale) + cell;
-  const bool kept = page_lo < start;
-  const float old_scale = kept ? *scale_at : 0.0f;
+// One head of one page: where it is, which of its slots are new, and the scale
+// that it has and gets.
+struct Cell {
+  int page_lo, lo, hi;  // positions: of the page's first slot, and of the new tokens in it
+  int start, first;     // of the sequence's new tokens: the first's position, and its row
+  int head;
+  int64_t cell;         // page * heads + head
+  float* scale_at;
+  float old_scale;
+  bool kept;            // the page holds earlier tokens
+  __device__ __forceinline__ bool is_new(int pos) const { return pos >= lo && pos < hi; }
+  __device__ __forceinline__ int old_slots() const { return kept ? start - page_lo : 0; }
+};
 
-  const int t4 = p / 4;
-  const int tid = threadIdx.x;
-  const bool active = tid < t4 * a.d8;
-  const int d8 = KEYS ? tid % a.d8 : tid / t4;
-  const int tg = KEYS ? tid / a.d8 : tid % t4;
-  // loads of the group's four tokens together; a slot that is not new reads a
-  // new one's row instead and drops it
-  f32x8 x[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (f32x8)(0.0f);
-  const int pos0 = page_lo + 4 * tg;
-  uint32_t peak = 0;
-  if (active && pos0 + 4 > lo && pos0 < hi) {
-    const Rows& src = KEYS ? a.k : a.v;
-    const int pairs = a.rot / 16;
-    const bool rotated = KEYS && 8 * d8 < a.rot;
-    const bool low = d8 < pairs;  // halves: which of the pair this thread stores
-    f32x8 y[4], c[4], s[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int pos = min(max(pos0 + i, lo), hi - 1);
-      const uint16_t* row = src.p + (int64_t)(first_token + (pos - start)) * src.token + (int64_t)head * src.head;
-      x[i] = load8(row + 8 * d8);
-      if (rotated && a.interleaved) {
-        angles4(a, pos, 4 * d8, c[i], s[i]);
-      } else if (rotated) {
-        y[i] = load8(row + 8 * (low ? d8 + pairs : d8 - pairs));
-        angles(a, pos, 8 * (low ? d8 : d8 - pairs), c[i], s[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int pos = pos0 + i;
-      if (rotated && a.interleaved) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float u = x[i][2 * j], w = x[i][2 * j + 1];
-          turn(u, w, c[i][j], s[i][j]);
-          x[i][2 * j] = u, x[i][2 * j + 1] = w;
-        }
-      } else if (rotated) {
-        f32x8 u = low ? x[i] : y[i], w = low ? y[i] : x[i];
-        rotate_pair(u, w, c[i], s[i], false);
-        x[i] = low ? u : w;
-      }
-      if (pos < lo || pos >= hi) {
-        x[i] = (f32x8)(0.0f);
-        continue;
-      }
-      if (KEYS && a.k_out.p)
-        store8(a.k_out.p + (int64_t)(first_token + (pos - start)) * a.k_out.token + (int64_t)head * a.k_out.head + 8 * d8,
-               x[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float e = x[i][j];
-        const uint32_t m = __builtin_bit_cast(uint32_t, e) & 0x7fffffffu;
-        peak = m > peak ? m : peak;
-      }
-    }
-  }
+// What the page's codes are scaled by.  `peak` is the largest bit pattern of a
+// new value; every thread of the workgroup calls this.
+struct Scaling {
+  float inverse, shrink;
+  bool grew;
+};
+__device__ __forceinline__ Scaling rescale(const Cell& c, uint32_t peak, uint32_t* lds) {
   peak = block_max(peak, lds);
   const float need = __builtin_bit_cast(float, peak) * (1.0f / 127.0f);
   // `need` may be NaN: then it is taken
-  const float scale = need <= old_scale ? old_scale : need;
-  const bool grew = kept && scale != old_scale;
-  if (tid == 0 && scale != old_scale) *scale_at = scale;
-  if (tid == 0 && !kept && scale == 0.0f) *scale_at = 0.0f;
-  const float inverse = scale > 0.0f ? 1.0f / scale : 0.0f;
-  const float shrink = grew ? old_scale / scale : 1.0f;
-  if (!active) return;
+  const float scale = need <= c.old_scale ? c.old_scale : need;
+  Scaling s;
+  s.grew = c.kept && scale != c.old_scale;
+  if (threadIdx.x == 0 && (scale != c.old_scale || !c.kept)) *c.scale_at = scale;
+  s.inverse = scale > 0.0f ? 1.0f / scale : 0.0f;
+  s.shrink = s.grew ? c.old_scale / scale : 1.0f;
+  return s;
+}
 
-  const int old_slots = kept ? start - page_lo : 0;  // slots before the new tokens
-  const int off0 = 4 * tg;
-  if (KEYS) {
-    int8_t* base = a.k_cache + ((cell << a.page_shift) + off0) * (8 * a.d8) + 8 * d8;
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+// Keys: a thread holds two neighbouring tokens at a pair of vectors that rotate
+// together, so each value and angle is loaded once; eight codes of a token are
+// one store of the layout [page][token][channel].
+__device__ __forceinline__ void append_keys(const AppendArgs& a, const Cell& c, uint32_t* lds) {
+  const int pairs = a.d8 / 2;
+  const int tid = threadIdx.x;
+  const int j = tid % pairs, off0 = 2 * (tid / pairs);
+  const bool active = off0 < 1 << a.page_shift;
+  const Pair pr = pair_of(a, j);
+  f32x8 x[2][2];
+  uint32_t peak = 0;
+  if (active && c.page_lo + off0 + 2 > c.lo && c.page_lo + off0 < c.hi) {
+    f32x8 cs[2], sn[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int pos = page_lo + off0 + i;
-      u32x2* at = reinterpret_cast<u32x2*>(base + i * 8 * a.d8);
-      if (pos >= lo && pos < hi) {
-        u32x2 w = {0, 0};
+    for (int i = 0; i < 2; ++i) {
+      // a slot that is not new reads the row of one that is, and drops it
+      const int pos = min(max(c.page_lo + off0 + i, c.lo), c.hi - 1);
+      const uint16_t* row = a.k.p + (int64_t)(c.first + (pos - c.start)) * a.k.token + (int64_t)c.head * a.k.head;
+      x[i][0] = load8(row + 8 * pr.v0), x[i][1] = load8(row + 8 * pr.v1);
+      if (pr.r0) angles(a, pos, pr, cs[i], sn[i]);
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j / 4] |= (uint32_t)(code_of(x[i][j], inverse) & 255) << (8 * (j % 4));
+    for (int i = 0; i < 2; ++i) {
+      rotate_pair(pr, a.interleaved, x[i][0], x[i][1], cs[i], sn[i]);
+      const int pos = c.page_lo + off0 + i;
+      if (!c.is_new(pos)) continue;
+      if (a.k_out.p) {
+        uint16_t* out = a.k_out.p + (int64_t)(c.first + (pos - c.start)) * a.k_out.token + (int64_t)c.head * a.k_out.head;
+        store8(out + 8 * pr.v0, x[i][0]);
+        store8(out + 8 * pr.v1, x[i][1]);
+      }
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t m = magnitude(x[i][v][e]);
+          peak = m > peak ? m : peak;
+        }
+    }
+  }
+  const Scaling s = rescale(c, peak, lds);
+  if (!active) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      u32x2* at = reinterpret_cast<u32x2*>(a.k_cache + ((c.cell << a.page_shift) + off0 + i) * (8 * a.d8) +
+                                           8 * (v ? pr.v1 : pr.v0));
+      u32x2 w = {0, 0};
+      if (c.is_new(c.page_lo + off0 + i)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e / 4] |= (uint32_t)(code_of(x[i][v][e], s.inverse) & 255) << (8 * (e % 4));
         *at = w;
-      } else if (grew && off0 + i < old_slots) {
+      } else if (s.grew && off0 + i < c.old_slots()) {
         const u32x2 old = *at;
-        u32x2 w = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          w[j / 4] |= (uint32_t)(code_of((float)byte_of(old[j / 4], j % 4), shrink) & 255) << (8 * (j % 4));
+        for (int e = 0; e < 8; ++e)
+          w[e / 4] |= (uint32_t)(code_of((float)byte_of(old[e / 4], e % 4), s.shrink) & 255) << (8 * (e % 4));
         *at = w;
       }
     }
-  } else {
-    int8_t* base = a.v_cache + ((cell * (8 * a.d8) + 8 * d8) << a.page_shift) + off0;
-    const bool full = page_lo + off0 >= lo && page_lo + off0 + 4 <= hi;
-    const bool olds = grew && off0 < old_slots;
-    const bool any_new = page_lo + off0 + 4 > lo && page_lo + off0 < hi;
-    if (!any_new && !olds) return;
+}
+
+// Values: a thread holds four neighbouring tokens at eight neighbouring
+// channels; four codes of a channel are one store of the layout
+// [page][channel][token].
+__device__ __forceinline__ void append_values(const AppendArgs& a, const Cell& c, uint32_t* lds) {
+  const int t4 = (1 << a.page_shift) / 4;
+  const int tid = threadIdx.x;
+  const int d8 = tid / t4, off0 = 4 * (tid % t4);
+  const bool active = d8 < a.d8;
+  const int pos0 = c.page_lo + off0;
+  const bool any_new = active && pos0 + 4 > c.lo && pos0 < c.hi;
+  f32x8 x[4];
+  uint32_t peak = 0;
+  if (any_new) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      int8_t* at = base + ((int64_t)j << a.page_shift);
-      uint32_t w = 0;
-      if (full) {
+    for (int i = 0; i < 4; ++i) {
+      const int pos = min(max(pos0 + i, c.lo), c.hi - 1);
+      x[i] = load8(a.v.p + (int64_t)(c.first + (pos - c.start)) * a.v.token + (int64_t)c.head * a.v.head + 8 * d8);
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= (uint32_t)(code_of(x[i][j], inverse) & 255) << (8 * i);
-        *reinterpret_cast<uint32_t*>(at) = w;
-      } else if (olds) {
-        const uint32_t old = *reinterpret_cast<const uint32_t*>(at);
+    for (int i = 0; i < 4; ++i)
+      if (c.is_new(pos0 + i))
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int pos = page_lo + off0 + i;
-          int c = byte_of(old, i);
-          if (pos >= lo && pos < hi) c = code_of(x[i][j], inverse);
-          else if (off0 + i < old_slots) c = code_of((float)c, shrink);
-          w |= (uint32_t)(c & 255) << (8 * i);
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t m = magnitude(x[i][e]);
+          peak = m > peak ? m : peak;
         }
-        *reinterpret_cast<uint32_t*>(at) = w;
-      } else {
+  }
+  const Scaling s = rescale(c, peak, lds);
+  const bool olds = active && s.grew && off0 < c.old_slots();
+  if (!any_new && !olds) return;
+  int8_t* base = a.v_cache + ((c.cell * (8 * a.d8) + 8 * d8) << a.page_shift) + off0;
+  const bool full = c.is_new(pos0) && c.is_new(pos0 + 3);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int pos = page_lo + off0 + i;
-          if (pos >= lo && pos < hi) at[i] = (int8_t)code_of(x[i][j], inverse);
-        }
+  for (int e = 0; e < 8; ++e) {
+    int8_t* at = base + ((int64_t)e << a.page_shift);
+    uint32_t w = 0;
+    if (full) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w |= (uint32_t)(code_of(x[i][e], s.inverse) & 255) << (8 * i);
+      *reinterpret_cast<uint32_t*>(at) = w;
+    } else if (olds) {
+      const uint32_t old = *reinterpret_cast<const uint32_t*>(at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int code = byte_of(old, i);
+        if (c.is_new(pos0 + i)) code = code_of(x[i][e], s.inverse);
+        else if (off0 + i < c.old_slots()) code = code_of((float)code, s.shrink);
+        w |= (uint32_t)(code & 255) << (8 * i);
       }
+      *reinterpret_cast<uint32_t*>(at) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c.is_new(pos0 + i)) at[i] = (int8_t)code_of(x[i][e], s.inverse);
     }
   }
 }
@@ -319,14 +329,14 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t job)
   const int pos = a.seq_lens[b] - n + (t - first);
   const Pair pr = pair_of(a, j);
   f32x8 c, s;
-  if (pr.rotated) angles(a, pos, 8 * j, c, s);
+  if (pr.r0) angles(a, pos, pr, c, s);
   const int h0 = chunk * a.q_heads_per_thread, h1 = min(h0 + a.q_heads_per_thread, a.heads_q);
 #pragma unroll 4
   for (int h = h0; h < h1; ++h) {
     const uint16_t* row = a.q.p + (int64_t)t * a.q.token + (int64_t)h * a.q.head;
     uint16_t* out = a.q_out.p + (int64_t)t * a.q_out.token + (int64_t)h * a.q_out.head;
     f32x8 x = load8(row + 8 * pr.v0), y = load8(row + 8 * pr.v1);
-    if (pr.rotated) rotate_pair(x, y, c, s, a.interleaved);
+    rotate_pair(pr, a.interleaved, x, y, c, s);
     if (pos < 0) x = y = (f32x8)(0.0f);
     store8(out + 8 * pr.v0, x);
     store8(out + 8 * pr.v1, y);
@@ -357,8 +367,19 @@ __global__ __launch_bounds__(1024) void kv8_append_kernel(AppendArgs a) {
   const int len = a.seq_lens[b];
   const int start = len - n;
   page += max(start, 0) >> a.page_shift;
-  if (kind == 0) append_page<true>(a, b, first, start, len, page, head, lds);
-  else append_page<false>(a, b, first, start, len, page, head, lds);
+  Cell c;
+  c.page_lo = page << a.page_shift;
+  c.lo = max(max(start, 0), c.page_lo), c.hi = min(len, c.page_lo + (1 << a.page_shift));
+  if (c.lo >= c.hi || page >= a.max_pages) return;
+  const int id = a.page_table[(int64_t)b * a.table_stride + page];
+  if ((unsigned)id >= (unsigned)a.num_pages) return;
+  c.start = start, c.first = first, c.head = head;
+  c.cell = (int64_t)id * a.heads_kv + head;
+  c.scale_at = (kind == 0 ? a.k_scale : a.v_scale) + c.cell;
+  c.kept = c.page_lo < start;
+  c.old_scale = c.kept ? *c.scale_at : 0.0f;
+  if (kind == 0) append_keys(a, c, lds);
+  else append_values(a, c, lds);
 }
 
 }  // namespace
@@ -420,7 +441,8 @@ extern "C" int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t 
   const int threads = (int)(page_size * head_dim / 32 < kWave ? kWave : page_size * head_dim / 32);
   // a thread's angles serve several heads once there are threads enough for the chip
   const int64_t lanes = tokens * (head_dim / 16);
-  a.q_heads_per_thread = lanes * heads_q >= (int64_t)8 * lbh::device_cus() * 2048 ? 8 : 1;
+  const int64_t shared = lanes * heads_q / ((int64_t)lbh::device_cus() * 1024);
+  a.q_heads_per_thread = shared < 1 ? 1 : shared > 8 ? 8 : (int)shared;
   const int64_t chunks = (heads_q + a.q_heads_per_thread - 1) / a.q_heads_per_thread;
   const int64_t q_blocks = queries ? (lanes * chunks + threads - 1) / threads : 0;
   if (kv_blocks + q_blocks > kIntMax) return LB_ERR_ARG;

@@ -54,6 +54,7 @@ constexpr float kSlack = 8.0f;
 constexpr int kLift = 7;
 constexpr int kNoExp = -1000;
 constexpr int kMinUnits = 2;
+constexpr int kJoinGroups = 16;  // groups of D / 4 threads that join a column's parts
 constexpr int kParts = 4;     // parts whose loads the joining workgroup has in flight
 constexpr int kFewParts = 16;  // up to here the last worker of a pair joins its parts, above a second launch
 
@@ -121,13 +122,22 @@ __device__ __forceinline__ Work work_of(const AttnArgs& a, int first_len) {
   int total = __builtin_amdgcn_readlane(wave_scan(units_or_none(first_len)), kWave - 1);
   for (int c = kWave; c < a.batch; c += kWave)
     total += __builtin_amdgcn_readlane(wave_scan(units_or_none(len_at(a, c + lane_id()))), kWave - 1);
-  const int pairs = a.batch * a.heads_kv * a.col_blocks;
+  const int per_seq = a.heads_kv * a.col_blocks, pairs = a.batch * per_seq;
   Work w;
-  w.units = total * a.heads_kv * a.col_blocks;
+  w.units = total * per_seq;
   w.slots = 4 * pairs <= a.workers;
-  // slots of `per` units: at most units / per + pairs of them, which is no more than the workers
-  const int among = w.slots ? a.workers - pairs : a.workers;
-  w.per = max((w.units + among - 1) / among, kMinUnits);
+  w.per = max((w.units + a.workers - 1) / a.workers, kMinUnits);
+  // the smallest slots of which there are no more than workers (at the latest
+  // `per` = units / (workers - pairs), as there are at most units / per + pairs)
+  while (w.slots) {
+    int slots = 0;
+    for (int c = 0; c < a.batch; c += kWave) {
+      const int nu = units_or_none(c ? len_at(a, c + lane_id()) : first_len);
+      slots += __builtin_amdgcn_readlane(wave_scan((nu + w.per - 1) / w.per), kWave - 1);
+    }
+    if (slots * per_seq <= a.workers) break;
+    ++w.per;
+  }
   return w;
 }
 
@@ -635,8 +645,8 @@ __global__ __launch_bounds__(kThreads<D>, (kPerCu<D, NQ>)) void kv8_attention_ke
 // pair a workgroup: D / 4 threads a part, the parts dealt to the thread groups
 // in turn and their sums added in group order.
 template <int D, int NQ>
-__global__ __launch_bounds__(256) void kv8_join_kernel(AttnArgs a) {
-  constexpr int COLS = 16 * NQ, T = D / 4, GROUPS = 256 / T;
+__global__ __launch_bounds__(kJoinGroups * D / 4) void kv8_join_kernel(AttnArgs a) {
+  constexpr int COLS = 16 * NQ, T = D / 4, GROUPS = kJoinGroups;
   __shared__ float sm[GROUPS], sl[GROUPS];
   __shared__ f32x4 so[GROUPS][T];
   const int pairs = a.heads_kv * a.col_blocks;
@@ -738,7 +748,7 @@ void launch(const AttnArgs& a, const Plan& p, hipStream_t st) {
   // 64 and 128 channels: up to 16 columns are always one block
   if (p.col_blocks == 1) kv8_attention_kernel<D, NQ, true><<<grid, block, 0, st>>>(a);
   else if constexpr (D == 256 || NQ == 2) kv8_attention_kernel<D, NQ, false><<<grid, block, 0, st>>>(a);
-  if (p.joined) kv8_join_kernel<D, NQ><<<dim3((unsigned)(p.counters * 16 * NQ)), dim3(256), 0, st>>>(a);
+  if (p.joined) kv8_join_kernel<D, NQ><<<dim3((unsigned)(p.counters * 16 * NQ)), dim3(kJoinGroups * D / 4), 0, st>>>(a);
 }
 
 }  // namespace

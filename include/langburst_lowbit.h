@@ -263,7 +263,7 @@ int lb_marlin_dequant(const int32_t* B, const uint16_t* s, uint16_t* w_nk,
  * A page's scale is max |x| / 127 over its tokens when they enter.  A page that
  * holds earlier tokens of the sequence keeps its scale unless the new tokens
  * need a larger one, and then its codes are rescaled.  A non-finite key or
- * value makes the scale non-finite.
+ * value makes the scale non-finite, and so it stays while the page is filled.
  * q and q_out may be NULL together (no queries); q_out may be q.  k_out, when
  * given, receives the rotated keys and must not be k.  A token before position
  * 0 (seq_lens[b] below the sequence's new tokens) is padding: its q_out row is

@@ -171,10 +171,10 @@ struct Scaling {
 __device__ __forceinline__ Scaling rescale(const Cell& c, uint32_t peak, uint32_t* lds) {
   peak = block_max(peak, lds);
   const float need = __builtin_bit_cast(float, peak) * (1.0f / 127.0f);
-  // `need` may be NaN: then it is taken
-  const float scale = need <= c.old_scale ? c.old_scale : need;
+  // NaN on either side stays: a page that held it once has no codes to rescale
+  const float scale = need <= c.old_scale || c.old_scale != c.old_scale ? c.old_scale : need;
   Scaling s;
-  s.grew = c.kept && scale != c.old_scale;
+  s.grew = c.kept && scale != c.old_scale && c.old_scale == c.old_scale;
   if (threadIdx.x == 0 && (scale != c.old_scale || !c.kept)) *c.scale_at = scale;
   s.inverse = scale > 0.0f ? 1.0f / scale : 0.0f;
   s.shrink = s.grew ? c.old_scale / scale : 1.0f;

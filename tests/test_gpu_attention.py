@@ -264,6 +264,26 @@ def test_append_shows_non_finite_values_and_positions_outside_the_table(dev):
     assert np.isnan(ks[c.table_np[0, 1]]).all()  # its keys have no angle
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_append_to_a_page_with_a_non_finite_scale_keeps_it(dev, bad):
+    import langburst_cuda as lc
+    import torch
+
+    print_case("append-after-non-finite", bad)
+    c = AppendCase(dev, [0, 0], [20, 20], 2, 1, 64, 16, 64, seed=4, positions=32)
+    c.k[17, 0, 5], c.v[37, 0, 7] = bad, bad  # the second page of sequence 0, and of sequence 1
+    c.run(lc, False)
+    table = c.table_np[:, 1]
+    for _ in range(2):  # finite tokens after it: what the page held is not known any more, and must not look finite
+        c.k[17, 0, 5], c.v[37, 0, 7] = 1.0, 1.0
+        lens = c.seq_lens + 1
+        rows = torch.tensor([17, 37], device=dev)
+        lc.kv8_append_out(None, c.k[rows].contiguous(), c.v[rows].contiguous(), c.k_cache, c.v_cache, c.k_scale, c.v_scale,
+                          c.table, lens, None, c.rotation, None, None, False)
+        ks, vs = _np(c.k_scale)[table, 0], _np(c.v_scale)[table, 0]
+        assert not np.isfinite(ks[0]) and np.isfinite(ks[1]) and np.isfinite(vs[0]) and not np.isfinite(vs[1])
+
+
 def test_append_of_nothing(dev):
     import langburst_cuda as lc
     import torch

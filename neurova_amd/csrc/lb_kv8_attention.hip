@@ -349,9 +349,11 @@ struct Walk {
     resolve(sg, tb);
     fetch_after(sg, tb + kUnit, ahead, to);
     load_k();
+    __builtin_amdgcn_sched_barrier(0);  // the values' loads after the keys'
     load_scales();
 #pragma unroll
     for (int d = 0; d < VT; ++d) load_v(d);
+    __builtin_amdgcn_sched_barrier(0);
     loaded = true;
   }
 
@@ -361,6 +363,12 @@ struct Walk {
   __device__ __forceinline__ void step(const Segment& sg, int tb, f32x4 (&o)[NQ][VT], float (&m)[NQ], float (&l)[NQ],
                                        int& e, bool ahead, const Segment& to) {
     const bool held0 = held;
+    // the keys are in LDS once no more loads are out than those of the values,
+    // which follow theirs (nothing else waits for a load into LDS here)
+    static_assert(VT < 16, "the low bits of the counter");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | VT);  // vmcnt(VT)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
     u32x4 kw[4][KI];
 #pragma unroll
     for (int t = 0; t < 4; ++t)

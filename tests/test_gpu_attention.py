@@ -403,6 +403,22 @@ def test_attention_over_the_cache_flat_and_sharp_scores(dev, sharp, scale):
     c.check(c.run(lc, scale=scale), scale=scale)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 64), (8, 2, 128), (6, 1, 256)])
+def test_attention_over_the_cache_with_cold_caches(dev, hq, hkv, d):
+    """One step of tokens a workgroup, and nothing of them in the GPU's caches: the loads take their longest."""
+    import langburst_cuda as lc
+    import torch
+
+    print_case("kv8-attention-cold", hq, hkv, d)
+    c = Cached(dev, [40, 256, 7000], 1, hq, hkv, d, 64, seed=4)
+    c.check(c.run(lc))
+    want = c.run(lc)
+    flush = torch.empty(2 ** 29, dtype=torch.uint8, device=dev)
+    for i in range(20):
+        flush.fill_(i)
+        assert torch.equal(c.run(lc), want), i
+
+
 def test_attention_over_pages_of_very_different_scales(dev):
     import langburst_cuda as lc
 

@@ -39,7 +39,7 @@ struct AttnArgs {
   int num_pages, page_shift, max_tokens;
   int batch, new_tokens, heads_kv, group;
   int col_blocks;
-  int workers, joined;  // joined: a second launch joins the parts
+  int workers, cus, min_units, joined;  // joined: a second launch joins the parts
   float scale;  // softmax scale * log2(e)
 };
 
@@ -53,10 +53,17 @@ constexpr float kNoMax = -1e30f;
 constexpr float kSlack = 8.0f;
 constexpr int kLift = 7;
 constexpr int kNoExp = -1000;
-constexpr int kMinUnits = 2;
-constexpr int kJoinGroups = 16;  // groups of D / 4 threads that join a column's parts
-constexpr int kParts = 4;     // parts whose loads the joining workgroup has in flight
-constexpr int kFewParts = 16;  // up to here the last worker of a pair joins its parts, above a second launch
+// Slots may be this many units longer if each then has a compute unit to itself:
+// 5 sequences of 700 to 6000 tokens, 3 new ones, 8 heads of 128: 18.0 us with 3
+// units in 200 slots, 19.3 with 2 in 280, where the last 24 share theirs.
+constexpr int kAlone = 1;
+// Up to 16 parts of a pair are joined by its last worker (4000 tokens, 8 heads of
+// 128: 11.2 us, 12.6 with a second launch); above that a second launch takes a
+// workgroup for each column (131072 tokens: 182 us with the last worker, 56).
+constexpr int kFewParts = 16;
+constexpr int kParts = 8;        // parts whose loads a thread of the last worker has in flight: 32768
+                                 // tokens beside 15 x 300: 30.6 us, 4 at a time 35.8, 16 the same
+constexpr int kJoinGroups = 16;  // groups of D / 4 threads that join a column's parts in the second launch
 
 // Sixteen signed bytes -> two MFMA fragments of eight fp16 (exact): the byte
 // with its sign flipped under the exponent of 1024 is 1024 + 128 + c.
@@ -118,6 +125,28 @@ __device__ __forceinline__ int len_at(const AttnArgs& a, int b) {
 // Units of a sequence's pairs; 0 past the batch (length -1).
 __device__ __forceinline__ int units_or_none(int len) { return len < 0 ? 0 : units_of(len); }
 
+// Slots of a pair: ceil(nu / per), for nu <= 2^20 and per <= nu or so.  A float
+// product is exact enough: (x + 1/2) / per is 1 / (2 per) away from an integer,
+// more than its error of x / per * 2^-22.
+__device__ __forceinline__ int slots_in(int nu, int per, float inverse) {
+  return (int)(((float)(nu + per - 1) + 0.5f) * inverse);
+}
+
+// The smallest slots from `per` to `last` units of which there are at most
+// `most`; 0 if there are none.
+__device__ __forceinline__ int slots_for(const AttnArgs& a, int first_len, int per, int last, int most) {
+  const int per_seq = a.heads_kv * a.col_blocks;
+  for (; per <= last; ++per) {
+    const float inverse = __builtin_amdgcn_rcpf((float)per);
+    int slots = 0;
+    for (int c = 0; c < a.batch; c += kWave)
+      slots += __builtin_amdgcn_readlane(
+          wave_scan(slots_in(units_or_none(c ? len_at(a, c + lane_id()) : first_len), per, inverse)), kWave - 1);
+    if (slots * per_seq <= most) return per;
+  }
+  return 0;
+}
+
 __device__ __forceinline__ Work work_of(const AttnArgs& a, int first_len) {
   int total = __builtin_amdgcn_readlane(wave_scan(units_or_none(first_len)), kWave - 1);
   for (int c = kWave; c < a.batch; c += kWave)
@@ -126,17 +155,12 @@ __device__ __forceinline__ Work work_of(const AttnArgs& a, int first_len) {
   Work w;
   w.units = total * per_seq;
   w.slots = 4 * pairs <= a.workers;
-  w.per = max((w.units + a.workers - 1) / a.workers, kMinUnits);
-  // the smallest slots of which there are no more than workers (at the latest
-  // `per` = units / (workers - pairs), as there are at most units / per + pairs)
-  while (w.slots) {
-    int slots = 0;
-    for (int c = 0; c < a.batch; c += kWave) {
-      const int nu = units_or_none(c ? len_at(a, c + lane_id()) : first_len);
-      slots += __builtin_amdgcn_readlane(wave_scan((nu + w.per - 1) / w.per), kWave - 1);
-    }
-    if (slots * per_seq <= a.workers) break;
-    ++w.per;
+  w.per = max((w.units + a.workers - 1) / a.workers, a.min_units);
+  if (w.slots) {
+    const int alone = max((w.units + a.cus - 1) / a.cus, a.min_units);
+    const int per = a.workers > a.cus ? slots_for(a, first_len, alone, w.per + kAlone, a.cus) : 0;
+    // at the latest units / (workers - pairs): there are at most units / per + pairs
+    w.per = per ? per : slots_for(a, first_len, w.per, w.units, a.workers);
   }
   return w;
 }
@@ -582,48 +606,36 @@ struct Walk {
 
   __device__ __forceinline__ void join(const Segment& sg, int live) {
     after_last_arrival();
-    for (int x0 = threadIdx.x; x0 < live * (D / 4); x0 += 2 * kThreads<D>) {
-      // two columns and channels a thread, kParts parts each: all their loads in flight
-      float up[2] = {kNoMax, kNoMax}, sum[2] = {0.0f, 0.0f};
-      f32x4 v[2] = {(f32x4)(0.0f), (f32x4)(0.0f)};
-      const bool both = x0 + kThreads<D> < live * (D / 4);
+    for (int x = threadIdx.x; x < live * (D / 4); x += kThreads<D>) {
+      const int c = x / (D / 4), d = 4 * (x % (D / 4));
+      float up = kNoMax, sum = 0.0f;
+      f32x4 v = (f32x4)(0.0f);
       for (int w0 = sg.w_first; w0 <= sg.w_last; w0 += kParts) {
-        float pm[2][kParts], pl[2][kParts];
-        f32x4 po[2][kParts];
+        float pm[kParts], pl[kParts];
+        f32x4 po[kParts];
 #pragma unroll
-        for (int i = 0; i < kParts; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            pm[j][i] = kNoMax, pl[j][i] = 0.0f, po[j][i] = (f32x4)(0.0f);
-            if (w0 + i <= sg.w_last) {
-              const int x = both ? x0 + j * kThreads<D> : x0;
-              const int c = x / (D / 4), d = 4 * (x % (D / 4));
-              const __amdgpu_buffer_rsrc_t from =
-                  buffer_of(a.parts + part_at<D, NQ>(w0 + i, sg.w_first), kPartFloats<D, NQ> * 4);
-              pm[j][i] = collect4(from, c * 4);
-              pl[j][i] = collect4(from, (COLS + c) * 4);
-              po[j][i] = collect16(from, (2 * COLS + c * D + d) * 4);
-            }
-          }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float top = up[j];
-#pragma unroll
-          for (int i = 0; i < kParts; ++i) top = __builtin_fmaxf(top, pm[j][i]);
-          const float f0 = __builtin_amdgcn_exp2f(up[j] - top);
-          up[j] = top, sum[j] *= f0, v[j] *= f0;
-#pragma unroll
-          for (int i = 0; i < kParts; ++i) {
-            const float f = __builtin_amdgcn_exp2f(pm[j][i] - top);
-            sum[j] += pl[j][i] * f, v[j] += po[j][i] * f;
+        for (int i = 0; i < kParts; ++i) {
+          pm[i] = kNoMax, pl[i] = 0.0f, po[i] = (f32x4)(0.0f);
+          if (w0 + i <= sg.w_last) {
+            const __amdgpu_buffer_rsrc_t from =
+                buffer_of(a.parts + part_at<D, NQ>(w0 + i, sg.w_first), kPartFloats<D, NQ> * 4);
+            pm[i] = collect4(from, c * 4);
+            pl[i] = collect4(from, (COLS + c) * 4);
+            po[i] = collect16(from, (2 * COLS + c * D + d) * 4);
           }
         }
-      }
+        float top = up;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int x = x0 + j * kThreads<D>;
-        if (j == 0 || both) store_out(a, sg.b, sg.head, sg.cb * COLS + x / (D / 4), 4 * (x % (D / 4)), v[j], sum[j]);
+        for (int i = 0; i < kParts; ++i) top = __builtin_fmaxf(top, pm[i]);
+        const float f0 = __builtin_amdgcn_exp2f(up - top);
+        up = top, sum *= f0, v *= f0;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          const float f = __builtin_amdgcn_exp2f(pm[i] - top);
+          sum += pl[i] * f, v += po[i] * f;
+        }
       }
+      store_out(a, sg.b, sg.head, sg.cb * COLS + c, d, v, sum);
     }
     if (threadIdx.x == 0) reset_counter(a.counters + sg.pair);
   }
@@ -708,7 +720,7 @@ __global__ __launch_bounds__(kJoinGroups * D / 4) void kv8_join_kernel(AttnArgs 
 }
 
 struct Plan {
-  int nq, col_blocks, joined;
+  int nq, col_blocks, min_units, joined;
   int64_t workers, counters;
   size_t scratch;
 };
@@ -729,7 +741,8 @@ Plan plan_of(int64_t batch, int64_t new_tokens, int64_t heads_q, int64_t heads_k
   // parts of a pair where all sequences fill the table (with one long sequence
   // among short ones it may have more; the last worker then joins those too)
   const int64_t per = (p.counters * units + p.workers - 1) / p.workers;
-  p.joined = units / (per > kMinUnits ? per : kMinUnits) + 1 > kFewParts;
+  p.min_units = p.nq;
+  p.joined = units / (per > p.min_units ? per : p.min_units) + 1 > kFewParts;
   p.scratch = ((size_t)p.workers * 2 * 16 * p.nq * (head_dim + 2) * 4 + 255) & ~(size_t)255;
   return p;
 }
@@ -805,7 +818,7 @@ extern "C" int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64
   a.max_tokens = num_pages > 0 ? (int)(max_pages * page_size) : 0;
   a.batch = (int)batch, a.new_tokens = (int)(tokens / batch), a.heads_kv = (int)heads_kv;
   a.group = (int)(heads_q / heads_kv), a.col_blocks = p.col_blocks;
-  a.workers = (int)p.workers, a.joined = p.joined;
+  a.workers = (int)p.workers, a.cus = lbh::device_cus(), a.min_units = p.min_units, a.joined = p.joined;
   a.scale = softmax_scale * kLog2e;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (head_dim == 256) launch<256, 1>(a, p, st);

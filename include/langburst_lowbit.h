@@ -282,7 +282,9 @@ int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stri
                   const float* cos_sin, int64_t positions, int64_t rot_dim, int32_t interleaved,
                   lb_stream_t stream);
 
-/* out = softmax(softmax_scale * q k^T) v over the cache, one launch.  The
+/* out = softmax(softmax_scale * q k^T) v over the cache: one launch, or a second
+ * one that joins the parts of a sequence where its table is long for the number
+ * of sequences and key/value heads (which depends on the sizes alone).  The
  * tokens / batch newest tokens of every sequence are the queries; token i of n
  * sees the keys 0 to seq_lens[b] - n + i, and a row that sees none is zero.
  * Scores, softmax and sums are fp32; a weight times its value scale is rounded
@@ -308,8 +310,9 @@ int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_s
  * i of the same sequence.  cu_seqlens NULL: one sequence (batch 1) of all
  * tokens.  Scores, softmax and sums are fp32, weights fp16 for the second
  * product.  Rows of tokens that belong to no sequence are left as they are.
- * A non-finite value may reach every row of its sequence from up to 63 tokens
- * before it on, but no other sequence.  softmax_scale positive and finite. */
+ * A non-finite key or value may reach every row of its sequence from up to 127
+ * tokens before it on (the rows that go through its tile of keys; a weight of
+ * zero times infinity), but no other sequence.  softmax_scale positive and finite. */
 int lb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                         const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
                         const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride,

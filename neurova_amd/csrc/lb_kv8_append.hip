@@ -10,6 +10,13 @@
 // The rotation and the codes are computed with each product and sum rounded to
 // fp32 by itself (no contraction), so a program that repeats the definition in
 // 32 bits gets the same codes.
+//
+// Bound by memory: each row is read and written once.  A workgroup holds one head
+// of one page, keys or values, in registers, since every code waits for the
+// page's largest value; the workgroups of the queries run beside them.  16384
+// tokens, 40 / 8 heads of 128: 102 us, 4.5 TB/s where a large copy reaches 5.0; one
+// token: 5.2 us, a launch and the loads that wait for one another (length, page,
+// scale and rows).
 #include "attn_common.hpp"
 
 namespace lb {
@@ -439,7 +446,9 @@ extern "C" int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t 
   const int64_t items = cu_seqlens ? tokens / page_size + 2 * batch : batch * a.page_bound;
   const int64_t kv_blocks = items * heads_kv * 2;
   const int threads = (int)(page_size * head_dim / 32 < kWave ? kWave : page_size * head_dim / 32);
-  // a thread's angles serve several heads once there are threads enough for the chip
+  // a thread's angles serve several heads once there are threads enough for the
+  // chip (16384 tokens, 40 heads: 102 us with eight, 104 with one; 64 tokens: 4.7 us
+  // with one, 6.1 with eight)
   const int64_t lanes = tokens * (head_dim / 16);
   const int64_t shared = lanes * heads_q / ((int64_t)lbh::device_cus() * 1024);
   a.q_heads_per_thread = shared < 1 ? 1 : shared > 8 ? 8 : (int)shared;

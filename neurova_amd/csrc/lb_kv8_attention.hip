@@ -18,6 +18,13 @@
 // weights go from the first product to the second without leaving the lane, and
 // a lane's tokens share a page (pages hold 16 tokens or more), so both scales
 // are one number a lane and step.
+//
+//   128 sequences of 500 to 8192 tokens, 8 heads of 128: 123 us, 5.4 TB/s where
+//   reads alone reach 6.2; one of 131072 tokens, 4 heads of 256: 56 us (4.8 TB/s;
+//   51.5 and 4.7 for the join).  Few tokens are bound by the chain of loads that
+//   wait for one another (length, page, keys) and a step's instructions, 800 a
+//   wave: 301 tokens, 4 heads of 256: 10.8 us, of which 2 are the two loads before
+//   the keys, 4 the first step, 1.7 the output.
 #include <type_traits>
 
 #include "attn_common.hpp"
@@ -85,7 +92,8 @@ __device__ __forceinline__ void codes_to_half(u32x4 w, f16x8& a, f16x8& b) {
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnit - 1) / kUnit : 1; }
 
 // Head dimension 256 is two waves of 128 channels for each stream of tokens (the
-// registers of all 256 would leave one wave a SIMD): each sums the scores over
+// registers of all 256 would leave one wave a SIMD; 301 tokens took 14.2 us so,
+// 12.5 with the halves): each sums the scores over
 // its half, the halves are exchanged through LDS, and both carry the same
 // softmax for their half of the output.
 template <int D>
@@ -111,9 +119,10 @@ struct Shared {
 // How a launch's work is cut.  A pair (sequence, key/value head, column block)
 // has `nu` units.  With many pairs the workgroups take equal contiguous ranges
 // of all units, numbered pair by pair, so one may end a pair and begin the
-// next.  With few pairs each is cut into slots of its own, `per` units or a
-// little less, one a workgroup: the fixed time of a segment (its first loads,
-// the join) is then paid once.
+// next.  With few pairs, up to a quarter of the workers, each is cut into slots
+// of its own, `per` units or a little less, one a workgroup: the fixed time of a
+// segment (its first loads, the join) is then paid once (5 sequences of 700 to
+// 6000 tokens, 3 new ones: 18.6 us, with ranges 25.6).
 struct Work {
   int units, per;
   bool slots;
@@ -725,8 +734,14 @@ struct Plan {
   size_t scratch;
 };
 
-// Two workgroups a compute unit; fewer where the longest possible sequences
-// hold fewer units.
+// A worker for each workgroup that the compute units hold at once; fewer where the
+// longest possible sequences hold fewer units.  Up to 16 columns (query heads of
+// a group times new tokens) are one column group, above that two at a time share
+// a key or value's conversion, but for 256 channels, where they do not fit the
+// registers.  The smallest slot is one unit for one column group and two for two,
+// whose parts take twice the work to join (1000 tokens, 8 heads of 128, one new:
+// 9.5 us, with two units 11.2; four new, 20 columns, 3000 tokens: 20.6, with two
+// units 19.0).
 Plan plan_of(int64_t batch, int64_t new_tokens, int64_t heads_q, int64_t heads_kv, int64_t head_dim,
              int64_t max_tokens) {
   Plan p;

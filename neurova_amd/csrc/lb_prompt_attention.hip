@@ -2,14 +2,26 @@
 //
 //   o[i] = sum_{j <= i} softmax_j(scale q[i] . k[j]) v[j]      per sequence and query head
 //
-// Bound by the matrix cores: 4 head_dim flop a query, key and head.  The rows of
-// a tile are (token, query head of the group) pairs of one key/value head, so a
-// tile of 256 rows spans few tokens: its waves end at the same keys and little
-// work falls past the diagonal.
-//
 //   S^T = K Q^T    32x32x16: a lane holds 16 keys of one row, so a row's maximum
 //                  and sum stay in the lane but for one exchange with lane ^ 32
 //   O^T = V^T P^T  the weights of a lane are already the second product's operand
+//
+// The 128 rows of a workgroup are (token, query head of the group) pairs of one
+// key/value head: a tile of 64 keys serves the whole group, the rows span few
+// tokens, and little work falls past the diagonal.  Four waves of 32 rows go
+// through the keys together, with the next tile on its way into LDS.
+//
+// Bound by the matrix cores and, as much, by LDS: a product of 32 cycles reads
+// 1 KB of keys or values, so four waves ask for all of the 128 bytes a cycle of a
+// compute unit.  64 rows a wave would halve that, but at 256 channels their
+// accumulators, queries and scores do not fit the registers, and at 128 they leave
+// one wave a SIMD, with nothing to run beside its softmax (8192 tokens: 920 us
+// where 32 rows took 742).
+//   8192 tokens, 40 / 8 heads of 128: 660 us, 1040 TFLOP/s of the 1154 that a large
+//   library product reaches (without exponentials 5 % less time, without reading
+//   the keys 23 %); 16384 tokens, 24 / 4 heads of 256: 3440 us, 960 TFLOP/s; 7
+//   packed prompts of 100 to 1500 tokens, same heads: 103 us, of which each
+//   workgroup spends 7 on its first loads and its output.
 #include "attn_common.hpp"
 
 namespace lb {
@@ -32,6 +44,11 @@ constexpr float kSlack = 8.0f, kLift = 7.0f;
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __fp16 fp16x4 __attribute__((__vector_size__(8)));
+
+// A weight is rounded to fp16 for the second product, its sum taken before that in
+// fp32: an error of at most 2^-12 sum p |v|, as large as the output's own rounding
+// where the values have one sign.  A second fp16 number for the rest, as over the
+// cache, would double that product where the matrix cores are the bound.
 
 // Sixteen-byte chunks of a key (value) row change places so that the 16-byte
 // reads of 16 rows at one column, and the transposing reads of 8 rows at one
@@ -63,7 +80,8 @@ struct Stage {
 };
 
 // The tiles with the most keys come first, whichever sequence they are of: a
-// workgroup's time is its number of keys, and short ones last fill the ends.
+// workgroup's time is its number of keys, and short ones last fill the ends (7
+// packed prompts: 111 us, in the order of the sequences 133).
 struct Place {
   int first, len, tile;  // of the sequence: its first token and length
 };
@@ -121,11 +139,11 @@ __device__ __forceinline__ Place place_of(const PromptArgs& a, int i) {
   return {0, 0, 0};
 }
 
-template <int D, int KT, int RB, int W, int PER_SIMD>
+template <int D, int KT, int W, int PER_SIMD>
 __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(PromptArgs a) {
-  constexpr int ROWS = W * RB * 32, DT = D / 32, KK = D / 16, ST = KT / 32;
+  constexpr int ROWS = W * 32, DT = D / 32, KK = D / 16, ST = KT / 32;
   // four arrays and not one: the compiler would make every read of a tile wait
-  // for the loads of the next into the same array
+  // for the loads of the next into the same array (16384 tokens: 3570 us, 4046)
   __shared__ __align__(16) uint16_t k0[KT * D], k1[KT * D], v0[KT * D], v1[KT * D];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 31, h = lane >> 5;
@@ -140,39 +158,31 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
   if (row0 >= rows) return;
   const int last_token = (min(rows, row0 + ROWS) - 1) / a.group;
   const int tiles = last_token / KT + 1;
-  const int wave_row = row0 + wave * RB * 32;
+  const int wave_row = row0 + wave * 32;
   const int wave_first = wave_row / a.group;  // token of the wave's first row
 
-  f16x8 qf[RB][KK];
-  int seen[RB];  // the last key of the lane's row
-#pragma unroll
-  for (int n = 0; n < RB; ++n) {
-    const int row = wave_row + 32 * n + r;
-    const int t = row / a.group;
-    seen[n] = row < rows ? t : -1;
-    const uint16_t* p = a.q + (int64_t)(first + t) * a.q_token + (int64_t)(kvh * a.group + row - t * a.group) * a.q_head;
+  const int row = wave_row + r, token = row / a.group, head = kvh * a.group + row - token * a.group;
+  const int seen = row < rows ? token : -1;  // the last key of the lane's row
+  f16x8 qf[KK];
+  {
+    const uint16_t* p = a.q + (int64_t)(first + token) * a.q_token + (int64_t)head * a.q_head;
 #pragma unroll
     for (int k = 0; k < KK; ++k) {
-      qf[n][k] = (f16x8)((f16)0.0f);
-      if (row < rows) qf[n][k] = *reinterpret_cast<const f16x8*>(p + 16 * k + 8 * h);
+      qf[k] = (f16x8)((f16)0.0f);
+      if (row < rows) qf[k] = *reinterpret_cast<const f16x8*>(p + 16 * k + 8 * h);
     }
   }
   const uint16_t* kbase = a.k + (int64_t)first * a.k_token + (int64_t)kvh * a.k_head;
   const uint16_t* vbase = a.v + (int64_t)first * a.v_token + (int64_t)kvh * a.v_head;
 
-  typedef float f32x16_t __attribute__((ext_vector_type(16)));
-  f32x16_t o[RB][DT];
-  float m[RB], l[RB];
+  f32x16 o[DT];
+  float m = kNoMax, l = 0.0f;
 #pragma unroll
-  for (int n = 0; n < RB; ++n) {
-    m[n] = kNoMax, l[n] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[n][d] = (f32x16_t)(0.0f);
-  }
+  for (int d = 0; d < DT; ++d) o[d] = (f32x16)(0.0f);
 
   typedef Stage<D, KT, W, true> Keys;
   typedef Stage<D, KT, W, false> Values;
-  static_assert(Keys::N + Values::N == KK * RB, "one load of the next tile for each channel step of the scores");
+  static_assert(Keys::N + Values::N == KK, "one load of the next tile for each channel step of the scores");
   const int k_token = (int)a.k_token, v_token = (int)a.v_token;
   {
     const Keys keys(kbase, k_token, len);
@@ -195,12 +205,10 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
       if (j < Keys::N) keys.load(j, k_token, kn, wave, lane);
       else values.load(j - Keys::N, v_token, vn, wave, lane);
     };
-    f32x16_t s[RB][ST];
+    f32x16 s[ST];
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int t = 0; t < ST; ++t)
-#pragma unroll
-      for (int n = 0; n < RB; ++n) s[n][t] = (f32x16_t)(0.0f);
+    for (int t = 0; t < ST; ++t) s[t] = (f32x16)(0.0f);
     constexpr int CH = KK / 4;  // channel steps of a quarter
     f16x8 kf[2][CH][ST];
     auto read_k = [&](int q) {
@@ -221,49 +229,44 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
       for (int k = 0; k < CH; ++k)
 #pragma unroll
         for (int t = 0; t < ST; ++t)
-#pragma unroll
-          for (int n = 0; n < RB; ++n)
-            s[n][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[q & 1][k][t], qf[n][q * CH + k], s[n][t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[q & 1][k][t], qf[q * CH + k], s[t], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < CH; ++k) load_next(q * CH + k);
       __builtin_amdgcn_sched_barrier(0);
     }
-    f16x8 pf[RB][2 * ST];
-#pragma unroll
-    for (int n = 0; n < RB; ++n) {
-      if (kt * KT + KT - 1 > wave_first) {
-        const int past = seen[n] - kt * KT - 4 * h;  // keys of the lane up to here are seen
-#pragma unroll
-        for (int t = 0; t < ST; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * t + 8 * (i >> 2) + (i & 3) > past) s[n][t][i] = -__builtin_inff();
-      }
-      float peak = kNoMax;
+    if (kt * KT + KT - 1 > wave_first) {
+      const int past = seen - kt * KT - 4 * h;  // keys of the lane up to here are seen
 #pragma unroll
       for (int t = 0; t < ST; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) peak = __builtin_fmaxf(peak, s[n][t][i]);
-      peak *= a.scale;
-      if (__any(peak > m[n] + kSlack)) {
-        const float up = __builtin_fmaxf(__builtin_fmaxf(peak, from_lane(peak, lane ^ 32)), m[n]);
-        const float f = __builtin_amdgcn_exp2f(m[n] - up);
-        m[n] = up;
-        l[n] *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[n][d] *= f;
-      }
-      const float lift = kLift - m[n];
-#pragma unroll
-      for (int t = 0; t < ST; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(s[n][t][i] * a.scale + lift);
-          l[n] += p;
-          pf[n][2 * t + i / 8][i % 8] = (f16)p;
-        }
+        for (int i = 0; i < 16; ++i)
+          if (32 * t + 8 * (i >> 2) + (i & 3) > past) s[t][i] = -__builtin_inff();
     }
+    float peak = kNoMax;
+#pragma unroll
+    for (int t = 0; t < ST; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) peak = __builtin_fmaxf(peak, s[t][i]);
+    peak *= a.scale;
+    if (__any(peak > m + kSlack)) {
+      const float up = __builtin_fmaxf(__builtin_fmaxf(peak, from_lane(peak, lane ^ 32)), m);
+      const float f = __builtin_amdgcn_exp2f(m - up);
+      m = up;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
+    f16x8 pf[2 * ST];
+    const float lift = kLift - m;
+#pragma unroll
+    for (int t = 0; t < ST; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(s[t][i] * a.scale + lift);
+        l += p;
+        pf[2 * t + i / 8][i % 8] = (f16)p;
+      }
 #pragma unroll
     for (int c = 0; c < 2 * ST; ++c) {
 #pragma unroll
@@ -278,8 +281,7 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
 #pragma unroll
           for (int i = 0; i < 4; ++i) vf[4 * u + i] = x[i];
         }
-#pragma unroll
-        for (int n = 0; n < RB; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[n][c], o[n][d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[c], o[d], 0, 0, 0);
       }
     }
   };
@@ -291,46 +293,43 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
 
   // The rows leave through LDS (a wave's 32 x D in an array that no wave reads
   // any more): a store then takes whole rows, where a lane's accumulators are
-  // four channels of a row each.  Chunks change places as in the tiles.
+  // four channels of a row each (97 tokens: 7.1 us, 7.9 without).  Chunks change
+  // places as in the tiles.
   lds_barrier();
   uint16_t* mine = wave < 2 ? (wave == 0 ? k0 : k1) : (wave == 2 ? v0 : v1);
   static_assert(W == 4 && KT >= 32, "one array a wave");
+  l += from_lane(l, lane ^ 32);
+  const float inv = 1.0f / l;
+  const int64_t place = (int64_t)(first + token) * a.o_token + (int64_t)head * a.o_head;
 #pragma unroll
-  for (int n = 0; n < RB; ++n) {
-    l[n] += from_lane(l[n], lane ^ 32);
-    const float inv = 1.0f / l[n];
-    const int row = wave_row + 32 * n + r, t = row / a.group;
-    const int64_t place = (int64_t)(first + t) * a.o_token + (int64_t)(kvh * a.group + row - t * a.group) * a.o_head;
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        u32x2 w;
-        w[0] = as_u32((f16x2){(f16)(o[n][d][i] * inv), (f16)(o[n][d][i + 1] * inv)});
-        w[1] = as_u32((f16x2){(f16)(o[n][d][i + 2] * inv), (f16)(o[n][d][i + 3] * inv)});
-        const int chunk = (4 * d + i / 4) ^ k_swizzle<D>(r);
-        *reinterpret_cast<u32x2*>(mine + r * D + 8 * chunk + 4 * h) = w;
-      }
-#pragma unroll
-    for (int j = 0; j < 32 * D / 8 / kWave; ++j) {
-      const int x = j * kWave + lane, rr = x / (D / 8), chunk = x % (D / 8);
-      const uint32_t lo = from_lane((uint32_t)place, rr), hi = from_lane((uint32_t)(place >> 32), rr);
-      const u32x4 w = *reinterpret_cast<const u32x4*>(mine + rr * D + 8 * (chunk ^ k_swizzle<D>(rr)));
-      if (wave_row + 32 * n + rr < rows)
-        *reinterpret_cast<u32x4*>(a.out + (int64_t)(((uint64_t)hi << 32) | lo) + 8 * chunk) = w;
+    for (int i = 0; i < 16; i += 4) {
+      u32x2 w;
+      w[0] = as_u32((f16x2){(f16)(o[d][i] * inv), (f16)(o[d][i + 1] * inv)});
+      w[1] = as_u32((f16x2){(f16)(o[d][i + 2] * inv), (f16)(o[d][i + 3] * inv)});
+      const int chunk = (4 * d + i / 4) ^ k_swizzle<D>(r);
+      *reinterpret_cast<u32x2*>(mine + r * D + 8 * chunk + 4 * h) = w;
     }
+#pragma unroll
+  for (int j = 0; j < 32 * D / 8 / kWave; ++j) {
+    const int x = j * kWave + lane, rr = x / (D / 8), chunk = x % (D / 8);
+    const uint32_t lo = from_lane((uint32_t)place, rr), hi = from_lane((uint32_t)(place >> 32), rr);
+    const u32x4 w = *reinterpret_cast<const u32x4*>(mine + rr * D + 8 * (chunk ^ k_swizzle<D>(rr)));
+    if (wave_row + rr < rows)
+      *reinterpret_cast<u32x4*>(a.out + (int64_t)(((uint64_t)hi << 32) | lo) + 8 * chunk) = w;
   }
 }
 
-template <int D, int KT, int RB, int W, int PER_SIMD>
+template <int D, int KT, int W, int PER_SIMD>
 int launch(PromptArgs a, hipStream_t st) {
-  constexpr int ROWS = W * RB * 32;
+  constexpr int ROWS = W * 32;
   const int64_t rows = (int64_t)a.tokens * a.group;
   // every sequence may end inside a tile
   const int64_t tiles = a.starts ? rows / ROWS + a.batch : (rows + ROWS - 1) / ROWS;
   if (tiles * a.heads_kv > 0x7fffffff) return LB_ERR_PROB_SHAPE;
   a.tiles = (int)tiles;
-  prompt_attention_kernel<D, KT, RB, W, PER_SIMD><<<dim3((unsigned)(tiles * a.heads_kv)), dim3(kWave * W), 0, st>>>(a);
+  prompt_attention_kernel<D, KT, W, PER_SIMD><<<dim3((unsigned)(tiles * a.heads_kv)), dim3(kWave * W), 0, st>>>(a);
   return lbh::launch_status();
 }
 
@@ -368,7 +367,10 @@ extern "C" int lb_prompt_attention(const uint16_t* q, int64_t q_token_stride, in
   a.starts = cu_seqlens, a.batch = (int)batch, a.tokens = (int)tokens, a.group = (int)(heads_q / heads_kv);
   a.heads_kv = (int)heads_kv, a.scale = softmax_scale * kLog2e;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (head_dim == 64) return launch<64, 64, 1, 4, 3>(a, st);
-  if (head_dim == 128) return launch<128, 64, 1, 4, 2>(a, st);
-  return launch<256, 64, 1, 4, 1>(a, st);
+  // Waves a SIMD as the registers allow (142 of them, 220, 512): two workgroups a
+  // compute unit, out of step by themselves, against one of eight waves at 128
+  // channels: 691 us, 742.  Tiles of 32 keys at 256 channels: 4043 us, of 64: 3570.
+  if (head_dim == 64) return launch<64, 64, 4, 3>(a, st);
+  if (head_dim == 128) return launch<128, 64, 4, 2>(a, st);
+  return launch<256, 64, 4, 1>(a, st);
 }

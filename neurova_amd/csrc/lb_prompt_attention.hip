@@ -19,8 +19,8 @@
 // where 32 rows took 742).
 //   8192 tokens, 40 / 8 heads of 128: 660 us, 1040 TFLOP/s of the 1154 that a large
 //   library product reaches (without exponentials 5 % less time, without reading
-//   the keys 23 %); 16384 tokens, 24 / 4 heads of 256: 3440 us, 960 TFLOP/s; 7
-//   packed prompts of 100 to 1500 tokens, same heads: 103 us, of which each
+//   the keys 23 %); 16384 tokens, 24 / 4 heads of 256: 3275 us, 1007 TFLOP/s; 7
+//   packed prompts of 100 to 1500 tokens, same heads: 98 us, of which each
 //   workgroup spends 7 on its first loads and its output.
 #include "attn_common.hpp"
 
@@ -139,6 +139,17 @@ __device__ __forceinline__ Place place_of(const PromptArgs& a, int i) {
   return {0, 0, 0};
 }
 
+// At 256 channels the output fills half of a wave's accumulation registers, which
+// only the matrix products reach.  Without these marks (around the scaling, and at
+// the end of the loop) the compiler copies all of it into vector registers in every
+// tile, for the rare tile that scales it: 16384 tokens 3275 us, without 3470.
+template <int D, int N>
+__device__ __forceinline__ void stay_in_accumulators(f32x16 (&o)[N]) {
+  if constexpr (D == 256)
+#pragma unroll
+    for (int d = 0; d < N; ++d) asm volatile("" : "+a"(o[d]));
+}
+
 template <int D, int KT, int W, int PER_SIMD>
 __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(PromptArgs a) {
   constexpr int ROWS = W * 32, DT = D / 32, KK = D / 16, ST = KT / 32;
@@ -249,6 +260,7 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
 #pragma unroll
       for (int i = 0; i < 16; ++i) peak = __builtin_fmaxf(peak, s[t][i]);
     peak *= a.scale;
+    stay_in_accumulators<D>(o);
     if (__any(peak > m + kSlack)) {
       const float up = __builtin_fmaxf(__builtin_fmaxf(peak, from_lane(peak, lane ^ 32)), m);
       const float f = __builtin_amdgcn_exp2f(m - up);
@@ -256,6 +268,7 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
       l *= f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= f;
+      stay_in_accumulators<D>(o);
     }
     f16x8 pf[2 * ST];
     const float lift = kLift - m;
@@ -288,6 +301,7 @@ __global__ __launch_bounds__(kWave * W, PER_SIMD) void prompt_attention_kernel(P
   for (int kt = 0; kt < tiles; kt += 2) {
     take(kt, k0, v0, k1, v1);
     if (kt + 1 < tiles) take(kt + 1, k1, v1, k0, v0);
+    stay_in_accumulators<D>(o);
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);  // no load may arrive in LDS after the workgroup
 

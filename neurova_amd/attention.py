@@ -122,25 +122,36 @@ class KV8Cache:
         _ops().kv8_append_out(q, k, v, *self._buffers(), page_table, seq_lens, cu_seqlens, rotation, q_out, k_out, interleaved)
         return (q_out, k_out) if return_k else q_out
 
-    def attend(self, q, page_table, seq_lens, *, scale: float | None = None, out=None):
+    def attend(self, q, page_table, seq_lens, *, scale: float | None = None, out=None, workspace=None):
         """Attention of the newest tokens of every sequence (``q`` holds the same number for each) over its pages.
 
         The queries of one call see the keys up to their own.  ``scale`` is
-        ``head_dim ** -0.5`` by default.
+        ``head_dim ** -0.5`` by default.  ``workspace`` int32, zeros, of tokens *
+        heads entries, is left zero and belongs to calls that run in order; without
+        it the cache keeps one for each stream, and a call captured into a graph
+        clears one of its own in every replay.
         """
         import torch
 
         _require_device(q, "KV8Cache.attend")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        need = q.shape[0] * q.shape[1]
-        key = (q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
-        ws = self._workspaces.get(key)
-        if ws is None or ws.numel() < need:  # calls on one stream run in order and share it
-            ws = self._workspaces[key] = torch.zeros((max(need, 4096),), dtype=torch.int32, device=q.device)
-        _ops().kv8_attention_out(q, *self._buffers(), page_table, seq_lens, out, ws,
+        _ops().kv8_attention_out(q, *self._buffers(), page_table, seq_lens, out, self._workspace(q) if workspace is None else workspace,
                                  q.shape[2] ** -0.5 if scale is None else scale)
         return out
+
+    def _workspace(self, q):
+        """A buffer of zeros for each stream, whose calls run in order; in a capture one from the graph's memory, which nothing else may keep."""
+        import torch
+
+        need = q.shape[0] * q.shape[1]
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros((need,), dtype=torch.int32, device=q.device)
+        key = (q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
+        ws = self._workspaces.get(key)
+        if ws is None or ws.numel() < need:
+            ws = self._workspaces[key] = torch.zeros((max(need, 4096),), dtype=torch.int32, device=q.device)
+        return ws
 
 
 def prompt_attention(q, k, v, cu_seqlens=None, *, scale: float | None = None, out=None):

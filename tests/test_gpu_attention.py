@@ -606,6 +606,39 @@ def test_prompt_attention_keeps_sequences_apart(dev):
 
 # --------------------------------------------------- graphs and the wrappers ---
 
+@pytest.mark.parametrize("own", [False, True])
+def test_cache_attend_captured_before_its_first_eager_call(dev, own):
+    """A workspace made in a capture is zeroed by replays alone: no eager call may take it."""
+    import torch
+
+    from neurova_amd.attention import KV8Cache
+
+    print_case("attend-captured-first", own)
+    c = Cached(dev, [2000, 77, 600], 1, 8, 2, 128, 32, seed=6)
+    cache = KV8Cache(*c.k_cache.shape[:2], 128, page_size=32, device=dev)
+    cache.k_cache, cache.v_cache, cache.k_scale, cache.v_scale = c.k_cache, c.v_cache, c.k_scale, c.v_scale
+    ws = torch.zeros(c.q.shape[0] * c.q.shape[1], dtype=torch.int32, device=dev) if own else None
+    out = torch.empty_like(c.q)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            cache.attend(c.q, c.table, c.seq_lens, out=out, workspace=ws)
+        assert not cache._workspaces
+        c.check(cache.attend(c.q, c.table, c.seq_lens))
+        eager = cache.attend(c.q, c.table, c.seq_lens)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        with torch.cuda.stream(side):
+            assert torch.equal(cache.attend(c.q, c.table, c.seq_lens), eager)
+        torch.cuda.synchronize()
+
+
 def test_operators_replay_from_graphs(dev):
     """Each operator captured, replayed with eager work between, equal to its eager result every time."""
     import langburst_cuda as lc

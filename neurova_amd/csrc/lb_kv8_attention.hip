@@ -500,7 +500,9 @@ struct Walk {
     }
     // the weights p * v_scale enter the second product relative to the largest
     // scale, as the sum of two fp16 numbers (one alone would add as much error
-    // as the rounding of the output; the matrix cores are mostly idle here)
+    // as the rounding of the output; the matrix cores are mostly idle here).  Both
+    // are cut off towards zero by an instruction that takes no part in a fused
+    // one: the first has to be the same number in the product and in the rest.
     const float vscale = held0 ? __builtin_amdgcn_ldexpf(vs, kLift - e) : 0.0f;
     f16x8 pf[NQ][2], pl[NQ][2];
 #pragma unroll
@@ -508,12 +510,18 @@ struct Walk {
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float p = __builtin_amdgcn_exp2f(s[n][2 * f + j / 4][j % 4] - m[n]);
-          l[n] += p;
-          const float w = p * vscale;
-          pf[n][f][j] = (f16)w;
-          pl[n][f][j] = (f16)(w - (float)(f16)w);
+        for (int j = 0; j < 8; j += 2) {
+          float w[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float p = __builtin_amdgcn_exp2f(s[n][2 * f + j / 4][j % 4 + i] - m[n]);
+            l[n] += p;
+            w[i] = p * vscale;
+          }
+          const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w[0], w[1]));
+          const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w[0] - (float)hi[0], w[1] - (float)hi[1]));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) pf[n][f][j + i] = hi[i], pl[n][f][j + i] = lo[i];
         }
     __builtin_amdgcn_sched_barrier(0);
     if (MORE) load_scales();

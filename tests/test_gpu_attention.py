@@ -403,6 +403,17 @@ def test_attention_over_the_cache_flat_and_sharp_scores(dev, sharp, scale):
     c.check(c.run(lc, scale=scale), scale=scale)
 
 
+@pytest.mark.parametrize("d,hkv", [(64, 4), (128, 2), (256, 1)])
+def test_attention_over_the_cache_rounds_its_weights_once(dev, d, hkv):
+    """Thousands of rows with few keys, so that a single weight rounded twice shows: outputs are within a rounding of exact."""
+    import langburst_cuda as lc
+
+    print_case("kv8-attention-weights", d, hkv)
+    for seed in range(12):
+        c = Cached(dev, [9 + 8 * i for i in range(8)], 1, 8 * hkv, hkv, d, 16, seed=100 + seed)
+        c.check(c.run(lc))
+
+
 @pytest.mark.parametrize("hq,hkv,d", [(8, 8, 64), (8, 2, 128), (6, 1, 256)])
 def test_attention_over_the_cache_with_cold_caches(dev, hq, hkv, d):
     """One step of tokens a workgroup, and nothing of them in the GPU's caches: the loads take their longest."""

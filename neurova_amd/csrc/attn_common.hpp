@@ -35,22 +35,4 @@ __device__ __forceinline__ float collect4(__amdgpu_buffer_rsrc_t r, uint32_t off
   return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kSc1));
 }
 
-// The packed sequence that holds work item `item`, where sequence b's items
-// start at starts[b] * per / span + slack * b (monotone in b for sorted starts):
-// the last b whose first item is <= item, -1 if there is none.  The whole wave
-// searches together, 64 sequences a load; `item` is wave-uniform.
-__device__ __forceinline__ int sequence_of_item(const int32_t* starts, int batch, int per, int span, int slack,
-                                                int item) {
-  const int lane = lane_id();
-  int count = 0;
-  for (int c = 0; c < batch; c += kWave) {
-    const int b = c + lane;
-    const bool le = b < batch && starts[b] * per / span + slack * b <= item;
-    const uint64_t m = __ballot(le);
-    count += __popcll(m);
-    if (m != ~0ull) break;
-  }
-  return __builtin_amdgcn_readfirstlane(count) - 1;
-}
-
 }  // namespace lb

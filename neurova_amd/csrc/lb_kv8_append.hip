@@ -350,6 +350,23 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t job)
   }
 }
 
+// The packed sequence that holds item `item` of the pages, where sequence b's
+// begin at item starts[b] / page_size + 2 b (rising for sorted starts): the last b
+// that begins at or before it, -1 if none does.  The whole wave searches together,
+// 64 sequences a load; `item` is wave-uniform.
+__device__ __forceinline__ int sequence_of_item(const AppendArgs& a, int item) {
+  const int lane = lane_id();
+  int count = 0;
+  for (int c = 0; c < a.batch; c += kWave) {
+    const int b = c + lane;
+    const bool le = b < a.batch && a.starts[b] / (1 << a.page_shift) + 2 * b <= item;
+    const uint64_t m = __ballot(le);
+    count += __popcll(m);
+    if (m != ~0ull) break;
+  }
+  return __builtin_amdgcn_readfirstlane(count) - 1;
+}
+
 __global__ __launch_bounds__(1024) void kv8_append_kernel(AppendArgs a) {
   __shared__ uint32_t lds[16];
   if ((int)blockIdx.x >= a.kv_blocks) {
@@ -365,7 +382,7 @@ __global__ __launch_bounds__(1024) void kv8_append_kernel(AppendArgs a) {
     b = item / a.page_bound, page = item % a.page_bound;
     first = b * a.per_seq, n = a.per_seq;
   } else {
-    b = sequence_of_item(a.starts, a.batch, 1, 1 << a.page_shift, 2, item);
+    b = sequence_of_item(a, item);
     if (b < 0) return;
     first = max(a.starts[b], 0), n = min(a.starts[b + 1], a.tokens) - first;
     page = item - (a.starts[b] / (1 << a.page_shift) + 2 * b);

@@ -64,6 +64,11 @@ constexpr int kNoExp = -1000;
 // 5 sequences of 700 to 6000 tokens, 3 new ones, 8 heads of 128: 18.0 us with 3
 // units in 200 slots, 19.3 with 2 in 280, where the last 24 share theirs.
 constexpr int kAlone = 1;
+// Above a quarter of the workers, pairs get slots if these are at most this many
+// units longer than equal ranges, and so mostly a workgroup each: 64 sequences of
+// 300 to 1000 tokens, 8 heads of 64: 15.7 us, with ranges 18.2; of 2000 to 4000
+// tokens, 4 heads of 256, where slots of 4 units more would serve: 86.7, 81.8.
+constexpr int kWhole = 1;
 // Up to 16 parts of a pair are joined by its last worker (4000 tokens, 8 heads of
 // 128: 11.2 us, 12.6 with a second launch); above that a second launch takes a
 // workgroup for each column (131072 tokens: 182 us with the last worker, 56).
@@ -117,12 +122,13 @@ struct Shared {
 };
 
 // How a launch's work is cut.  A pair (sequence, key/value head, column block)
-// has `nu` units.  With many pairs the workgroups take equal contiguous ranges
-// of all units, numbered pair by pair, so one may end a pair and begin the
-// next.  With few pairs, up to a quarter of the workers, each is cut into slots
-// of its own, `per` units or a little less, one a workgroup: the fixed time of a
-// segment (its first loads, the join) is then paid once (5 sequences of 700 to
-// 6000 tokens, 3 new ones: 18.6 us, with ranges 25.6).
+// has `nu` units.  In general the workgroups take equal contiguous ranges of all
+// units, numbered pair by pair, so one may end a pair and begin the next.  Where
+// the pairs are no more than the workers, each can be cut into slots of its own,
+// `per` units or a little less, one a workgroup: the fixed time of a segment (its
+// first loads, the join) is then paid once.  Up to a quarter of the workers, pairs
+// always are (5 sequences of 700 to 6000 tokens, 3 new ones, 8 heads of 128: 18.6
+// us, with ranges 25.6).
 struct Work {
   int units, per;
   bool slots;
@@ -163,13 +169,15 @@ __device__ __forceinline__ Work work_of(const AttnArgs& a, int first_len) {
   const int per_seq = a.heads_kv * a.col_blocks, pairs = a.batch * per_seq;
   Work w;
   w.units = total * per_seq;
-  w.slots = 4 * pairs <= a.workers;
   w.per = max((w.units + a.workers - 1) / a.workers, a.min_units);
-  if (w.slots) {
+  w.slots = false;
+  if (pairs <= a.workers) {
+    int per = 0;
     const int alone = max((w.units + a.cus - 1) / a.cus, a.min_units);
-    const int per = a.workers > a.cus ? slots_for(a, first_len, alone, w.per + kAlone, a.cus) : 0;
+    if (a.workers > a.cus) per = slots_for(a, first_len, alone, w.per + kAlone, a.cus);
     // at the latest units / (workers - pairs): there are at most units / per + pairs
-    w.per = per ? per : slots_for(a, first_len, w.per, w.units, a.workers);
+    if (!per) per = slots_for(a, first_len, w.per, 4 * pairs <= a.workers ? w.units : w.per + kWhole, a.workers);
+    if (per) w.slots = true, w.per = per;
   }
   return w;
 }

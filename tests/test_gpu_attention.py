@@ -379,6 +379,9 @@ CACHED = [
     ([1] * 70 + [300] + [5] * 70, 1, 2, 2, 64, 16),   # more sequences than a wave has lanes
     ([9000], 1, 6, 1, 128, 16),                  # one long sequence over many workgroups
     ([20000, 30, 5000], 2, 8, 2, 128, 64),       # ragged: parts of three sequences meet in a workgroup
+    ([300, 900, 5, 0, 620] * 12, 1, 8, 8, 64, 16),    # about as many pairs as workgroups: most hold a pair
+    ([300, 900, 5, 0, 620] * 14, 1, 8, 8, 64, 16),    # and somewhat more pairs than workgroups
+    ([9000] + [300] * 31, 1, 8, 4, 128, 32),     # one long sequence among short ones
 ]
 
 

@@ -20,8 +20,8 @@
 // are one number a lane and step.
 //
 //   128 sequences of 500 to 8192 tokens, 8 heads of 128: 123 us, 5.4 TB/s where
-//   reads alone reach 6.2; one of 131072 tokens, 4 heads of 256: 56 us (4.8 TB/s;
-//   51.5 and 4.7 for the join).  Few tokens are bound by the chain of loads that
+//   reads alone reach 6.2; one of 131072 tokens, 4 heads of 256: 55 us (4.9 TB/s;
+//   50.9 and 4.8 for the join).  Few tokens are bound by the chain of loads that
 //   wait for one another (length, page, keys) and a step's instructions, 800 a
 //   wave: 301 tokens, 4 heads of 256: 10.8 us, of which 2 are the two loads before
 //   the keys, 4 the first step, 1.7 the output.

@@ -11,16 +11,15 @@
 // tokens, and little work falls past the diagonal.  Four waves of 32 rows go
 // through the keys together, with the next tile on its way into LDS.
 //
-// Bound by the matrix cores and, as much, by LDS: a product of 32 cycles reads
-// 1 KB of keys or values, so four waves ask for all of the 128 bytes a cycle of a
-// compute unit.  64 rows a wave would halve that, but at 256 channels their
-// accumulators, queries and scores do not fit the registers, and at 128 they leave
-// one wave a SIMD, with nothing to run beside its softmax (8192 tokens: 920 us
-// where 32 rows took 742).
-//   8192 tokens, 40 / 8 heads of 128: 660 us, 1040 TFLOP/s of the 1154 that a large
-//   library product reaches (without exponentials 5 % less time, without reading
-//   the keys 23 %); 16384 tokens, 24 / 4 heads of 256: 3275 us, 1007 TFLOP/s; 7
-//   packed prompts of 100 to 1500 tokens, same heads: 98 us, of which each
+// Bound by the matrix cores at the clock that their load leaves (1.6 GHz of 2.4 at
+// 128 channels), with LDS close behind: a product of 32 cycles reads 1 KB of keys or
+// values, so four waves ask for all of the 128 bytes a cycle of a compute unit.  64
+// rows a wave would halve that, but at 256 channels their accumulators, queries and
+// scores do not fit the registers, and at 128 they leave one wave a SIMD, with
+// nothing to run beside its softmax (8192 tokens: 920 us where 32 rows took 742).
+//   8192 tokens, 40 / 8 heads of 128: 665 us, 1034 TFLOP/s of the 1154 that a large
+//   library product reaches; 16384 tokens, 24 / 4 heads of 256: 3275 us, 1007
+//   TFLOP/s; 7 packed prompts of 100 to 1500 tokens, same heads: 95 us, of which each
 //   workgroup spends 7 on its first loads and its output.
 #include "attn_common.hpp"
 

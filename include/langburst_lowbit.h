@@ -265,10 +265,11 @@ int lb_marlin_dequant(const int32_t* B, const uint16_t* s, uint16_t* w_nk,
  * need a larger one, and then its codes are rescaled.  A non-finite key or
  * value makes the scale non-finite, and so it stays while the page is filled.
  * q and q_out may be NULL together (no queries); q_out may be q.  k_out, when
- * given, receives the rotated keys and must not be k.  A token before position
- * 0 (seq_lens[b] below the sequence's new tokens) is padding: its q_out row is
- * zero and nothing is stored.  Two sequences of one call must not append to the
- * same page. */
+ * given, receives the rotated keys, also of tokens without a page or past
+ * max_pages * page_size, and must not be k.  A token before position 0
+ * (seq_lens[b] below the sequence's new tokens) is padding: its q_out and k_out
+ * rows are zero and nothing is stored.  Two sequences of one call must not append
+ * to the same page. */
 int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                   const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
                   const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride,

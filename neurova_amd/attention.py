@@ -110,8 +110,10 @@ class KV8Cache:
         ``cu_seqlens`` int32 ``[batch + 1]`` says which of the packed tokens are
         whose; without it every sequence has the same number.  ``rotation`` is a
         :func:`rotation_table` (None: no rotation), ``q_out`` where the rotated
-        queries go (it may be ``q`` itself).  A token's page and its scale are
-        described at ``lb_kv8_append`` in ``include/langburst_lowbit.h``.
+        queries go (it may be ``q`` itself).  With ``return_k`` every token of a
+        sequence has its rotated key, with or without a page; padding has zeros.
+        A token's page and its scale are described at ``lb_kv8_append`` in
+        ``include/langburst_lowbit.h``.
         """
         import torch
 

@@ -161,6 +161,7 @@ struct Cell {
   int page_lo, lo, hi;  // positions: of the page's first slot, and of the new tokens in it
   int start, first;     // of the sequence's new tokens: the first's position, and its row
   int head;
+  bool stored;          // the page is one of the cache; else its tokens' keys are only returned
   int64_t cell;         // page * heads + head
   float* scale_at;
   float old_scale;
@@ -190,6 +191,10 @@ __device__ __forceinline__ Scaling rescale(const Cell& c, uint32_t peak, uint32_
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
 
+// Rows of k_out are the page's workgroup's too, which holds the rotated keys:
+// also those of a page that is absent, or past the table, and the zeros of padding
+// (pages before position 0).
+//
 // Keys: a thread holds two neighbouring tokens at a pair of vectors that rotate
 // together, so each value and angle is loaded once; eight codes of a token are
 // one store of the layout [page][token][channel].
@@ -217,6 +222,7 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, const Cell& c, 
       const int pos = c.page_lo + off0 + i;
       if (!c.is_new(pos)) continue;
       if (a.k_out.p) {
+        if (c.page_lo < 0) x[i][0] = x[i][1] = (f32x8)(0.0f);
         uint16_t* out = a.k_out.p + (int64_t)(c.first + (pos - c.start)) * a.k_out.token + (int64_t)c.head * a.k_out.head;
         store8(out + 8 * pr.v0, x[i][0]);
         store8(out + 8 * pr.v1, x[i][1]);
@@ -230,6 +236,7 @@ __device__ __forceinline__ void append_keys(const AppendArgs& a, const Cell& c, 
         }
     }
   }
+  if (!c.stored) return;
   const Scaling s = rescale(c, peak, lds);
   if (!active) return;
 #pragma unroll
@@ -333,7 +340,7 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t job)
     b = lo, first = a.starts[b], n = a.starts[b + 1] - first;
     if (t < first || t >= first + n) return;  // outside every sequence
   }
-  const int pos = a.seq_lens[b] - n + (t - first);
+  const int pos = max(a.seq_lens[b], 0) - n + (t - first);
   const Pair pr = pair_of(a, j);
   f32x8 c, s;
   if (pr.r0) angles(a, pos, pr, c, s);
@@ -388,19 +395,21 @@ __global__ __launch_bounds__(1024) void kv8_append_kernel(AppendArgs a) {
     page = item - (a.starts[b] / (1 << a.page_shift) + 2 * b);
     if (n <= 0) return;
   }
-  const int len = a.seq_lens[b];
-  const int start = len - n;
-  page += max(start, 0) >> a.page_shift;
+  const int len = max(a.seq_lens[b], 0);
+  const int start = len - n;  // before position 0 where the first tokens are padding
+  page += start >> a.page_shift;
   Cell c;
-  c.page_lo = page << a.page_shift;
-  c.lo = max(max(start, 0), c.page_lo), c.hi = min(len, c.page_lo + (1 << a.page_shift));
-  if (c.lo >= c.hi || page >= a.max_pages) return;
-  const int id = a.page_table[(int64_t)b * a.table_stride + page];
-  if ((unsigned)id >= (unsigned)a.num_pages) return;
+  c.page_lo = page * (1 << a.page_shift);
+  c.lo = max(start, c.page_lo), c.hi = min(len, c.page_lo + (1 << a.page_shift));
+  if (c.lo >= c.hi) return;
+  int id = -1;
+  if ((unsigned)page < (unsigned)a.max_pages) id = a.page_table[(int64_t)b * a.table_stride + page];
+  c.stored = (unsigned)id < (unsigned)a.num_pages;
+  if (!c.stored && (kind == 1 || a.k_out.p == nullptr)) return;
   c.start = start, c.first = first, c.head = head;
   c.cell = (int64_t)id * a.heads_kv + head;
   c.scale_at = (kind == 0 ? a.k_scale : a.v_scale) + c.cell;
-  c.kept = c.page_lo < start;
+  c.kept = c.stored && c.page_lo < start;
   c.old_scale = c.kept ? *c.scale_at : 0.0f;
   if (kind == 0) append_keys(a, c, lds);
   else append_values(a, c, lds);

@@ -1,0 +1,117 @@
+"""The attention operators where a call is only partly ordinary: absent pages, padding, non-finite and very unequal scales, wide columns.
+
+Oracles and tolerances are those of ``test_gpu_attention.py``; where one is
+added here, its derivation stands with it.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import attention_oracle as A
+from tests.gpu_util import print_case
+from tests.test_gpu_attention import AppendCase, Cached, _np
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ append ---
+
+def _rows_near(got, want):
+    size = np.abs(want).max() + 1
+    return (np.abs(got - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -22 * size + 2.0 ** -25).all()
+
+
+KEYS_OUT = [
+    # lens (new tokens included), new, heads_q, heads_kv, d, page, rot, interleaved, pages left out as (sequence, page), table pages
+    ([40, 70], [40, 70], 4, 2, 64, 16, 64, False, [(0, 0), (1, 0), (1, 1), (1, 3)], 9),     # only a window keeps its pages
+    ([90, 33], [90, 33], 3, 1, 128, 32, 128, True, [(0, 1)], 2),                            # the table ends before the tokens
+    ([0, 2, 24, 34, -3], [4, 4, 4, 4, 4], 2, 1, 64, 16, 64, False, [(2, 1), (3, 2)], 4),    # padding: none, some and all of a sequence
+    ([7, 19, 130], [20, 40, 130], 2, 2, 256, 64, 64, True, [(2, 0)], 2),
+    ([50, 3], [150, 3], 5, 1, 128, 16, 0, False, [(0, 0), (0, 3)], 3),                      # more padding than a page holds
+]
+
+
+@pytest.mark.parametrize("case", range(len(KEYS_OUT)))
+@pytest.mark.parametrize("strided,queries", [(False, True), (True, False)])
+def test_append_returns_the_keys_of_every_token(dev, case, strided, queries):
+    """A token without a page, or past the table, has its rotated key all the same; padding has zeros; a token of no sequence is left out."""
+    import langburst_cuda as lc
+    import torch
+
+    lens, news, hq, hkv, d, p, rot, inter, absent, width = KEYS_OUT[case]
+    print_case("append-keys-out", case, strided, queries)
+
+    made = []
+    for _ in range(2):
+        torch.manual_seed(case)  # the order of the pages
+        made.append(AppendCase(dev, [max(x - n, 0) for x, n in zip(lens, news)], news, hq, hkv, d, p, rot, seed=case, strided=strided,
+                               positions=max(lens)))
+    c, plain = made
+    for x in (c, plain):
+        x.seq_lens = torch.tensor(lens, dtype=torch.int32, device=dev)
+        for b, page in absent:
+            if page < x.table.shape[1]:
+                x.table[b, page] = -1 if b else 10 ** 6
+        x.table = x.table[:, :width].contiguous()
+        if strided and len(set(news)) == 1:
+            x.starts = None
+    tokens = sum(news)
+    k_out = torch.full((tokens, hkv, d), float("nan"), dtype=torch.float16, device=dev)
+    q_out = torch.full((tokens, hq, d), float("nan"), dtype=torch.float16, device=dev) if queries else None
+    lc.kv8_append_out(c.q if queries else None, c.k, c.v, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.table, c.seq_lens,
+                      c.starts, c.rotation, q_out, k_out, inter)
+    torch.cuda.synchronize()
+    angles, at = None if c.rotation is None else _np(c.rotation), 0
+    for b, n in enumerate(news):
+        for i in range(n):
+            pos = lens[b] - n + i
+            for got, x in ((k_out, c.k),) + (((q_out, c.q),) if queries else ()):
+                if pos < 0:
+                    assert (got[at + i] == 0).all(), (b, i)
+                    continue
+                want = _np(x[at + i]) if angles is None else A.rotate(_np(x[at + i]), angles[pos, :rot // 2], angles[pos, rot // 2:], inter)
+                assert _rows_near(_np(got[at + i]), want), (b, i, pos)
+        at += n
+    # the cache is what it is without the keys' rows
+    lc.kv8_append_out(None, plain.k, plain.v, plain.k_cache, plain.v_cache, plain.k_scale, plain.v_scale, plain.table, plain.seq_lens,
+                      plain.starts, plain.rotation, None, None, inter)
+    for x, y in ((c.k_cache, plain.k_cache), (c.v_cache, plain.v_cache), (c.k_scale, plain.k_scale), (c.v_scale, plain.v_scale)):
+        assert torch.equal(x, y)
+
+
+def test_append_leaves_the_keys_rows_of_no_sequence(dev):
+    import langburst_cuda as lc
+    import torch
+
+    print_case("append-keys-out-rest")
+    c = AppendCase(dev, [0, 0, 0], [5, 40, 7], 2, 1, 64, 16, 64, seed=1)
+    k_out = torch.full((52, 1, 64), 7.0, dtype=torch.float16, device=dev)
+    # the last seven tokens are of no sequence
+    lc.kv8_append_out(None, c.k, c.v, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.table[:2].contiguous(), c.seq_lens[:2].contiguous(),
+                      c.starts[:3].contiguous(), c.rotation, None, k_out, False)
+    torch.cuda.synchronize()
+    assert (k_out[45:] == 7).all() and (k_out[:45] != 7).any(-1).all()
+
+
+def test_cache_append_returns_keys_that_prompt_attention_can_read(dev):
+    """Through the cache object: early pages left out, and the prompt's attention still sees every key."""
+    import torch
+
+    from neurova_amd.attention import KV8Cache, prompt_attention, rotation_table
+
+    print_case("append-window-then-prompt")
+    hq, hkv, d, n = 4, 2, 128, 100
+    g = torch.Generator(device=dev)
+    g.manual_seed(3)
+    qkv = torch.randn((n, hq + 2 * hkv, d), device=dev, generator=g).half()
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+    table = rotation_table(n, 64, device=dev)
+    lens = torch.tensor([n], dtype=torch.int32, device=dev)
+    whole, window = KV8Cache(8, hkv, d, page_size=16, device=dev), KV8Cache(8, hkv, d, page_size=16, device=dev)
+    junk = torch.full((n, hkv, d), float("nan"), dtype=torch.float16, device=dev)
+    del junk  # what an allocation may hold
+    got = window.append(q, k, v, torch.tensor([[-1, -1, -1, -1, -1, 4, 2]], dtype=torch.int32, device=dev), lens, rotation=table, return_k=True)
+    want = whole.append(q, k, v, torch.tensor([[5, 1, 0, 7, 3, 4, 2]], dtype=torch.int32, device=dev), lens, rotation=table, return_k=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(prompt_attention(*got, v), prompt_attention(*want, v))

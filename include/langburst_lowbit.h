@@ -252,7 +252,8 @@ int lb_marlin_dequant(const int32_t* B, const uint16_t* s, uint16_t* w_nk,
  * at most max_pages * page_size are read.
  * cu_seqlens int32 [batch + 1]: the packed tokens cu_seqlens[b] to
  * cu_seqlens[b + 1] - 1 are sequence b's (its newest, in order); NULL: every
- * sequence has tokens / batch.  Tokens that belong to no sequence are skipped. */
+ * sequence has tokens / batch.  Tokens that belong to no sequence are skipped;
+ * of a sequence that ends past the given tokens these are its first. */
 
 /* Rotates queries and keys and stores keys and values, in one launch.
  * cos_sin fp32 [positions, rot_dim]: cos of the rot_dim / 2 angles of a

@@ -318,6 +318,9 @@ __device__ __forceinline__ void append_values(const AppendArgs& a, const Cell& c
   }
 }
 
+// The first of sequence b's packed tokens.
+__device__ __forceinline__ int first_of(const AppendArgs& a, int b) { return max(a.starts[b], 0); }
+
 // Rows of padding (a token before position 0) come out as zeros.
 __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t job) {
   const int pairs = a.d8 / 2;
@@ -337,7 +340,7 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int64_t job)
       const int mid = (lo + hi) / 2;
       if (a.starts[mid] <= t) lo = mid; else hi = mid;
     }
-    b = lo, first = a.starts[b], n = a.starts[b + 1] - first;
+    b = lo, first = first_of(a, b), n = a.starts[b + 1] - first;
     if (t < first || t >= first + n) return;  // outside every sequence
   }
   const int pos = max(a.seq_lens[b], 0) - n + (t - first);
@@ -366,7 +369,7 @@ __device__ __forceinline__ int sequence_of_item(const AppendArgs& a, int item) {
   int count = 0;
   for (int c = 0; c < a.batch; c += kWave) {
     const int b = c + lane;
-    const bool le = b < a.batch && a.starts[b] / (1 << a.page_shift) + 2 * b <= item;
+    const bool le = b < a.batch && first_of(a, b) / (1 << a.page_shift) + 2 * b <= item;
     const uint64_t m = __ballot(le);
     count += __popcll(m);
     if (m != ~0ull) break;
@@ -391,8 +394,9 @@ __global__ __launch_bounds__(1024) void kv8_append_kernel(AppendArgs a) {
   } else {
     b = sequence_of_item(a, item);
     if (b < 0) return;
-    first = max(a.starts[b], 0), n = min(a.starts[b + 1], a.tokens) - first;
-    page = item - (a.starts[b] / (1 << a.page_shift) + 2 * b);
+    // the last of the n may not be given: those that are keep their places
+    first = first_of(a, b), n = a.starts[b + 1] - first;
+    page = item - (first / (1 << a.page_shift) + 2 * b);
     if (n <= 0) return;
   }
   const int len = max(a.seq_lens[b], 0);
@@ -400,7 +404,7 @@ __global__ __launch_bounds__(1024) void kv8_append_kernel(AppendArgs a) {
   page += start >> a.page_shift;
   Cell c;
   c.page_lo = page * (1 << a.page_shift);
-  c.lo = max(start, c.page_lo), c.hi = min(len, c.page_lo + (1 << a.page_shift));
+  c.lo = max(start, c.page_lo), c.hi = min(min(len, start + (a.tokens - first)), c.page_lo + (1 << a.page_shift));
   if (c.lo >= c.hi) return;
   int id = -1;
   if ((unsigned)page < (unsigned)a.max_pages) id = a.page_table[(int64_t)b * a.table_stride + page];

@@ -115,3 +115,28 @@ def test_cache_append_returns_keys_that_prompt_attention_can_read(dev):
     want = whole.append(q, k, v, torch.tensor([[5, 1, 0, 7, 3, 4, 2]], dtype=torch.int32, device=dev), lens, rotation=table, return_k=True)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert torch.equal(prompt_attention(*got, v), prompt_attention(*want, v))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_of_a_sequence_whose_last_tokens_are_not_given(dev, interleaved):
+    """cu_seqlens[b + 1] - 1 is a sequence's newest token: one past the given tokens moves none of these, keys or queries."""
+    import langburst_cuda as lc
+    import torch
+
+    print_case("append-cut-short", interleaved)
+    made = []
+    for _ in range(2):
+        torch.manual_seed(5)
+        made.append(AppendCase(dev, [0, 30], [20, 30], 3, 2, 64, 16, 64, seed=6))
+    long, short = made
+    tokens = 40  # of 50: ten of the second sequence are missing
+    outs = []
+    for c, lens, starts in ((long, [20, 60], [0, 20, 50]), (short, [20, 50], [0, 20, 40])):
+        q, k = (torch.full((tokens, h, 64), float("nan"), dtype=torch.float16, device=dev) for h in (3, 2))
+        lc.kv8_append_out(c.q[:tokens], c.k[:tokens], c.v[:tokens], c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.table,
+                          torch.tensor(lens, dtype=torch.int32, device=dev), torch.tensor(starts, dtype=torch.int32, device=dev),
+                          c.rotation, q, k, interleaved)
+        outs.append((q, k, c.k_cache, c.v_cache, c.k_scale, c.v_scale))
+    torch.cuda.synchronize()
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)

@@ -290,7 +290,8 @@ int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stri
  * tokens / batch newest tokens of every sequence are the queries; token i of n
  * sees the keys 0 to seq_lens[b] - n + i, and a row that sees none is zero.
  * Scores, softmax and sums are fp32; a weight times its value scale is rounded
- * to fp16 for the second product, relative to the largest scale met.
+ * to fp16 for the second product, relative to the largest scale met.  A page's
+ * scale that is not finite reaches the rows that see a token of the page.
  * workspace: int32, zero on entry, left zero, at least
  * batch * heads_kv * ceil(tokens / batch * heads_q / heads_kv / 16) entries
  * (tokens * heads_q always suffice).  scratch: lb_kv8_attention_scratch_bytes()

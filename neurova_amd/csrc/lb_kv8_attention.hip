@@ -511,10 +511,13 @@ struct Walk {
     // as the rounding of the output; the matrix cores are mostly idle here).  Both
     // are cut off towards zero by an instruction that takes no part in a fused
     // one: the first has to be the same number in the product and in the rest.
-    const float vscale = held0 ? __builtin_amdgcn_ldexpf(vs, kLift - e) : 0.0f;
+    // A column that sees none of a lane's tokens takes zero for their scale: its
+    // weights are zero, and zero times a scale that is not finite is not.
+    const float lifted = __builtin_amdgcn_ldexpf(vs, kLift - e);
     f16x8 pf[NQ][2], pl[NQ][2];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    for (int n = 0; n < NQ; ++n) {
+      const float vscale = held0 && tv < limit[n] ? lifted : 0.0f;
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
@@ -531,6 +534,7 @@ struct Walk {
 #pragma unroll
           for (int i = 0; i < 2; ++i) pf[n][f][j + i] = hi[i], pl[n][f][j + i] = lo[i];
         }
+    }
     __builtin_amdgcn_sched_barrier(0);
     if (MORE) load_scales();
 #pragma unroll

@@ -140,3 +140,28 @@ def test_append_of_a_sequence_whose_last_tokens_are_not_given(dev, interleaved):
     torch.cuda.synchronize()
     for x, y in zip(*outs):
         assert torch.equal(x, y)
+
+
+# --------------------------------------------------------- attention, cache ---
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("hq,hkv,d,n", [(4, 2, 64, 3), (12, 2, 64, 4), (6, 2, 128, 3), (10, 1, 128, 4), (6, 1, 256, 3), (24, 2, 256, 3)])
+def test_attention_over_the_cache_keeps_non_finite_scales_behind_the_causal_limit(dev, bad, hq, hkv, d, n):
+    """A new token's page that is not finite reaches the rows that see a token of it, and no earlier row."""
+    import langburst_cuda as lc
+
+    print_case("kv8-attention-masked-scale", bad, hq, hkv, d, n)
+    for which in ("v_scale", "k_scale"):
+        for length in (16 + n - 1, 304 + n - 1, 2001):  # row 0 is its page's last token; 2001 is one past a page
+            c = Cached(dev, [length], n, hq, hkv, d, 16, seed=length)
+            last = (length - 1) // 16
+            clean = c.run(lc)
+            c.check(clean)
+            clean = _np(clean)
+            getattr(c, which)[int(c.table[0, last])] = bad
+            got = _np(c.run(lc))
+            for i in range(n):
+                if length - n + i < last * 16:  # within the outputs' rounding of the clean call's: fp16 at either side
+                    assert (np.abs(got[i] - clean[i]) <= 2.0 ** -10 * np.abs(clean[i]) + 2.0 ** -17 * np.abs(clean[i]).max() + 2.0 ** -24).all(), (which, length, i)
+                elif which == "v_scale":
+                    assert np.isnan(got[i]).all(), (which, length, i)

@@ -467,7 +467,9 @@ struct Walk {
       flip ^= 1;
     }
     const int tv = tb + 16 * g;
-    const float kscale = held0 ? ks * a.scale : 0.0f;
+    // a scale of infinity has no scores (those below zero would have no weight and
+    // its keys go unseen): ks - ks makes it NaN and is zero otherwise
+    const float kscale = held0 ? ks * a.scale + (ks - ks) : 0.0f;
     // the exponent of the value scale; a page of zeros, or none, has the lowest
     const int ve = held0 && vs > 0.0f ? __builtin_amdgcn_frexp_expf(vs) : kNoExp;
     const bool mask = tb + kStep > sg.len - a.new_tokens + 1 || __any(!held0);

@@ -165,3 +165,18 @@ def test_attention_over_the_cache_keeps_non_finite_scales_behind_the_causal_limi
                     assert (np.abs(got[i] - clean[i]) <= 2.0 ** -10 * np.abs(clean[i]) + 2.0 ** -17 * np.abs(clean[i]).max() + 2.0 ** -24).all(), (which, length, i)
                 elif which == "v_scale":
                     assert np.isnan(got[i]).all(), (which, length, i)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (4, 4, 128), (6, 1, 256)])
+def test_attention_over_the_cache_shows_an_infinite_key_scale(dev, hq, hkv, d):
+    """Keys that are not finite have no scores, below zero or above: every row that sees them is NaN."""
+    import langburst_cuda as lc
+
+    print_case("kv8-attention-key-scale", hq, hkv, d)
+    for length, page in ((40, 1), (700, 3), (700, 43), (33, 2), (1025, 64)):  # the last two with a single token in the page
+        c = Cached(dev, [length], 1, hq, hkv, d, 16, seed=length + page)
+        c.k_scale[int(c.table[0, page]), 0] = float("inf")
+        got = c.run(lc)
+        assert np.isnan(_np(got[:, :hq // hkv])).all()
+        if hkv > 1:
+            c.check(got, heads=range(1, hkv))

@@ -289,9 +289,10 @@ int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stri
  * of sequences and key/value heads (which depends on the sizes alone).  The
  * tokens / batch newest tokens of every sequence are the queries; token i of n
  * sees the keys 0 to seq_lens[b] - n + i, and a row that sees none is zero.
- * Scores, softmax and sums are fp32; a weight times its value scale is rounded
- * to fp16 for the second product, relative to the largest scale met.  A page's
- * scale that is not finite reaches the rows that see a token of the page.
+ * Scores, softmax and sums are fp32; a weight times its value scale enters the
+ * second product as the sum of two fp16 numbers, cut off by at most 2^-21 of
+ * itself plus 2^-31 of the row's largest (value scales from 2^-80 to 2^80).  A
+ * page's scale that is not finite reaches the rows that see a token of the page.
  * workspace: int32, zero on entry, left zero, at least
  * batch * heads_kv * ceil(tokens / batch * heads_q / heads_kv / 16) entries
  * (tokens * heads_q always suffice).  scratch: lb_kv8_attention_scratch_bytes()

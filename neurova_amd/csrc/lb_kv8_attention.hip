@@ -54,12 +54,15 @@ constexpr int kStep = 64;           // tokens a wave takes at a time
 constexpr int kStreams = 4;            // streams of tokens in a workgroup
 constexpr int kUnit = kStep * kStreams;  // tokens of a unit of work
 constexpr float kNoMax = -1e30f;
-// The running maximum moves only when a score exceeds it by 2^kSlack, and the
-// weights carry 2^kLift more: at most 2^15, inside fp16, and 2^7 farther from its
-// subnormals.
-constexpr float kSlack = 8.0f;
-constexpr int kLift = 7;
-constexpr int kNoExp = -1000;
+// The running maximum is that of weight times value scale (a score plus the
+// scale's logarithm), which is what the second product takes: a page that a row
+// ignores costs the others none of their bits, however large its values.  It moves
+// only when exceeded by 2^kSlack, and the weights carry 2^kLift more: at most
+// 2^15, inside fp16, and 2^7 farther from its subnormals.  Scales count from
+// 2^-kScales to 2^kScales (a page of zeros as the lowest), so that the sums of the
+// weights alone stay inside fp32: at most 2^(kSlack + kScales) for each of 2^28
+// tokens.
+constexpr float kSlack = 8.0f, kLift = 7.0f, kScales = 80.0f;
 // Slots may be this many units longer if each then has a compute unit to itself:
 // 5 sequences of 700 to 6000 tokens, 3 new ones, 8 heads of 128: 18.0 us with 3
 // units in 200 slots, 19.3 with 2 in 280, where the last 24 share theirs.
@@ -402,7 +405,7 @@ struct Walk {
   // not; with MORE another one follows, in sg or in `to`.
   template <bool MORE, bool LAST>
   __device__ __forceinline__ void step(const Segment& sg, int tb, f32x4 (&o)[NQ][VT], float (&m)[NQ], float (&l)[NQ],
-                                       int& e, bool ahead, const Segment& to) {
+                                       bool ahead, const Segment& to) {
     const bool held0 = held;
     // the keys are in LDS once no more loads are out than those of the values,
     // which follow theirs (nothing else waits for a load into LDS here)
@@ -470,11 +473,10 @@ struct Walk {
     // a scale of infinity has no scores (those below zero would have no weight and
     // its keys go unseen): ks - ks makes it NaN and is zero otherwise
     const float kscale = held0 ? ks * a.scale + (ks - ks) : 0.0f;
-    // the exponent of the value scale; a page of zeros, or none, has the lowest
-    const int ve = held0 && vs > 0.0f ? __builtin_amdgcn_frexp_expf(vs) : kNoExp;
+    const float vlog = __builtin_fmaxf(__builtin_fminf(__builtin_amdgcn_logf(__builtin_fabsf(vs)), kScales), -kScales);
     const bool mask = tb + kStep > sg.len - a.new_tokens + 1 || __any(!held0);
     float peak[NQ];
-    bool up = ve > e;
+    bool up = false;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       peak[n] = kNoMax;
@@ -487,14 +489,10 @@ struct Walk {
           s[n][t][i] = x;
           peak[n] = __builtin_fmaxf(peak[n], x);
         }
+      peak[n] += vlog;
       up |= peak[n] > m[n] + kSlack;
     }
     if (__any(up)) {
-      int top = max(ve, e);
-      top = max(top, (int)from_lane((uint32_t)top, lane ^ 16));
-      top = max(top, (int)from_lane((uint32_t)top, lane ^ 32));
-      const int down = max(e - top, -300);
-      e = top;
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         float x = __builtin_fmaxf(peak[n], m[n]);
@@ -503,19 +501,18 @@ struct Walk {
         const float f = __builtin_amdgcn_exp2f(m[n] - x);
         m[n] = x;
         l[n] *= f;
-        const float fo = __builtin_amdgcn_ldexpf(f, down);
 #pragma unroll
-        for (int d = 0; d < VT; ++d) o[n][d] *= fo;
+        for (int d = 0; d < VT; ++d) o[n][d] *= f;
       }
     }
     // the weights p * v_scale enter the second product relative to the largest
-    // scale, as the sum of two fp16 numbers (one alone would add as much error
+    // of them, as the sum of two fp16 numbers (one alone would add as much error
     // as the rounding of the output; the matrix cores are mostly idle here).  Both
     // are cut off towards zero by an instruction that takes no part in a fused
     // one: the first has to be the same number in the product and in the rest.
     // A column that sees none of a lane's tokens takes zero for their scale: its
     // weights are zero, and zero times a scale that is not finite is not.
-    const float lifted = __builtin_amdgcn_ldexpf(vs, kLift - e);
+    const float lifted = vs * __builtin_exp2f(kLift);
     f16x8 pf[NQ][2], pl[NQ][2];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -560,7 +557,6 @@ struct Walk {
   __device__ __forceinline__ void run(const Segment& sg, bool ahead, const Segment& to, int worker) {
     f32x4 o[NQ][VT];
     float m[NQ], l[NQ];
-    int e = kNoExp;  // o is relative to 2^(e - kLift), the largest value scale met
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       m[n] = kNoMax, l[n] = 0.0f;
@@ -570,10 +566,10 @@ struct Walk {
     start(sg, ahead, to);
     const int end = end_token(sg);
     int tb = first_token(sg);
-    for (; tb + kUnit < end; tb += kUnit) step<true, false>(sg, tb, o, m, l, e, ahead, to);
+    for (; tb + kUnit < end; tb += kUnit) step<true, false>(sg, tb, o, m, l, ahead, to);
     if (tb < end) {
-      if (ahead && first_token(to) < end_token(to)) step<true, true>(sg, tb, o, m, l, e, ahead, to);
-      else step<false, true>(sg, tb, o, m, l, e, ahead, to);
+      if (ahead && first_token(to) < end_token(to)) step<true, true>(sg, tb, o, m, l, ahead, to);
+      else step<false, true>(sg, tb, o, m, l, ahead, to);
     }
     // a round of steps in which this stream has none: its barrier all the same
     if (H == 2 && end > sg.u0 * kUnit && steps_from(first_token(sg), end) < steps_from(sg.u0 * kUnit, end)) lds_barrier();
@@ -593,7 +589,7 @@ struct Walk {
       float up = kNoMax;
 #pragma unroll
       for (int w = 0; w < kStreams; ++w) up = __builtin_fmaxf(up, sh.m[w][c]);
-      const float f = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(m[n] - up), max(e, -300) - kLift);
+      const float f = __builtin_amdgcn_exp2f(m[n] - up - kLift);
 #pragma unroll
       for (int d = 0; d < VT; ++d)
         *reinterpret_cast<f32x4*>(&sh.o[stream][c][half * DW + 16 * d + 4 * g]) = o[n][d] * f;

@@ -180,3 +180,37 @@ def test_attention_over_the_cache_shows_an_infinite_key_scale(dev, hq, hkv, d):
         assert np.isnan(_np(got[:, :hq // hkv])).all()
         if hkv > 1:
             c.check(got, heads=range(1, hkv))
+
+
+@pytest.mark.parametrize("ratio", [1e-6, 1e-7, 1e-9])
+@pytest.mark.parametrize("hq,hkv,d,n", [(4, 4, 64, 1), (10, 1, 64, 2), (4, 1, 128, 1), (12, 1, 128, 2), (6, 1, 256, 1)])
+def test_attention_over_the_cache_to_a_page_of_small_values_among_large_ones(dev, ratio, hq, hkv, d, n):
+    """Pages that a row ignores do not cost the others' weights their bits, however large their values.
+
+    The page attended to is 28 above the rest in its scores, so all others have
+    2^-40 of the weight, and the output is its values' average.  The largest value
+    scale is 200: values of the small page stay normal fp16 numbers down to 1e-7.
+    """
+    import langburst_cuda as lc
+
+    print_case("kv8-attention-small-page", ratio, hq, hkv, d, n)
+    length, page = 700, 16
+    for target in (0, 19, 43 - n):  # the first page, one in the middle, the last whole one
+        c = Cached(dev, [length], n, hq, hkv, d, page, seed=target)
+        pages = c.table[0, :-(-length // page)].long()
+        small = int(pages[target])
+        c.k_scale[pages] = 0.02
+        c.v_scale[pages], c.v_scale[small] = 200.0, 200.0 * ratio
+        c.k_cache[pages, :, :, 0], c.k_cache[small, :, :, 0] = -127, 127
+        c.q.mul_(0.05)[:, :, 0] = 14 / 2.54
+        out = c.run(lc, scale=1.0)
+        for h in range(hkv):
+            k, v, _ = c.keys(0, h)
+            for j in range(hq // hkv):
+                q = _np(c.q[:, h * (hq // hkv) + j])
+                sees = [length - n + i + 1 for i in range(n)]
+                want, spread, _ = A.attend(q, k, v, 1.0, sees)
+                w = 2 * A.score_error(q, k, 1.0) + 2.0 ** -18
+                err = np.abs(_np(out[:, h * (hq // hkv) + j]) - want)
+                bad = err > 2.0 ** -11 * np.abs(want) + w * spread + 2.0 ** -25
+                assert not bad.any(), (target, h, j, err.max(), np.abs(want).max())

@@ -300,6 +300,13 @@ int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stri
  * softmax_scale positive and finite. */
 size_t lb_kv8_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv,
                                       int64_t head_dim, int64_t page_size, int64_t max_pages);
+/* The plan of lb_kv8_attention for these sizes (for tests and tools, no device
+ * work).  Fills out[7]: [0] columns a workgroup takes together; [1] blocks of
+ * them; [2] workgroups; [3] tokens of the smallest slot; [4] kernel launches;
+ * [5] workspace entries; [6] scratch bytes.  Returns LB_OK, or the status that
+ * lb_kv8_attention would return for the sizes. */
+int lb_kv8_attention_describe_plan(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv,
+                                   int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t* out);
 int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                      const int8_t* k_cache, const int8_t* v_cache, const float* k_scale, const float* v_scale,
                      int64_t num_pages, int64_t page_size,

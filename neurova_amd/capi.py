@@ -55,6 +55,7 @@ _SIGNATURES = {
     "lb_kv8_append": ([P, I64, I64] * 5 + [P, P, P, P, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, P, I64, I64, I32, P],
                       ctypes.c_int),
     "lb_kv8_attention_scratch_bytes": ([I64] * 7, SZ),
+    "lb_kv8_attention_describe_plan": ([I64] * 7 + [P], ctypes.c_int),
     "lb_kv8_attention": ([P, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P, I64, I64, I64, I64, I64, P, I64, I64, F32, P,
                           I64, P, SZ, P], ctypes.c_int),
     "lb_prompt_attention": ([P, I64, I64] * 3 + [P, I64, I64, I64, I64, I64, P, I64, I64, F32, P], ctypes.c_int),
@@ -233,6 +234,19 @@ def kv8_append(q, k, v, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens
 
 def kv8_attention_scratch_bytes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages) -> int:
     return int(lib().lb_kv8_attention_scratch_bytes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages))
+
+
+KV8_PLAN_FIELDS = ("columns", "column_blocks", "workgroups", "slot_tokens", "launches", "workspace_entries", "scratch_bytes")
+
+
+def kv8_attention_describe_plan(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages) -> dict:
+    """The plan lb_kv8_attention makes for these sizes; no device work.  Raises on refused ones."""
+    out = (ctypes.c_int64 * 7)()
+    st = lib().lb_kv8_attention_describe_plan(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages,
+                                              ctypes.cast(out, ctypes.c_void_p))
+    if st != LB_OK:
+        raise ValueError(f"lb_kv8_attention_describe_plan: {status_string(st)}")
+    return dict(zip(KV8_PLAN_FIELDS, (int(v) for v in out)))
 
 
 def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, out, workspace, scratch,

@@ -816,6 +816,19 @@ extern "C" size_t lb_kv8_attention_scratch_bytes(int64_t batch, int64_t tokens, 
   return lb::plan_of(batch, tokens / batch, heads_q, heads_kv, head_dim, page_size * max_pages).scratch;
 }
 
+extern "C" int lb_kv8_attention_describe_plan(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv,
+                                              int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t* out) {
+  if (!out) return LB_ERR_ARG;
+  const int err = lb::check_sizes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages);
+  if (err != LB_OK) return err;
+  for (int i = 0; i < 7; ++i) out[i] = 0;
+  if (batch == 0 || tokens == 0) return LB_OK;
+  const lb::Plan p = lb::plan_of(batch, tokens / batch, heads_q, heads_kv, head_dim, page_size * max_pages);
+  out[0] = 16 * p.nq, out[1] = p.col_blocks, out[2] = p.workers, out[3] = p.min_units * lb::kUnit;
+  out[4] = 1 + p.joined, out[5] = p.counters, out[6] = (int64_t)p.scratch;
+  return LB_OK;
+}
+
 extern "C" int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                                 const int8_t* k_cache, const int8_t* v_cache, const float* k_scale,
                                 const float* v_scale, int64_t num_pages, int64_t page_size, const int32_t* page_table,

@@ -214,3 +214,38 @@ def test_attention_over_the_cache_to_a_page_of_small_values_among_large_ones(dev
                 err = np.abs(_np(out[:, h * (hq // hkv) + j]) - want)
                 bad = err > 2.0 ** -11 * np.abs(want) + w * spread + 2.0 ** -25
                 assert not bad.any(), (target, h, j, err.max(), np.abs(want).max())
+
+
+WIDE = [
+    # lens, n, heads_q, heads_kv, d, page: columns in one block of 16, one of 32, and more blocks, joined by
+    # the last worker and by a second launch
+    ([5000], 1, 4, 1, 64, 16),                   # 64 channels, 4 columns, second launch
+    ([2000, 900, 70], 4, 12, 2, 64, 64),         # 24 columns, ranges of several units
+    ([9000, 400], 3, 16, 2, 64, 32),             # 24 columns, second launch
+    ([2000, 900], 6, 12, 2, 64, 64),             # 36 columns: two blocks
+    ([9000, 33], 6, 16, 2, 64, 128),             # 48 columns: two blocks, second launch
+    ([3000, 700, 2000], 5, 8, 2, 128, 16),       # 20 columns
+    ([9000], 5, 4, 1, 128, 32),                  # 20 columns, second launch
+    ([3000, 700, 5], 9, 8, 2, 128, 16),          # 36 columns: two blocks
+    ([9000], 10, 4, 1, 128, 64),                 # 40 columns: two blocks, second launch
+    ([6000], 1, 6, 1, 256, 64),                  # second launch
+    ([3000, 100], 4, 12, 2, 256, 32),            # 24 columns: two blocks of 16
+    ([6000], 4, 12, 1, 256, 64),                 # 48 columns: three blocks, second launch
+    ([260, 100], 70, 4, 2, 64, 16),              # 140 columns: five blocks, a sequence with little more than the new tokens
+    ([600] * 40, 3, 12, 2, 128, 16),             # 18 columns, about a slot for each worker
+    ([1500] * 90, 3, 12, 2, 128, 16),            # and ranges that end inside pairs
+    ([300] + [5] * 70 + [2600], 3, 7, 1, 128, 32),  # more sequences than a wave has lanes
+]
+
+
+@pytest.mark.parametrize("case", range(len(WIDE)))
+def test_attention_over_the_cache_in_every_form(dev, case):
+    import langburst_cuda as lc
+    import torch
+
+    print_case("kv8-attention-wide", case, *WIDE[case][1:])
+    c = Cached(dev, *WIDE[case], seed=case)
+    out = c.run(lc)
+    c.check(out, heads=None if len(WIDE[case][0]) < 40 else [0])
+    for _ in range(3):
+        assert torch.equal(out, c.run(lc)), "repeated calls differ"

@@ -72,10 +72,14 @@ constexpr int kAlone = 1;
 // 300 to 1000 tokens, 8 heads of 64: 15.7 us, with ranges 18.2; of 2000 to 4000
 // tokens, 4 heads of 256, where slots of 4 units more would serve: 86.7, 81.8.
 constexpr int kWhole = 1;
-// Up to 16 parts of a pair are joined by its last worker (4000 tokens, 8 heads of
-// 128: 11.2 us, 12.6 with a second launch); above that a second launch takes a
-// workgroup for each column (131072 tokens: 182 us with the last worker, 56).
-constexpr int kFewParts = 16;
+// A pair's parts are joined by its last worker, or by a second launch with a
+// workgroup for each column where pairs that fill their tables have 16 slots or
+// more (one sequence, 8 heads of 128: 2500 tokens 10.8 us, with a second launch
+// 11.4; 4000 tokens, 16 slots, 12.4 and 10.7; 131072 tokens 182 and 56).  The
+// sizes decide, since lengths are on the device: a short sequence in such a table
+// pays for the second launch too (301 tokens 8.5 us in a table of 3840, 10.9 in
+// one of 4096 or more), which is why it does not begin earlier.
+constexpr int kManySlots = 16;
 constexpr int kParts = 8;        // parts whose loads a thread of the last worker has in flight: 32768
                                  // tokens beside 15 x 300: 30.6 us, 4 at a time 35.8, 16 the same
 constexpr int kJoinGroups = 16;  // groups of D / 4 threads that join a column's parts in the second launch
@@ -775,7 +779,7 @@ Plan plan_of(int64_t batch, int64_t new_tokens, int64_t heads_q, int64_t heads_k
   // among short ones it may have more; the last worker then joins those too)
   const int64_t per = (p.counters * units + p.workers - 1) / p.workers;
   p.min_units = p.nq;
-  p.joined = units / (per > p.min_units ? per : p.min_units) + 1 > kFewParts;
+  p.joined = units / (per > p.min_units ? per : p.min_units) >= kManySlots;
   p.scratch = ((size_t)p.workers * 2 * 16 * p.nq * (head_dim + 2) * 4 + 255) & ~(size_t)255;
   return p;
 }

@@ -183,7 +183,7 @@ __device__ __forceinline__ Work work_of(const AttnArgs& a, int first_len) {
     const int alone = max((w.units + a.cus - 1) / a.cus, a.min_units);
     if (a.workers > a.cus) per = slots_for(a, first_len, alone, w.per + kAlone, a.cus);
     // at the latest units / (workers - pairs): there are at most units / per + pairs
-    if (!per) per = slots_for(a, first_len, w.per, 4 * pairs <= a.workers ? w.units : w.per + kWhole, a.workers);
+    if (!per) per = slots_for(a, first_len, w.per, 4 * pairs <= a.workers ? max(w.units, w.per) : w.per + kWhole, a.workers);
     if (per) w.slots = true, w.per = per;
   }
   return w;
@@ -694,7 +694,9 @@ __global__ __launch_bounds__(kThreads<D>, (kPerCu<D, NQ>)) void kv8_attention_ke
 
 // Joins the parts of the pairs that several workers share, one column of one
 // pair a workgroup: D / 4 threads a part, the parts dealt to the thread groups
-// in turn and their sums added in group order.
+// in turn and their sums added in group order.  With this launch the pairs are at
+// most a sixteenth of the workers (kManySlots), 32 on 256 compute units: their
+// sequences' lengths fit a wave, and they are cut into slots.
 template <int D, int NQ>
 __global__ __launch_bounds__(kJoinGroups * D / 4) void kv8_join_kernel(AttnArgs a) {
   constexpr int COLS = 16 * NQ, T = D / 4, GROUPS = kJoinGroups;
@@ -704,24 +706,11 @@ __global__ __launch_bounds__(kJoinGroups * D / 4) void kv8_join_kernel(AttnArgs 
   const int c = blockIdx.x % COLS, pair = blockIdx.x / COLS;
   const int b = pair / pairs, x = pair % pairs, cb = x % a.col_blocks, head = x / a.col_blocks;
   if (cb * COLS + c >= a.new_tokens * a.group) return;
-  const int first_lens = len_at(a, lane_id());
-  const Work work = work_of(a, first_lens);
-  int base = 0, len = 0;
-  for (int i = 0; i <= b; i += kWave) {
-    const int lens = i ? len_at(a, i + lane_id()) : first_lens;
-    const int nu = units_or_none(lens);
-    const int size = work.slots ? (nu + work.per - 1) / work.per : nu;
-    const int upto = wave_scan(size);
-    const bool here = b < i + kWave;
-    base += __builtin_amdgcn_readlane(here ? upto - size : upto, here ? b - i : kWave - 1);
-    if (here) len = __builtin_amdgcn_readlane(lens, b - i);
-  }
-  const int nu = units_of(len);
-  const int slots = work.slots ? (nu + work.per - 1) / work.per : nu;
-  const int first = base * pairs + x * slots;
-  const int w_first = work.slots ? first : first / work.per;
-  const int w_last = work.slots ? first + slots - 1 : (first + nu - 1) / work.per;
-  if (w_first == w_last) return;  // one worker held the whole pair and stored its rows
+  const int lens = len_at(a, lane_id()), per = work_of(a, lens).per;
+  const int size = (units_or_none(lens) + per - 1) / per, upto = wave_scan(size);
+  const int slots = __builtin_amdgcn_readlane(size, b);
+  const int w_first = __builtin_amdgcn_readlane(upto - size, b) * pairs + x * slots, w_last = w_first + slots - 1;
+  if (slots == 1) return;  // one worker held the whole pair and stored its rows
   const int grp = threadIdx.x / T, d = 4 * (threadIdx.x % T);
   float m = kNoMax, l = 0.0f;
   f32x4 o = (f32x4)(0.0f);

@@ -448,7 +448,8 @@ extern "C" int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t 
   if (!k || !v || !k_cache || !v_cache || !k_scale || !v_scale || !page_table || !seq_lens || (queries && !q) ||
       (rot_dim > 0 && !cos_sin))
     return LB_ERR_ARG;
-  if (k_out == k) return LB_ERR_ARG;  // a thread reads both halves of a pair and writes one
+  // a slot that is not new reads a neighbour's row (and drops it), which that one's thread would be writing
+  if (k_out == k) return LB_ERR_ARG;
   const void* ptrs[] = {k, v, queries ? q : nullptr, q_out, k_out, k_cache, v_cache, cos_sin};
   for (const void* p : ptrs)
     if (!lbh::aligned(p, 16)) return LB_ERR_ALIGN;

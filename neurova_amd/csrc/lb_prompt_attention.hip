@@ -45,9 +45,10 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __fp16 fp16x4 __attribute__((__vector_size__(8)));
 
 // A weight is rounded to fp16 for the second product, its sum taken before that in
-// fp32: an error of at most 2^-12 sum p |v|, as large as the output's own rounding
-// where the values have one sign.  A second fp16 number for the rest, as over the
-// cache, would double that product where the matrix cores are the bound.
+// fp32: an error of at most 2^-11 sum p |v|, as large as the output's own rounding
+// where the values have one sign, and 2^-32 of the largest weight for one below
+// fp16's normal numbers.  A second fp16 number for the rest, as over the cache,
+// would double that product where the matrix cores are the bound.
 
 // Sixteen-byte chunks of a key (value) row change places so that the 16-byte
 // reads of 16 rows at one column, and the transposing reads of 8 rows at one

@@ -47,8 +47,12 @@ typedef __fp16 fp16x4 __attribute__((__vector_size__(8)));
 // A weight is rounded to fp16 for the second product, its sum taken before that in
 // fp32: an error of at most 2^-11 sum p |v|, as large as the output's own rounding
 // where the values have one sign, and 2^-32 of the largest weight for one below
-// fp16's normal numbers.  A second fp16 number for the rest, as over the cache,
-// would double that product where the matrix cores are the bound.
+// fp16's normal numbers.  With normally distributed values the outputs are 2.7e-4
+// (97 tokens: 2.2e-4) from exact, root mean square, where rounding them alone leaves
+// 2.1e-4.  A second fp16 number for the rest, as over the cache, doubles that
+// product: 8192 tokens, 128 channels, 664 -> 911 us, and no size has it for nothing
+// (97 tokens 7.15 -> 7.75, 16 tokens 5.60 -> 5.87; 7 packed prompts of 256 channels
+// 95 -> 115).
 
 // Sixteen-byte chunks of a key (value) row change places so that the 16-byte
 // reads of 16 rows at one column, and the transposing reads of 8 rows at one

@@ -249,7 +249,7 @@ int lb_marlin_dequant(const int32_t* B, const uint16_t* s, uint16_t* w_nk,
  * number outside [0, num_pages) has no page: nothing is stored there and its
  * tokens are not attended; numbers past a sequence's length are not read.
  * seq_lens int32 [batch]: tokens of each sequence, the new ones included;
- * at most max_pages * page_size are read.
+ * at most max_pages * page_size are read, and new tokens past those see them all.
  * cu_seqlens int32 [batch + 1]: the packed tokens cu_seqlens[b] to
  * cu_seqlens[b + 1] - 1 are sequence b's (its newest, in order); NULL: every
  * sequence has tokens / batch.  Tokens that belong to no sequence are skipped;

@@ -144,6 +144,10 @@ struct Work {
 __device__ __forceinline__ int len_at(const AttnArgs& a, int b) {
   return b < a.batch ? max(min(a.seq_lens[b], a.max_tokens), 0) : -1;
 }
+// Tokens of a sequence past its table: they say which keys the new ones see.
+__device__ __forceinline__ int past_at(const AttnArgs& a, int b) {
+  return b < a.batch ? max(a.seq_lens[b], a.max_tokens) - a.max_tokens : 0;
+}
 // Units of a sequence's pairs; 0 past the batch (length -1).
 __device__ __forceinline__ int units_or_none(int len) { return len < 0 ? 0 : units_of(len); }
 
@@ -194,6 +198,7 @@ struct Segment {
   int b, head, cb, u0, u1, nu, len;
   int w_first, w_last;  // the workers of the whole pair
   int pair;
+  int past;  // tokens past the table; in a vector register, the scalar ones are all taken
 };
 
 // Four channels of an output row, divided by the sum of the weights (a row that
@@ -226,12 +231,12 @@ struct Segments {
   int worker, pairs;  // pairs of a sequence
   int u, u_end;       // position: in units, or with slots in slots
   int chunk, at, base;  // sequence chunk + at, which begins at position base
-  int lens;             // lengths of the 64 sequences from chunk on
+  int lens, past;       // lengths of the 64 sequences from chunk on, and what the table leaves out of them
 
   __device__ __forceinline__ bool begin(const AttnArgs& a) {
     const int lane = lane_id();
     pairs = a.heads_kv * a.col_blocks;
-    lens = len_at(a, lane);
+    lens = len_at(a, lane), past = past_at(a, lane);
     work = work_of(a, lens);
     worker = blockIdx.x;
     u = work.slots ? worker : worker * work.per;
@@ -245,7 +250,7 @@ struct Segments {
       if (base + all > u) break;
       base += all, chunk += kWave;
       if (chunk >= a.batch) return false;
-      lens = len_at(a, chunk + lane);
+      lens = len_at(a, chunk + lane), past = past_at(a, chunk + lane);
     }
     at = __builtin_ctzll(__ballot(base + upto > u));  // the sequence that holds u
     base += __builtin_amdgcn_readlane(upto - size, at);
@@ -261,6 +266,7 @@ struct Segments {
     sg.b = chunk + at, sg.nu = nu, sg.len = len;
     sg.head = x / a.col_blocks, sg.cb = x - sg.head * a.col_blocks;
     sg.pair = sg.b * pairs + x;
+    sg.past = (int)from_lane((uint32_t)past, at);
     if (work.slots) {
       const int i = u - first;
       sg.u0 = nu * i / slots, sg.u1 = nu * (i + 1) / slots;  // nu <= 2^20, slots <= workers
@@ -272,7 +278,7 @@ struct Segments {
       u = first + sg.u1;
       if (u < u_end && x == pairs - 1 && sg.u1 == nu) {  // on to the next sequence
         base += nu * pairs;
-        if (++at == kWave) at = 0, chunk += kWave, lens = len_at(a, chunk + lane_id());
+        if (++at == kWave) at = 0, chunk += kWave, lens = len_at(a, chunk + lane_id()), past = past_at(a, chunk + lane_id());
       }
     }
     return true;
@@ -370,7 +376,7 @@ struct Walk {
     for (int n = 0; n < NQ; ++n) {
       const int col = sg.cb * COLS + 16 * n + r;
       const int i = col / a.group;
-      limit[n] = col < cols ? sg.len - a.new_tokens + i + 1 : 0;
+      limit[n] = col < cols ? sg.len - a.new_tokens + i + 1 + sg.past : 0;
       const uint16_t* row = a.q + ((int64_t)sg.b * a.new_tokens + i) * a.q_token +
                             (int64_t)(sg.head * a.group + (col - i * a.group)) * a.q_head + half * DW + 16 * g;
 #pragma unroll

@@ -216,6 +216,30 @@ def test_attention_over_the_cache_to_a_page_of_small_values_among_large_ones(dev
                 assert not bad.any(), (target, h, j, err.max(), np.abs(want).max())
 
 
+@pytest.mark.parametrize("hq,hkv,d,n", [(4, 2, 64, 3), (12, 1, 128, 3), (6, 1, 256, 5)])
+def test_attention_over_the_cache_of_lengths_past_the_table(dev, hq, hkv, d, n):
+    """Token i of n sees the keys up to seq_lens - n + i, of which those in the table exist."""
+    import langburst_cuda as lc
+    import torch
+
+    print_case("kv8-attention-past-table", hq, hkv, d, n)
+    for pages in (6, 40):
+        for past in (0, 1, n - 1, n, 1000):
+            c = Cached(dev, [pages * 16, 50], n, hq, hkv, d, 16, seed=pages + past)
+            c.table = c.table[:, :pages].contiguous()
+            c.seq_lens = torch.tensor([pages * 16 + past, 50], dtype=torch.int32, device=dev)
+            out = c.run(lc)
+            for h in range(hkv):
+                k, v, _ = c.keys(0, h)
+                for j in range(hq // hkv):
+                    at = h * (hq // hkv) + j
+                    q = _np(c.q[:n, at])
+                    want, spread, _ = A.attend(q, k, v, d ** -0.5, [pages * 16 + past - n + i + 1 for i in range(n)])
+                    err = np.abs(_np(out[:n, at]) - want)
+                    bad = err > 2.0 ** -11 * np.abs(want) + (2 * A.score_error(q, k, d ** -0.5) + 2.0 ** -18) * spread + 2.0 ** -25
+                    assert not bad.any(), (pages, past, at, err.max())
+
+
 WIDE = [
     # lens, n, heads_q, heads_kv, d, page: columns in one block of 16, one of 32, and more blocks, joined by
     # the last worker and by a second launch

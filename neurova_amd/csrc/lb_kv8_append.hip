@@ -445,9 +445,10 @@ extern "C" int lb_kv8_append(const uint16_t* q, int64_t q_token_stride, int64_t 
   if (tokens == 0 || batch == 0) return LB_OK;
   if (cu_seqlens == nullptr && tokens % batch != 0) return LB_ERR_ARG;
   const bool queries = q_out != nullptr && heads_q > 0;
-  if (!k || !v || !k_cache || !v_cache || !k_scale || !v_scale || !page_table || !seq_lens || (queries && !q) ||
-      (rot_dim > 0 && !cos_sin))
-    return LB_ERR_ARG;
+  if (!k || !v || !seq_lens || (queries && !q) || (rot_dim > 0 && !cos_sin)) return LB_ERR_ARG;
+  // a cache or a table of nothing has no address: no token has a page then
+  if (max_pages > 0 && !page_table) return LB_ERR_ARG;
+  if (max_pages > 0 && num_pages > 0 && (!k_cache || !v_cache || !k_scale || !v_scale)) return LB_ERR_ARG;
   // a slot that is not new reads a neighbour's row (and drops it), which that one's thread would be writing
   if (k_out == k) return LB_ERR_ARG;
   const void* ptrs[] = {k, v, queries ? q : nullptr, q_out, k_out, k_cache, v_cache, cos_sin};

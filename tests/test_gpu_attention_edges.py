@@ -142,6 +142,25 @@ def test_append_of_a_sequence_whose_last_tokens_are_not_given(dev, interleaved):
         assert torch.equal(x, y)
 
 
+def test_append_without_a_single_page(dev):
+    """A table of no pages, or a cache of none: nothing is stored, and the rotated rows are there."""
+    import langburst_cuda as lc
+    import torch
+
+    print_case("append-no-pages")
+    for no_pages in (False, True):
+        c = AppendCase(dev, [0, 0], [5, 40], 2, 1, 64, 16, 64, seed=1)
+        want_q, want_k = (torch.empty((45, h, 64), dtype=torch.float16, device=dev) for h in (2, 1))
+        lc.kv8_append_out(c.q, c.k, c.v, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.table, c.seq_lens, c.starts, c.rotation,
+                          want_q, want_k, False)
+        q, k = torch.zeros_like(want_q), torch.zeros_like(want_k)
+        cache = [torch.empty((0,) + t.shape[1:], dtype=t.dtype, device=dev) for t in (c.k_cache, c.v_cache, c.k_scale, c.v_scale)] if no_pages else [c.k_cache, c.v_cache, c.k_scale, c.v_scale]
+        table = c.table if no_pages else torch.empty((2, 0), dtype=torch.int32, device=dev)
+        lc.kv8_append_out(c.q, c.k, c.v, *cache, table, c.seq_lens, c.starts, c.rotation, q, k, False)
+        torch.cuda.synchronize()
+        assert torch.equal(q, want_q) and torch.equal(k, want_k)
+
+
 # --------------------------------------------------------- attention, cache ---
 
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])

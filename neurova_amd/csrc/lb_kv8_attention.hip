@@ -19,11 +19,11 @@
 // a lane's tokens share a page (pages hold 16 tokens or more), so both scales
 // are one number a lane and step.
 //
-//   128 sequences of 500 to 8192 tokens, 8 heads of 128: 123 us, 5.4 TB/s where
-//   reads alone reach 6.2; one of 131072 tokens, 4 heads of 256: 55 us (4.9 TB/s;
-//   50.9 and 4.8 for the join).  Few tokens are bound by the chain of loads that
+//   128 sequences of 500 to 8192 tokens, 8 heads of 128: 122 us, 5.5 TB/s where
+//   reads alone reach 6.2; one of 131072 tokens, 4 heads of 256: 53 us (5.0 TB/s;
+//   49.0 and 4.7 for the join).  Few tokens are bound by the chain of loads that
 //   wait for one another (length, page, keys) and a step's instructions, 800 a
-//   wave: 301 tokens, 4 heads of 256: 10.8 us, of which 2 are the two loads before
+//   wave: 301 tokens, 4 heads of 256: 10.6 us, of which 2 are the two loads before
 //   the keys, 4 the first step, 1.7 the output.
 #include <type_traits>
 
@@ -75,10 +75,11 @@ constexpr int kWhole = 1;
 // A pair's parts are joined by its last worker, or by a second launch with a
 // workgroup for each column where pairs that fill their tables have 16 slots or
 // more (one sequence, 8 heads of 128: 2500 tokens 10.8 us, with a second launch
-// 11.4; 4000 tokens, 16 slots, 12.4 and 10.7; 131072 tokens 182 and 56).  The
+// 11.4; 4000 tokens, 16 slots, 12.4 and 10.7; 131072 tokens 182 and 53).  The
 // sizes decide, since lengths are on the device: a short sequence in such a table
-// pays for the second launch too (301 tokens 8.5 us in a table of 3840, 10.9 in
-// one of 4096 or more), which is why it does not begin earlier.
+// pays for the second launch too (301 tokens 8.5 us in a table of 3840, 10.0 in
+// one of 4096 or more, 10.9 where each call is launched by itself), which is why it
+// does not begin earlier.
 constexpr int kManySlots = 16;
 constexpr int kParts = 8;        // parts whose loads a thread of the last worker has in flight: 32768
                                  // tokens beside 15 x 300: 30.6 us, 4 at a time 35.8, 16 the same

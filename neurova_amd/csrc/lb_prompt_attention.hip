@@ -17,9 +17,10 @@
 // rows a wave would halve that, but at 256 channels their accumulators, queries and
 // scores do not fit the registers, and at 128 they leave one wave a SIMD, with
 // nothing to run beside its softmax (8192 tokens: 920 us where 32 rows took 742).
-//   8192 tokens, 40 / 8 heads of 128: 665 us, 1034 TFLOP/s of the 1154 that a large
-//   library product reaches; 16384 tokens, 24 / 4 heads of 256: 3275 us, 1007
-//   TFLOP/s; 7 packed prompts of 100 to 1500 tokens, same heads: 95 us, of which each
+//   8192 tokens, 40 / 8 heads of 128: 652 to 665 us, 1034 to 1054 TFLOP/s of the 1154
+//   that a large library product reaches; 16384 tokens, 24 / 4 heads of 256: 3220 to
+//   3310 us, 1000 to 1025 TFLOP/s; 8192 tokens, 32 / 8 heads of 64: 311 us, 884; 7
+//   packed prompts of 100 to 1500 tokens, 24 / 4 heads of 256: 95 us, of which each
 //   workgroup spends 7 on its first loads and its output.
 #include "attn_common.hpp"
 

@@ -259,6 +259,29 @@ def test_attention_over_the_cache_of_lengths_past_the_table(dev, hq, hkv, d, n):
                     assert not bad.any(), (pages, past, at, err.max())
 
 
+def test_attention_over_the_cache_of_lengths_past_the_table_among_many(dev):
+    """The lengths are read 64 sequences at a time: one past the table in every part of them."""
+    import langburst_cuda as lc
+    import torch
+
+    print_case("kv8-attention-past-table-many")
+    n, pages, past = 3, 20, 2
+    lens = [pages * 16 if b % 37 == 5 else 5 + b % 7 for b in range(150)]
+    c = Cached(dev, lens, n, 4, 1, 64, 16, seed=9)
+    c.table = c.table[:, :pages].contiguous()
+    c.seq_lens = torch.tensor([x + past * (x == pages * 16) for x in lens], dtype=torch.int32, device=dev)
+    out = _np(c.run(lc))
+    for b, length in enumerate(lens):
+        k, v, _ = c.keys(b, 0)
+        for h in range(4):
+            rows = slice(b * n, (b + 1) * n)
+            sees = [length + past * (length == pages * 16) - n + i + 1 for i in range(n)]
+            q = _np(c.q[rows, h])
+            want, spread, _ = A.attend(q, k, v, 0.125, sees)
+            bad = np.abs(out[rows, h] - want) > 2.0 ** -11 * np.abs(want) + (2 * A.score_error(q, k, 0.125) + 2.0 ** -18) * spread + 2.0 ** -25
+            assert not bad.any(), (b, h)
+
+
 WIDE = [
     # lens, n, heads_q, heads_kv, d, page: columns in one block of 16, one of 32, and more blocks, joined by
     # the last worker and by a second launch

@@ -170,8 +170,7 @@ def prepare(case, seed):
         s.update(q=torch.randn((tokens, case["hq"], case["d"]), device=DEV, generator=g).half(), scale=case["d"] ** -0.5,
                  seq_lens=_i32([a + b for a, b in seqs]), starts=_i32([0] + torch.tensor([a for a, _ in seqs]).cumsum(0).tolist()),
                  table=_table(g, counts, sum(counts), max(counts))[0], **_caches(g, case, sum(counts)),
-                 out=torch.empty((tokens, case["hq"], case["d"]), dtype=torch.float16, device=DEV),
-                 workspace=torch.zeros((tokens * case["hq"],), dtype=torch.int32, device=DEV))
+                 out=torch.empty((tokens, case["hq"], case["d"]), dtype=torch.float16, device=DEV))
     elif kind == "grow":
         lens = _lens(case, case["rows"])
         rows, cut = torch.randperm(case["rows"], device=DEV, generator=g).to(torch.int32), case["cut"]
@@ -344,7 +343,7 @@ def run(s):
         if not own:
             return _plain_chunk(s)
         ops.kv8_chunk_attention_out(s["q"], s["k_cache"], s["v_cache"], s["k_scale"], s["v_scale"], s["table"], s["seq_lens"],
-                                    s["starts"], s["out"], s["workspace"], s["scale"])
+                                    s["starts"], s["out"], s["scale"])
         return s["out"]
     if kind == "grow":
         if own:

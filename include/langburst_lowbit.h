@@ -317,6 +317,32 @@ int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_s
                      int32_t* workspace, int64_t workspace_len, void* scratch, size_t scratch_bytes,
                      lb_stream_t stream);
 
+/* The same for any number of new tokens of each sequence, packed one after the
+ * other: a sequence's rows are cu_seqlens[b] to cu_seqlens[b + 1], its newest
+ * tokens (cu_seqlens int32 [batch + 1], on the device, as seq_lens).  Pieces of
+ * prompts, whole ones, and sequences that decode a token or a few go into one
+ * call.  Row i of n sees the keys 0 to seq_lens[b] - n + i that the table holds;
+ * one that sees none (padding before position 0) is zero, and rows of tokens that
+ * belong to no sequence are left as they are.  Scores, softmax and sums are fp32;
+ * a weight times its value scale enters the second product as one fp16 number
+ * (2^-11, and 2^-32 of the row's largest; value scales from 2^-80 to 2^80).  A
+ * page's scale that is not finite reaches the rows that see a token of the page.
+ * One launch, or a second one that joins the parts of rows whose keys were cut,
+ * which tables of more than a few hundred tokens take.  scratch:
+ * lb_kv8_chunk_attention_scratch_bytes() bytes, 16-byte aligned, no
+ * initialisation; calls that share it must not overlap.  softmax_scale positive
+ * and finite. */
+size_t lb_kv8_chunk_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv,
+                                            int64_t head_dim, int64_t page_size, int64_t max_pages);
+int lb_kv8_chunk_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                           const int8_t* k_cache, const int8_t* v_cache, const float* k_scale, const float* v_scale,
+                           int64_t num_pages, int64_t page_size,
+                           const int32_t* page_table, int64_t max_pages, int64_t table_stride,
+                           const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t batch, int64_t tokens,
+                           int64_t heads_q, int64_t heads_kv, int64_t head_dim,
+                           uint16_t* out, int64_t o_token_stride, int64_t o_head_stride, float softmax_scale,
+                           void* scratch, size_t scratch_bytes, lb_stream_t stream);
+
 /* Causal attention of whole prompts: token i of a sequence sees the keys 0 to
  * i of the same sequence.  cu_seqlens NULL: one sequence (batch 1) of all
  * tokens.  Scores, softmax and sums are fp32, weights fp16 for the second

@@ -124,22 +124,31 @@ class KV8Cache:
         _ops().kv8_append_out(q, k, v, *self._buffers(), page_table, seq_lens, cu_seqlens, rotation, q_out, k_out, interleaved)
         return (q_out, k_out) if return_k else q_out
 
-    def attend(self, q, page_table, seq_lens, *, scale: float | None = None, out=None, workspace=None):
-        """Attention of the newest tokens of every sequence (``q`` holds the same number for each) over its pages.
+    def attend(self, q, page_table, seq_lens, cu_seqlens=None, *, scale: float | None = None, out=None, workspace=None):
+        """Attention of the newest tokens of every sequence over its pages; a query sees the keys up to its own.
 
-        The queries of one call see the keys up to their own.  ``scale`` is
-        ``head_dim ** -0.5`` by default.  ``workspace`` int32, zeros, of tokens *
-        heads entries, is left zero and belongs to calls that run in order; without
-        it the cache keeps one for each stream, and a call captured into a graph
-        clears one of its own in every replay.
+        With ``cu_seqlens`` int32 ``[batch + 1]`` it says which of the packed
+        queries are whose: pieces of prompts, whole ones and single tokens in one
+        call.  Without it ``q`` holds the same number for every sequence, a token or
+        a few.  ``scale`` is ``head_dim ** -0.5`` by default.  ``workspace`` (only
+        without ``cu_seqlens``) int32, zeros, of tokens * heads entries, is left zero
+        and belongs to calls that run in order; without it the cache keeps one for
+        each stream, and a call captured into a graph clears one of its own in every
+        replay.
         """
         import torch
 
         _require_device(q, "KV8Cache.attend")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _ops().kv8_attention_out(q, *self._buffers(), page_table, seq_lens, out, self._workspace(q) if workspace is None else workspace,
-                                 q.shape[2] ** -0.5 if scale is None else scale)
+        scale = q.shape[2] ** -0.5 if scale is None else scale
+        if cu_seqlens is not None:
+            if workspace is not None:
+                raise ValueError("attention of packed chunks takes no workspace")
+            _ops().kv8_chunk_attention_out(q, *self._buffers(), page_table, seq_lens, cu_seqlens, out, scale)
+        else:
+            _ops().kv8_attention_out(q, *self._buffers(), page_table, seq_lens, out,
+                                     self._workspace(q) if workspace is None else workspace, scale)
         return out
 
     def _workspace(self, q):

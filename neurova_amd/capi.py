@@ -58,6 +58,9 @@ _SIGNATURES = {
     "lb_kv8_attention_describe_plan": ([I64] * 7 + [P], ctypes.c_int),
     "lb_kv8_attention": ([P, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P, I64, I64, I64, I64, I64, P, I64, I64, F32, P,
                           I64, P, SZ, P], ctypes.c_int),
+    "lb_kv8_chunk_attention_scratch_bytes": ([I64] * 7, SZ),
+    "lb_kv8_chunk_attention": ([P, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, P, I64, I64, F32,
+                                P, SZ, P], ctypes.c_int),
     "lb_prompt_attention": ([P, I64, I64] * 3 + [P, I64, I64, I64, I64, I64, P, I64, I64, F32, P], ctypes.c_int),
     "lb_marlin_mlp_fused": ([P, P, P, P, P, P, I64, I64, I64, I64, I64, P, I64, P, SZ, P], ctypes.c_int),
 }
@@ -258,6 +261,20 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, o
                                   _ptr(seq_lens), seq_lens.shape[0], q.shape[0], q.shape[1], heads_kv, head_dim,
                                   *_rows(out), softmax_scale, _ptr(workspace), workspace.numel(), _ptr(scratch), nbytes,
                                   _stream(q))
+
+
+def kv8_chunk_attention_scratch_bytes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages) -> int:
+    return int(lib().lb_kv8_chunk_attention_scratch_bytes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages))
+
+
+def kv8_chunk_attention(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cu_seqlens, out, scratch,
+                        softmax_scale) -> int:
+    pages, heads_kv, page_size, head_dim = k_cache.shape
+    nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    return lib().lb_kv8_chunk_attention(*_rows(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), pages,
+                                        page_size, _ptr(page_table), page_table.shape[1], page_table.stride(0),
+                                        _ptr(seq_lens), _ptr(cu_seqlens), seq_lens.shape[0], q.shape[0], q.shape[1], heads_kv,
+                                        head_dim, *_rows(out), softmax_scale, _ptr(scratch), nbytes, _stream(q))
 
 
 def prompt_attention(q, k, v, cu_seqlens, out, softmax_scale) -> int:

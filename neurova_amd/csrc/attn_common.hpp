@@ -35,4 +35,21 @@ __device__ __forceinline__ float collect4(__amdgpu_buffer_rsrc_t r, uint32_t off
   return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kSc1));
 }
 
+// Sixteen signed bytes -> two MFMA fragments of eight fp16 (exact): the byte
+// with its sign flipped under the exponent of 1024 is 1024 + 128 + c.
+__device__ __forceinline__ void codes_to_half(u32x4 w, f16x8& a, f16x8& b) {
+  u32x4 lo, hi;
+  const f16x2 bias = {(f16)1152.0f, (f16)1152.0f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = w[i] ^ 0x80808080u;
+    const uint32_t x = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
+    const uint32_t y = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
+    if (i < 2) lo[2 * i] = x, lo[2 * i + 1] = y;
+    else hi[2 * i - 4] = x, hi[2 * i - 3] = y;
+  }
+  a = __builtin_bit_cast(f16x8, lo);
+  b = __builtin_bit_cast(f16x8, hi);
+}
+
 }  // namespace lb

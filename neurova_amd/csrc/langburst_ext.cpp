@@ -573,6 +573,28 @@ void kv8_attention_out(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_c
         "kv8_attention_out");
 }
 
+void kv8_chunk_attention_out(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
+                             torch::Tensor v_scale, torch::Tensor page_table, torch::Tensor seq_lens,
+                             torch::Tensor cu_seqlens, torch::Tensor out, double softmax_scale) {
+  const CacheShape c = check_kv8_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens);
+  const RowsView qr = rows_of(q, "q", k_cache), ov = rows_of(out, "out", k_cache);
+  const int64_t tokens = q.size(0), heads_q = q.size(1);
+  TORCH_CHECK(q.size(2) == c.head_dim, "q must be [tokens, heads_q, head_dim]");
+  TORCH_CHECK(heads_q > 0 && c.heads > 0 && heads_q % c.heads == 0, "heads_q must be a multiple of the cache's heads");
+  TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
+  const int32_t* cu = check_cu_seqlens(cu_seqlens, c.batch, k_cache);
+  TORCH_CHECK(softmax_scale > 0 && softmax_scale < 3e38, "softmax_scale must be positive and finite");
+  const c10::DeviceGuard guard(k_cache.device());
+  auto scratch = op_scratch(
+      lb_kv8_chunk_attention_scratch_bytes(c.batch, tokens, heads_q, c.heads, c.head_dim, c.page_size, c.max_pages), q);
+  lb_ok(lb_kv8_chunk_attention(qr.p, qr.token, qr.head, k_cache.data_ptr<int8_t>(), v_cache.data_ptr<int8_t>(),
+                               k_scale.data_ptr<float>(), v_scale.data_ptr<float>(), c.pages, c.page_size,
+                               page_table.data_ptr<int32_t>(), c.max_pages, c.table_stride,
+                               seq_lens.data_ptr<int32_t>(), cu, c.batch, tokens, heads_q, c.heads, c.head_dim, ov.p,
+                               ov.token, ov.head, (float)softmax_scale, scratch.ptr, scratch.bytes, stream_of(k_cache)),
+        "kv8_chunk_attention_out");
+}
+
 void prompt_attention_out(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> cu_seqlens,
                           torch::Tensor out, double softmax_scale) {
   const RowsView qr = rows_of(q, "q", q), kr = rows_of(k, "k", q), vr = rows_of(v, "v", q), ov = rows_of(out, "out", q);
@@ -648,6 +670,10 @@ PYBIND11_MODULE(langburst_cuda, m) {
         "Attention of each sequence's newest tokens over its pages of the 8-bit cache", py::arg("q"),
         py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("page_table"),
         py::arg("seq_lens"), py::arg("out"), py::arg("workspace"), py::arg("softmax_scale"));
+  m.def("kv8_chunk_attention_out", &kv8_chunk_attention_out,
+        "Attention of any number of new tokens of each sequence, packed, over its pages of the 8-bit cache", py::arg("q"),
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("page_table"),
+        py::arg("seq_lens"), py::arg("cu_seqlens"), py::arg("out"), py::arg("softmax_scale"));
   m.def("prompt_attention_out", &prompt_attention_out,
         "Causal attention inside each of the packed sequences of a batch of prompts", py::arg("q"), py::arg("k"),
         py::arg("v"), py::arg("cu_seqlens"), py::arg("out"), py::arg("softmax_scale"));

@@ -85,23 +85,6 @@ constexpr int kParts = 8;        // parts whose loads a thread of the last worke
                                  // tokens beside 15 x 300: 30.6 us, 4 at a time 35.8, 16 the same
 constexpr int kJoinGroups = 16;  // groups of D / 4 threads that join a column's parts in the second launch
 
-// Sixteen signed bytes -> two MFMA fragments of eight fp16 (exact): the byte
-// with its sign flipped under the exponent of 1024 is 1024 + 128 + c.
-__device__ __forceinline__ void codes_to_half(u32x4 w, f16x8& a, f16x8& b) {
-  u32x4 lo, hi;
-  const f16x2 bias = {(f16)1152.0f, (f16)1152.0f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t u = w[i] ^ 0x80808080u;
-    const uint32_t x = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
-    const uint32_t y = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
-    if (i < 2) lo[2 * i] = x, lo[2 * i + 1] = y;
-    else hi[2 * i - 4] = x, hi[2 * i - 3] = y;
-  }
-  a = __builtin_bit_cast(f16x8, lo);
-  b = __builtin_bit_cast(f16x8, hi);
-}
-
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnit - 1) / kUnit : 1; }
 
 // Head dimension 256 is two waves of 128 channels for each stream of tokens (the

@@ -1,0 +1,596 @@
+// Attention of chunks of new tokens over the pages of the 8-bit cache: any number of
+// new tokens a sequence, packed one after the other.
+//
+//   o[i] = sum_j softmax_j(scale q[i] . k[j]) v[j],  j <= len - n + i
+//   k[j] = k_scale[page] ck[j],  v[j] = v_scale[page] cv[j]
+//
+//   S^T = K Q^T    32x32x16: a lane holds 32 keys of one row, so a row's maximum and
+//                  sum stay in the lane but for one exchange with lane ^ 32
+//   O^T = V^T P^T  the weights of a lane are already the second product's operand, and
+//                  the value layout [channel][token] is its other one
+//
+// The 128 rows of a workgroup are (token, query head of the group) pairs of one
+// key/value head.  Four waves of 32 rows go through tiles of 64 keys together: the
+// codes of a tile come into registers while the tile before is computed, become fp16
+// (exactly) and lie in LDS for all four.
+#include "attn_common.hpp"
+
+namespace lb {
+namespace {
+
+struct ChunkArgs {
+  const uint16_t* q;
+  int64_t q_token, q_head;
+  const int8_t *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  const int32_t *page_table, *seq_lens, *starts;
+  uint16_t* out;
+  int64_t o_token, o_head;
+  float* parts;
+  int64_t table_stride;
+  int num_pages, page_shift, max_tokens;
+  int batch, tokens, heads_kv, group;
+  int workers, slots;  // workgroups that run at once; parts that the scratch holds
+  float scale;         // softmax scale * log2(e)
+};
+
+constexpr int kRows = 128, kKeys = 64, kWaves = 4;
+constexpr float kNoMax = -1e30f;
+// The running maximum is that of weight times value scale.  It moves only when
+// exceeded by 2^kSlack, and the weights carry 2^kLift more: at most 2^15, inside
+// fp16, and 2^7 farther from its subnormals.  Value scales count from 2^-kScales to
+// 2^kScales; where all of a tile's are within 2^kNear of one, the scale is part of
+// the exponent, and a weight without it the exponential divided by it.
+constexpr float kSlack = 8.0f, kLift = 7.0f, kScales = 80.0f, kNear = 32.0f;
+// A piece of a row block's keys is this many tiles at least.
+constexpr int kMinTiles = 4;
+
+template <int D>
+constexpr int kPerSimd = D == 64 ? 3 : D == 128 ? 2 : 1;
+
+// ------------------------------------------------------------- the work ---
+
+// A sequence's new tokens begin at packed token `first`, position `at` (below 0 for
+// padding); the table holds its first `len` tokens.
+struct Seq {
+  int first, n, len, at;
+};
+__device__ __forceinline__ Seq seq_of(const ChunkArgs& a, int b) {
+  if (b >= a.batch) return {0, 0, 0, 0};
+  Seq s;
+  s.first = max(a.starts[b], 0);
+  s.n = max(min(a.starts[b + 1], a.tokens) - s.first, 0);
+  const int full = max(a.seq_lens[b], 0);
+  s.len = min(full, a.max_tokens), s.at = full - s.n;
+  return s;
+}
+__device__ __forceinline__ int blocks_of(const ChunkArgs& a, const Seq& s) { return (s.n * a.group + kRows - 1) / kRows; }
+__device__ __forceinline__ int tiles_of(const Seq& s) { return max((s.len + kKeys - 1) / kKeys, 1); }
+// Pieces of each of a sequence's row blocks.  The float quotient is exact enough:
+// (x + 1/2) / most is 1 / (2 most) away from an integer, more than its error.
+__device__ __forceinline__ int pieces_in(int tiles, int most, float inverse) {
+  return (int)(((float)(tiles + most - 1) + 0.5f) * inverse);
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), kWave - 1); }
+
+// Every row block's keys are cut into pieces of at most `most` tiles, a workgroup
+// each: about as many as run at once, where there are fewer row blocks than that.
+struct Work {
+  int most, total;
+};
+__device__ __forceinline__ Work work_of(const ChunkArgs& a, const Seq& own) {
+  const int lane = lane_id();
+  auto sum = [&](auto of) {
+    int n = wave_total(of(own));
+    for (int c = kWave; c < a.batch; c += kWave) n += wave_total(of(seq_of(a, c + lane)));
+    return n;
+  };
+  const int tiles = sum([&](const Seq& s) { return blocks_of(a, s) * tiles_of(s); }) * a.heads_kv;
+  Work w;
+  w.most = max((tiles + a.workers - 1) / a.workers, kMinTiles);
+  for (int tries = 0;; ++tries) {
+    const float inverse = __builtin_amdgcn_rcpf((float)w.most);
+    w.total = sum([&](const Seq& s) { return blocks_of(a, s) * pieces_in(tiles_of(s), w.most, inverse); });
+    if (tries == 8 || w.total * a.heads_kv <= a.workers) return w;
+    w.most += max(w.most / 16, 1);
+  }
+}
+
+// A row block's piece of keys, tiles [t0, t1).
+struct Piece {
+  int b, block, pieces, piece, t0, t1;
+  int slot;  // among the pieces of all split row blocks of one head
+  Seq s;
+};
+__device__ __forceinline__ int block_tiles(const ChunkArgs& a, const Seq& s, int block) {
+  const int last = min(s.n - 1, ((block + 1) * kRows - 1) / a.group);  // token of the last row
+  return max((min(s.at + last + 1, s.len) + kKeys - 1) / kKeys, 0);
+}
+__device__ __forceinline__ Seq seq_from(const Seq& s, int lane) {
+  return {__builtin_amdgcn_readlane(s.first, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.len, lane),
+          __builtin_amdgcn_readlane(s.at, lane)};
+}
+// Piece i of all, in the order of the sequences and the last row block first.
+// JOIN: row block i of those that have several pieces, and its first.
+template <bool JOIN>
+__device__ __forceinline__ bool piece_of(const ChunkArgs& a, const Seq& own, const Work& w, int i, Piece& p) {
+  const int lane = lane_id();
+  const float inverse = __builtin_amdgcn_rcpf((float)w.most);
+  int base = 0, slots = 0;
+  for (int c = 0; c < a.batch; c += kWave) {
+    const Seq s = c ? seq_of(a, c + lane) : own;
+    const int blocks = blocks_of(a, s), pieces = pieces_in(tiles_of(s), w.most, inverse);
+    const int split = pieces > 1 ? blocks * pieces : 0;
+    const int size = JOIN ? (pieces > 1 ? blocks : 0) : blocks * pieces;
+    const int upto = wave_scan(size), all = __builtin_amdgcn_readlane(upto, kWave - 1);
+    const int split_upto = wave_scan(split);
+    if (base + all > i) {
+      const int at = __builtin_ctzll(__ballot(base + upto > i));
+      const int x = i - base - __builtin_amdgcn_readlane(upto - size, at);
+      p.s = seq_from(s, at);
+      p.b = c + at, p.pieces = __builtin_amdgcn_readlane(pieces, at);
+      const int from_last = JOIN ? x : x / p.pieces;
+      p.block = __builtin_amdgcn_readlane(blocks, at) - 1 - from_last;
+      p.piece = JOIN ? 0 : x - from_last * p.pieces;
+      p.slot = slots + __builtin_amdgcn_readlane(split_upto - split, at) + from_last * p.pieces + p.piece;
+      const uint32_t tiles = block_tiles(a, p.s, p.block);
+      p.t0 = tiles * p.piece / p.pieces, p.t1 = tiles * (p.piece + 1) / p.pieces;
+      return true;
+    }
+    base += all, slots += __builtin_amdgcn_readlane(split_upto, kWave - 1);
+  }
+  return false;
+}
+
+// A part: the rows' maxima and sums, then each wave's accumulators as its lanes hold
+// them, sixteen bytes a lane side by side.
+template <int D>
+constexpr int kPartFloats = kRows * (D + 2);
+
+// ------------------------------------------------------------- a tile ---
+
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) {
+  return D == 64 ? (row >> 1) & 7 : row & 15;
+}
+
+// The pages of a tile, lane l those of its 16 tokens l % 4, and the next tile's codes.
+template <int D>
+struct Tiles {
+  static constexpr int N = D / 64;  // loads of keys (and of values) of a thread
+  const ChunkArgs& a;
+  const int32_t* table;
+  int head, len, lane, wave;
+  int groups_shift;  // log2 of the groups of 16 tokens that a page's row holds, of a tile's four
+  uint32_t k_off[N], v_off[N];
+  int page;       // of the tile after the one whose codes are loaded
+  bool held;
+  float ks, vs;   // of the tile whose codes are loaded
+  bool held_codes;
+  u32x4 kc[N], vc[N];
+
+  __device__ __forceinline__ Tiles(const ChunkArgs& args, const Piece& p, int kv_head, int w) : a(args), head(kv_head), len(p.s.len), lane(lane_id()), wave(w) {
+    table = a.page_table + (int64_t)p.b * a.table_stride;
+    groups_shift = min(a.page_shift - 4, 2);
+    const int per = kWave >> groups_shift;  // channels of a load
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = (i * kWaves + wave) * kWave + lane;
+      k_off[i] = ((x / (D / 16)) & 15) * D + (x % (D / 16)) * 16;
+      const int y = i * kWaves + wave, in = D / per;
+      v_off[i] = (((y % in) * per + (lane >> groups_shift)) << a.page_shift) + (lane & ((1 << groups_shift) - 1)) * 16;
+    }
+  }
+  __device__ __forceinline__ void load_page(int tile) {
+    const int t = tile * kKeys + 16 * (lane & 3);
+    page = table[min(t, len - 1) >> a.page_shift];
+    held = t < len;
+  }
+  // Codes and scales of `tile`, whose pages are known.
+  __device__ __forceinline__ void load_codes(int tile) {
+    const int mask = (1 << a.page_shift) - 1;
+    held_codes = held && (unsigned)page < (unsigned)a.num_pages;
+    const int safe = held_codes ? page : 0;
+    const int cell = safe * a.heads_kv + head;
+    ks = a.k_scale[cell], vs = a.v_scale[cell];
+    const int in = D / (kWave >> groups_shift);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int g = (i * kWaves + wave) * (kWave * 16 / D) / 16;  // the load's 16 tokens
+      const int64_t c = __builtin_amdgcn_readlane(cell, g);
+      const int8_t* from = a.k_cache + ((c << a.page_shift) + ((tile * kKeys + 16 * g) & mask)) * D;
+      kc[i] = *reinterpret_cast<const u32x4*>(from + k_off[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int g = (i * kWaves + wave) / in << groups_shift;
+      const int64_t c = __builtin_amdgcn_readlane(cell, g);
+      const int8_t* from = a.v_cache + ((c * D) << a.page_shift) + ((tile * kKeys + 16 * g) & mask);
+      vc[i] = *reinterpret_cast<const u32x4*>(from + v_off[i]);
+    }
+  }
+  // As fp16 into LDS: keys [token][channel], values [channel][token], the tokens of a
+  // group in the order of the second product's operand (of 4 h .. 4 h + 3 and 8 more
+  // the half h); chunks of 16 bytes change places so that reads use every bank.
+  __device__ __forceinline__ void store(uint16_t* kl, uint16_t* vl) const {
+    const int in = D / (kWave >> groups_shift);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      f16x8 x, y;
+      codes_to_half(kc[i], x, y);
+      const int c = (i * kWaves + wave) * kWave + lane, row = c / (D / 16), col = 2 * (c % (D / 16)), swz = k_swizzle<D>(row);
+      *reinterpret_cast<f16x8*>(kl + row * D + 8 * (col ^ swz)) = x;
+      *reinterpret_cast<f16x8*>(kl + row * D + 8 * ((col + 1) ^ swz)) = y;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      f16x8 x, y;
+      codes_to_half((u32x4){vc[i][0], vc[i][2], vc[i][1], vc[i][3]}, x, y);
+      const int w = i * kWaves + wave;
+      const int g = ((w / in) << groups_shift) + (lane & ((1 << groups_shift) - 1));
+      const int ch = (w % in) * (kWave >> groups_shift) + (lane >> groups_shift);
+      *reinterpret_cast<f16x8*>(vl + ch * kKeys + 8 * ((2 * g) ^ (ch & 7))) = x;
+      *reinterpret_cast<f16x8*>(vl + ch * kKeys + 8 * ((2 * g + 1) ^ (ch & 7))) = y;
+    }
+  }
+};
+
+// What the scores of a tile's four groups of 16 tokens are multiplied with, and their
+// values' scales.
+struct Scales {
+  float k[4], log[4], inverse[4], v[4];
+  uint32_t held;  // bit g
+  bool plain;     // nothing special about any of them
+};
+
+template <int D>
+__global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(ChunkArgs a) {
+  constexpr int DT = D / 32, KK = D / 16, ST = kKeys / 32;
+  // four arrays and not one: reads of a tile then need not wait for writes of the next
+  __shared__ __align__(16) uint16_t k0[kKeys * D], k1[kKeys * D], v0[kKeys * D], v1[kKeys * D];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.x % a.heads_kv, item = blockIdx.x / a.heads_kv;
+  Piece p;
+  {
+    const Seq own = seq_of(a, lane);
+    const Work w = work_of(a, own);
+    if (!piece_of<false>(a, own, w, item, p)) return;
+  }
+  const int rows = p.s.n * a.group, wave_row = p.block * kRows + wave * 32;
+  const int row = wave_row + r, token = row / a.group, q_head = kvh * a.group + row - token * a.group;
+  const bool real = row < rows;
+  // the wave's rows see the keys up to `seen`, all of them those up to `all_see`
+  const int seen = real ? min(p.s.at + token, p.s.len - 1) : -1;
+  const int all_see = min(p.s.at + wave_row / a.group, p.s.len - 1);
+  const int any_see = wave_row < rows ? min(p.s.at + min(rows - 1, wave_row + 31) / a.group, p.s.len - 1) : -1;
+
+  f16x8 qf[KK];
+  {
+    const uint16_t* from = a.q + (int64_t)(p.s.first + token) * a.q_token + (int64_t)q_head * a.q_head;
+#pragma unroll
+    for (int k = 0; k < KK; ++k) {
+      qf[k] = (f16x8)((f16)0.0f);
+      if (real) qf[k] = *reinterpret_cast<const f16x8*>(from + 16 * k + 8 * h);
+    }
+  }
+  f32x16 o[DT];
+  float m = kNoMax, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = (f32x16)(0.0f);
+
+  Tiles<D> tiles(a, p, kvh, wave);
+  if (p.t0 < p.t1) {
+    tiles.load_page(p.t0);
+    tiles.load_codes(p.t0);
+    tiles.load_page(p.t0 + 1);
+    tiles.store(k0, v0);
+  }
+
+  // Tile kt from (kl, vl); the next tile's codes go to (kn, vn).
+  Scales sc;
+  auto scales = [&]() {
+    const float k = tiles.held_codes ? tiles.ks * a.scale + (tiles.ks - tiles.ks) : 0.0f;
+    const float lg = __builtin_fmaxf(__builtin_fminf(__builtin_amdgcn_logf(__builtin_fabsf(tiles.vs)), kScales), -kScales);
+    const float inv = __builtin_amdgcn_exp2f(-lg - kLift);
+    const bool plain = tiles.held_codes && k > 0.0f && k < __builtin_inff() && tiles.vs > 0.0f && __builtin_fabsf(lg) <= kNear;
+    sc.held = (uint32_t)__ballot(tiles.held_codes) & 15;
+    sc.plain = ((uint32_t)__ballot(plain) & 15) == 15;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      auto at = [&](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), g)); };
+      sc.k[g] = at(k), sc.log[g] = at(lg), sc.inverse[g] = at(inv), sc.v[g] = at(tiles.vs);
+    }
+  };
+  auto take = [&](int kt, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
+    scales();
+    lds_barrier();
+    if (kt + 1 < p.t1) {
+      tiles.load_codes(kt + 1);
+      tiles.load_page(kt + 2);
+    }
+    if (kt * kKeys <= any_see) {
+      f32x16 s[ST];
+#pragma unroll
+      for (int t = 0; t < ST; ++t) s[t] = (f32x16)(0.0f);
+#pragma unroll
+      for (int k = 0; k < KK; ++k)
+#pragma unroll
+        for (int t = 0; t < ST; ++t) {
+          const int key = 32 * t + r;
+          const f16x8 kf = *reinterpret_cast<const f16x8*>(kl + key * D + 8 * ((2 * k + h) ^ k_swizzle<D>(key)));
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[k], s[t], 0, 0, 0);
+        }
+      const bool plain = sc.plain && kt * kKeys + kKeys - 1 <= all_see;
+      float peak = kNoMax;
+      if (plain) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float x = s[g / 2][8 * (g % 2)];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) x = __builtin_fmaxf(x, s[g / 2][8 * (g % 2) + i]);
+          peak = __builtin_fmaxf(peak, x * sc.k[g] + sc.log[g]);
+        }
+      } else {
+        const int past = seen - kt * kKeys - 4 * h;  // keys of the lane up to here are seen
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int g = 2 * t + i / 8;
+            float x = s[t][i] * sc.k[g];
+            if (32 * t + 8 * (i >> 2) + (i & 3) > past || !(sc.held >> g & 1)) x = -__builtin_inff();
+            s[t][i] = x;
+            peak = __builtin_fmaxf(peak, x + sc.log[g]);
+          }
+      }
+      if (__any(peak > m + kSlack)) {
+        // row by row: what other rows of the wave see changes no bit of a row
+        float up = __builtin_fmaxf(peak, from_lane(peak, lane ^ 32));
+        if (!(up > m + kSlack)) up = m;
+        const float f = __builtin_amdgcn_exp2f(m - up);
+        m = up;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= f;
+      }
+      f16x8 pf[2 * ST];
+      if (plain) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float lift = sc.log[g] + kLift - m;
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float w = __builtin_amdgcn_exp2f(s[g / 2][8 * (g % 2) + i] * sc.k[g] + lift);
+            sum += w;
+            pf[g][i] = (f16)w;
+          }
+          l += sum * sc.inverse[g];
+        }
+      } else {
+        const int past = seen - kt * kKeys - 4 * h;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float lifted = sc.v[g] * __builtin_exp2f(kLift);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float w = __builtin_amdgcn_exp2f(s[g / 2][8 * (g % 2) + i] - m);
+            l += w;
+            // no weight, and none of a value scale that is not finite either
+            const bool sees = 16 * g + 8 * (i >> 2) + (i & 3) <= past && (sc.held >> g & 1);
+            pf[g][i] = (f16)(sees ? w * lifted : 0.0f);
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2 * ST; ++c)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const int ch = 32 * d + r;
+          const f16x8 vf = *reinterpret_cast<const f16x8*>(vl + ch * kKeys + 8 * ((2 * c + h) ^ (ch & 7)));
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[c], o[d], 0, 0, 0);
+        }
+    }
+    if (kt + 1 < p.t1) tiles.store(kn, vn);
+  };
+  for (int kt = p.t0; kt < p.t1; kt += 2) {
+    take(kt, k0, v0, k1, v1);
+    if (kt + 1 < p.t1) take(kt + 1, k1, v1, k0, v0);
+  }
+
+  l += from_lane(l, lane ^ 32);
+  if (p.pieces > 1) {
+    const int slot = p.slot * a.heads_kv + kvh;
+    if (slot >= a.slots) return;
+    float* part = a.parts + (int64_t)slot * kPartFloats<D>;
+    if (real) {
+      if (h == 0) part[wave * 32 + r] = m, part[kRows + wave * 32 + r] = l;
+      f32x4* to = reinterpret_cast<f32x4*>(part + 2 * kRows + wave * 32 * D) + lane;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          to[(4 * d + i) * kWave] = (f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+    }
+    return;
+  }
+  // the rows leave through LDS, a wave's 32 x D in an array that no wave reads any more
+  lds_barrier();
+  uint16_t* mine = wave < 2 ? (wave == 0 ? k0 : k1) : (wave == 2 ? v0 : v1);
+  const float inv = l > 0.0f ? __builtin_exp2f(-kLift) / l : l == 0.0f ? 0.0f : l;
+  const int64_t place = (int64_t)(p.s.first + token) * a.o_token + (int64_t)q_head * a.o_head;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      u32x2 w;
+      w[0] = as_u32((f16x2){(f16)(o[d][i] * inv), (f16)(o[d][i + 1] * inv)});
+      w[1] = as_u32((f16x2){(f16)(o[d][i + 2] * inv), (f16)(o[d][i + 3] * inv)});
+      const int chunk = (4 * d + i / 4) ^ k_swizzle<D>(r);
+      *reinterpret_cast<u32x2*>(mine + r * D + 8 * chunk + 4 * h) = w;
+    }
+#pragma unroll
+  for (int j = 0; j < 32 * D / 8 / kWave; ++j) {
+    const int x = j * kWave + lane, rr = x / (D / 8), chunk = x % (D / 8);
+    const uint32_t lo = from_lane((uint32_t)place, rr), hi = from_lane((uint32_t)(place >> 32), rr);
+    const u32x4 w = *reinterpret_cast<const u32x4*>(mine + rr * D + 8 * (chunk ^ k_swizzle<D>(rr)));
+    if (wave_row + rr < rows)
+      *reinterpret_cast<u32x4*>(a.out + (int64_t)(((uint64_t)hi << 32) | lo) + 8 * chunk) = w;
+  }
+}
+
+// Joins the parts of the row blocks that were cut: 32 rows and 32 channels a
+// workgroup, the parts dealt to its waves in turn.
+template <int D>
+__global__ __launch_bounds__(kWave * kWaves) void kv8_chunk_join_kernel(ChunkArgs a) {
+  __shared__ float sm[kWaves][kWave], sl[kWaves][kWave];
+  __shared__ f32x4 so[kWaves][4][kWave];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 31, h = lane >> 5;
+  constexpr int DT = D / 32;
+  const Seq own = seq_of(a, lane);
+  const Work w = work_of(a, own);
+  for (int x = blockIdx.x;; x += gridDim.x) {
+    int y = x / a.heads_kv;
+    const int kvh = x - y * a.heads_kv, d = y % DT, quarter = y / DT % kWaves;
+    Piece p;
+    if (!piece_of<true>(a, own, w, y / (DT * kWaves), p)) return;
+    const int rows = p.s.n * a.group, first_row = p.block * kRows + quarter * 32;
+    if (first_row >= rows) continue;
+    const int row = first_row + r, token = row / a.group, q_head = kvh * a.group + row - token * a.group;
+    float m = kNoMax, l = 0.0f;
+    f32x4 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = (f32x4)(0.0f);
+    if (row < rows)
+      for (int j = wave; j < p.pieces; j += kWaves) {
+        const int slot = (p.slot + j) * a.heads_kv + kvh;
+        if (slot >= a.slots) break;
+        const float* part = a.parts + (int64_t)slot * kPartFloats<D>;
+        const float pm = part[quarter * 32 + r], pl = part[kRows + quarter * 32 + r];
+        const f32x4* from = reinterpret_cast<const f32x4*>(part + 2 * kRows + quarter * 32 * D) + 4 * d * kWave + lane;
+        const float up = __builtin_fmaxf(m, pm);
+        const float f = __builtin_amdgcn_exp2f(m - up), fp = __builtin_amdgcn_exp2f(pm - up);
+        m = up, l = l * f + pl * fp;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = o[i] * f + from[i * kWave] * fp;
+      }
+    sm[wave][lane] = m, sl[wave][lane] = l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) so[wave][i][lane] = o[i];
+    __syncthreads();
+    float up = kNoMax, sum = 0.0f;
+    f32x4 v = (f32x4)(0.0f);  // wave i: the lane's channels 8 i .. 8 i + 3 past 4 h
+#pragma unroll
+    for (int j = 0; j < kWaves; ++j) up = __builtin_fmaxf(up, sm[j][lane]);
+#pragma unroll
+    for (int j = 0; j < kWaves; ++j) {
+      const float f = __builtin_amdgcn_exp2f(sm[j][lane] - up);
+      sum += sl[j][lane] * f, v += so[j][wave][lane] * f;
+    }
+    if (row < rows) {
+      const float inv = sum > 0.0f ? __builtin_exp2f(-kLift) / sum : sum == 0.0f ? 0.0f : sum;
+      u32x2 c;
+      c[0] = as_u32((f16x2){(f16)(v[0] * inv), (f16)(v[1] * inv)});
+      c[1] = as_u32((f16x2){(f16)(v[2] * inv), (f16)(v[3] * inv)});
+      *reinterpret_cast<u32x2*>(a.out + (int64_t)(p.s.first + token) * a.o_token + (int64_t)q_head * a.o_head + 32 * d + 8 * wave + 4 * h) = c;
+    }
+    __syncthreads();
+  }
+}
+
+struct Plan {
+  int64_t workers, slots, grid;
+  int joined;
+  size_t scratch;
+};
+
+// Row blocks that are cut have more than `most` tiles each, of workers * most in all:
+// at most as many as the workers, and their pieces twice that.
+Plan plan_of(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv, int64_t head_dim, int64_t max_tokens) {
+  Plan p;
+  p.workers = (head_dim == 64 ? kPerSimd<64> : head_dim == 128 ? kPerSimd<128> : kPerSimd<256>) * (int64_t)lbh::device_cus();
+  const int64_t blocks = (tokens * (heads_q / heads_kv) / kRows + batch) * heads_kv;
+  const int64_t tiles = (max_tokens + kKeys - 1) / kKeys;
+  p.joined = tiles > kMinTiles;
+  // no more pieces than all row blocks have of the smallest size
+  const int64_t pieces = blocks * ((tiles + kMinTiles - 1) / kMinTiles);
+  p.slots = !p.joined ? 0 : pieces < 2 * p.workers ? pieces : 2 * p.workers;
+  p.grid = blocks + p.slots;
+  p.scratch = ((size_t)p.slots * kRows * (head_dim + 2) * 4 + 255) & ~(size_t)255;
+  return p;
+}
+
+int check_sizes(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv, int64_t head_dim, int64_t page_size,
+                int64_t max_pages) {
+  if (batch < 0 || tokens < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0 || max_pages < 0) return LB_ERR_ARG;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return LB_ERR_PROB_SHAPE;
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return LB_ERR_PROB_SHAPE;
+  if (heads_q > 4096 || batch > (1 << 20) || tokens > (1 << 24) || max_pages > (1 << 28) / page_size) return LB_ERR_ARG;
+  // tiles and pieces are numbered in 32 bits
+  const int64_t blocks = (tokens * (heads_q / heads_kv) / kRows + batch) * heads_kv;
+  const int64_t tiles = max_pages * page_size / kKeys + 1;
+  if (blocks > (1 << 30) / tiles || tokens * (heads_q / heads_kv) > (1 << 30)) return LB_ERR_PROB_SHAPE;
+  return LB_OK;
+}
+
+template <int D>
+void launch(const ChunkArgs& a, const Plan& p, hipStream_t st) {
+  kv8_chunk_kernel<D><<<dim3((unsigned)p.grid), dim3(kWave * kWaves), 0, st>>>(a);
+  if (!p.joined) return;
+  const int64_t units = p.workers * kWaves * (D / 32), most = 8 * (int64_t)lbh::device_cus();
+  kv8_chunk_join_kernel<D><<<dim3((unsigned)(units < most ? units : most)), dim3(kWave * kWaves), 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace lb
+
+extern "C" size_t lb_kv8_chunk_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv,
+                                                       int64_t head_dim, int64_t page_size, int64_t max_pages) {
+  if (lb::check_sizes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages) != LB_OK || batch == 0 || tokens == 0)
+    return 0;
+  return lb::plan_of(batch, tokens, heads_q, heads_kv, head_dim, page_size * max_pages).scratch;
+}
+
+extern "C" int lb_kv8_chunk_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const int8_t* k_cache,
+                                      const int8_t* v_cache, const float* k_scale, const float* v_scale, int64_t num_pages,
+                                      int64_t page_size, const int32_t* page_table, int64_t max_pages, int64_t table_stride,
+                                      const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t batch, int64_t tokens,
+                                      int64_t heads_q, int64_t heads_kv, int64_t head_dim, uint16_t* out,
+                                      int64_t o_token_stride, int64_t o_head_stride, float softmax_scale, void* scratch,
+                                      size_t scratch_bytes, lb_stream_t stream) {
+  using namespace lb;
+  const int err = check_sizes(batch, tokens, heads_q, heads_kv, head_dim, page_size, max_pages);
+  if (err != LB_OK) return err;
+  if (num_pages < 0 || num_pages > 0x7fffffff / heads_kv || table_stride < max_pages) return LB_ERR_ARG;
+  if (!(softmax_scale > 0.0f) || softmax_scale > 3e38f) return LB_ERR_ARG;
+  if (batch == 0 || tokens == 0) return LB_OK;
+  if (!q || !out || !seq_lens || !cu_seqlens) return LB_ERR_ARG;
+  if (num_pages > 0 && max_pages > 0 && (!k_cache || !v_cache || !k_scale || !v_scale || !page_table)) return LB_ERR_ARG;
+  const void* ptrs[] = {q, out, k_cache, v_cache, scratch};
+  for (const void* p : ptrs)
+    if (!lbh::aligned(p, 16)) return LB_ERR_ALIGN;
+  if ((q_token_stride | q_head_stride | o_token_stride | o_head_stride) % 8 != 0) return LB_ERR_ALIGN;
+  // without pages no sequence holds a token
+  const int64_t max_tokens = num_pages > 0 ? max_pages * page_size : 0;
+  const Plan p = plan_of(batch, tokens, heads_q, heads_kv, head_dim, max_tokens);
+  if (p.scratch > 0 && (scratch_bytes < p.scratch || !scratch)) return LB_ERR_SCRATCH;
+
+  ChunkArgs a;
+  a.q = q, a.q_token = q_token_stride, a.q_head = q_head_stride;
+  a.k_cache = k_cache, a.v_cache = v_cache, a.k_scale = k_scale, a.v_scale = v_scale;
+  a.page_table = page_table, a.seq_lens = seq_lens, a.starts = cu_seqlens;
+  a.out = out, a.o_token = o_token_stride, a.o_head = o_head_stride;
+  a.parts = static_cast<float*>(scratch), a.table_stride = table_stride;
+  a.num_pages = (int)num_pages, a.page_shift = __builtin_ctzll((unsigned long long)page_size);
+  a.max_tokens = (int)max_tokens;
+  a.batch = (int)batch, a.tokens = (int)tokens, a.heads_kv = (int)heads_kv, a.group = (int)(heads_q / heads_kv);
+  a.workers = (int)p.workers, a.slots = (int)p.slots;
+  a.scale = softmax_scale * kLog2e;
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (head_dim == 256) launch<256>(a, p, st);
+  else if (head_dim == 128) launch<128>(a, p, st);
+  else launch<64>(a, p, st);
+  return lbh::launch_status();
+}

@@ -358,6 +358,78 @@ int lb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_hea
                         uint16_t* out, int64_t o_token_stride, int64_t o_head_stride, float softmax_scale,
                         lb_stream_t stream);
 
+/* ---------------- Pages of the 8-bit cache (no reference counterpart) ----------------
+ * Which row of a table holds which page, and how many rows hold each: page_table
+ * int32 [rows, max_pages] (rows table_stride apart), seq_lens int32 [rows] and refs
+ * int32 [num_pages] (16-byte aligned), all on the device and changed in place.  A
+ * row of n tokens holds the first ceil(n / page_size) entries of its table row, -1
+ * behind them; a page that no row holds (refs 0) is free.  All zeros and -1 is a
+ * table without tokens.  `which`, `parents`, `children` name rows of the table, at
+ * most 4096 in a call; one outside the table is left out, one that is named twice
+ * counts as stated.  Results depend on the state alone, never on timing.  Calls
+ * that change the same tables must be ordered. */
+
+/* One layer's cache, as lb_kv8_append writes it. */
+typedef struct lb_kv8_layer {
+  int8_t* k_cache;
+  int8_t* v_cache;
+  float* k_scale;
+  float* v_scale;
+} lb_kv8_layer;
+
+/* The rows keep their first keep[i] tokens (NULL: none), at most what they hold,
+ * and give up the pages behind them.  A row named twice keeps the least.  One launch. */
+int lb_kv8_pages_free(int32_t* page_table, int64_t rows, int64_t max_pages, int64_t table_stride,
+                      int32_t* seq_lens, int32_t* refs, int64_t num_pages, int64_t page_size,
+                      const int32_t* which, const int32_t* keep, int64_t count, lb_stream_t stream);
+
+/* children[i] becomes the first lens[i] tokens (NULL: all) of parents[i], at most
+ * what that holds, by holding its pages too: nothing is copied.  Every request goes
+ * by the tables as they were before the call.  A child that holds tokens, or that an
+ * earlier request names, is left as it is; done (may be NULL) int32 [count] says 1
+ * for the others.  Two launches. */
+int lb_kv8_pages_fork(int32_t* page_table, int64_t rows, int64_t max_pages, int64_t table_stride,
+                      int32_t* seq_lens, int32_t* refs, int64_t num_pages, int64_t page_size,
+                      const int32_t* parents, const int32_t* children, const int32_t* lens, int32_t* done,
+                      int64_t count, lb_stream_t stream);
+
+/* The rows get add[i] more tokens and the pages for them, the lowest free ones in
+ * the order of the rows.  A row's last page that is not full and that others hold
+ * too is copied, in every layer, before it gets tokens: of its holders among the
+ * rows of the call all but the last get a copy, and the last too where others hold
+ * it.  (A copy has the whole page's codes and scales.)  A row's page comes before
+ * its new ones.  All or nothing: *status is 0, or how many pages are missing, -1
+ * where a row would pass the end of its table, -2 where a page would have to be
+ * copied and no layers are given; nothing has changed then.  Of a row that is named
+ * twice the first counts.  layers: host array, num_layers caches of num_pages pages
+ * of the same shape (0: none).  One launch, and one more for each 32 layers.
+ * scratch: lb_kv8_pages_extend_scratch_bytes(), 16-byte aligned, no initialisation. */
+size_t lb_kv8_pages_extend_scratch_bytes(int64_t num_pages);
+int lb_kv8_pages_extend(int32_t* page_table, int64_t rows, int64_t max_pages, int64_t table_stride,
+                        int32_t* seq_lens, int32_t* refs, int64_t num_pages, int64_t page_size,
+                        const int32_t* which, const int32_t* add, int64_t count, int32_t* status,
+                        const lb_kv8_layer* layers, int64_t num_layers, int64_t heads_kv, int64_t head_dim,
+                        void* scratch, size_t scratch_bytes, lb_stream_t stream);
+
+/* Moves the pages in use to the front of the pool: with *used of them, the i-th page
+ * in use behind the first *used places goes to the i-th free one of these, in every
+ * layer, and every entry of the table follows.  What the places behind hold
+ * afterwards stays there and means nothing.  One launch, and one for each 32 layers (one without).
+ * scratch: lb_kv8_pages_compact_scratch_bytes(), 16-byte aligned, no initialisation. */
+size_t lb_kv8_pages_compact_scratch_bytes(int64_t num_pages);
+int lb_kv8_pages_compact(int32_t* page_table, int64_t rows, int64_t max_pages, int64_t table_stride,
+                         int32_t* refs, int64_t num_pages, int32_t* used,
+                         const lb_kv8_layer* layers, int64_t num_layers, int64_t heads_kv, int64_t page_size,
+                         int64_t head_dim, void* scratch, size_t scratch_bytes, lb_stream_t stream);
+
+/* Copies pages src[i] to dst[i], codes and scales, in every layer; a pair with a
+ * number outside the pool is left out.  A page must not be the destination of two
+ * pairs, nor the destination of one and the source of another: what it then holds
+ * is undefined.  One launch for each 32 layers. */
+int lb_kv8_copy_pages(const lb_kv8_layer* layers, int64_t num_layers, int64_t num_pages, int64_t heads_kv,
+                      int64_t page_size, int64_t head_dim, const int32_t* src, const int32_t* dst, int64_t count,
+                      lb_stream_t stream);
+
 /* ---------------- Measurement probe (no reference counterpart) ----------------
  * Reads `bytes` (a multiple of 16) of device memory at `src` with 16-byte
  * non-temporal loads over `workgroups` workgroups of 256 threads, each a

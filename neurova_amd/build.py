@@ -42,7 +42,7 @@ HIP_SOURCES = [(f"{n}.hip", n, []) for n in ("lb_rowwise", "lb_marlin", "lb_prob
 # fp contraction follows the pragmas in the attention sources: the cache's writer
 # rounds each operation of the rotation and the codes by itself
 HIP_SOURCES += [(f"{n}.hip", n, ["-ffp-contract=fast-honor-pragmas"])
-                for n in ("lb_kv8_append", "lb_kv8_attention", "lb_kv8_chunk", "lb_prompt_attention")]
+                for n in ("lb_kv8_append", "lb_kv8_attention", "lb_kv8_chunk", "lb_kv8_pages", "lb_prompt_attention")]
 HIP_SOURCES += [("lb_rowwise_mm.hip", f"lb_rowwise_mm{b}", [f"-DLB_RW_BITS={b}"]) for b in range(2, 9)]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",

@@ -61,6 +61,13 @@ _SIGNATURES = {
     "lb_kv8_chunk_attention_scratch_bytes": ([I64] * 7, SZ),
     "lb_kv8_chunk_attention": ([P, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, P, I64, I64, F32,
                                 P, SZ, P], ctypes.c_int),
+    "lb_kv8_pages_free": ([P, I64, I64, I64, P, P, I64, I64, P, P, I64, P], ctypes.c_int),
+    "lb_kv8_pages_fork": ([P, I64, I64, I64, P, P, I64, I64, P, P, P, P, I64, P], ctypes.c_int),
+    "lb_kv8_pages_extend_scratch_bytes": ([I64], SZ),
+    "lb_kv8_pages_extend": ([P, I64, I64, I64, P, P, I64, I64, P, P, I64, P, P, I64, I64, I64, P, SZ, P], ctypes.c_int),
+    "lb_kv8_pages_compact_scratch_bytes": ([I64], SZ),
+    "lb_kv8_pages_compact": ([P, I64, I64, I64, P, I64, P, P, I64, I64, I64, I64, P, SZ, P], ctypes.c_int),
+    "lb_kv8_copy_pages": ([P, I64, I64, I64, I64, I64, P, P, I64, P], ctypes.c_int),
     "lb_prompt_attention": ([P, I64, I64] * 3 + [P, I64, I64, I64, I64, I64, P, I64, I64, F32, P], ctypes.c_int),
     "lb_marlin_mlp_fused": ([P, P, P, P, P, P, I64, I64, I64, I64, I64, P, I64, P, SZ, P], ctypes.c_int),
 }
@@ -275,6 +282,48 @@ def kv8_chunk_attention(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_l
                                         page_size, _ptr(page_table), page_table.shape[1], page_table.stride(0),
                                         _ptr(seq_lens), _ptr(cu_seqlens), seq_lens.shape[0], q.shape[0], q.shape[1], heads_kv,
                                         head_dim, *_rows(out), softmax_scale, _ptr(scratch), nbytes, _stream(q))
+
+
+class KV8Layer(ctypes.Structure):
+    _fields_ = [("k_cache", P), ("v_cache", P), ("k_scale", P), ("v_scale", P)]
+
+
+def kv8_layers(caches):
+    """The host array of layers' caches, each (k_cache, v_cache, k_scale, v_scale)."""
+    return (KV8Layer * max(1, len(caches)))(*(KV8Layer(*map(_ptr, c)) for c in caches))
+
+
+def _pages(page_table, *after) -> tuple:
+    return (_ptr(page_table), page_table.shape[0], page_table.shape[1], page_table.stride(0), *map(_ptr, after))
+
+
+def kv8_pages_free(page_table, seq_lens, refs, page_size, rows, keep=None) -> int:
+    return lib().lb_kv8_pages_free(*_pages(page_table, seq_lens, refs), refs.numel(), page_size, _ptr(rows), _ptr(keep), rows.numel(),
+                                   _stream(refs))
+
+
+def kv8_pages_fork(page_table, seq_lens, refs, page_size, parents, children, lens=None, done=None) -> int:
+    return lib().lb_kv8_pages_fork(*_pages(page_table, seq_lens, refs), refs.numel(), page_size, _ptr(parents), _ptr(children),
+                                   _ptr(lens), _ptr(done), parents.numel(), _stream(refs))
+
+
+def kv8_pages_extend(page_table, seq_lens, refs, page_size, rows, add, status, caches, scratch) -> int:
+    heads, dim = (caches[0][0].shape[1], caches[0][0].shape[3]) if caches else (0, 0)
+    return lib().lb_kv8_pages_extend(*_pages(page_table, seq_lens, refs), refs.numel(), page_size, _ptr(rows), _ptr(add), rows.numel(),
+                                     _ptr(status), kv8_layers(caches), len(caches), heads, dim, _ptr(scratch), scratch.numel(),
+                                     _stream(refs))
+
+
+def kv8_pages_compact(page_table, refs, page_size, used, caches, scratch) -> int:
+    heads, dim = (caches[0][0].shape[1], caches[0][0].shape[3]) if caches else (0, 0)
+    return lib().lb_kv8_pages_compact(*_pages(page_table, refs), refs.numel(), _ptr(used), kv8_layers(caches), len(caches), heads,
+                                      page_size, dim, _ptr(scratch), scratch.numel(), _stream(refs))
+
+
+def kv8_copy_pages(caches, src, dst) -> int:
+    pages, heads, page_size, dim = caches[0][0].shape
+    return lib().lb_kv8_copy_pages(kv8_layers(caches), len(caches), pages, heads, page_size, dim, _ptr(src), _ptr(dst), src.numel(),
+                                   _stream(src))
 
 
 def prompt_attention(q, k, v, cu_seqlens, out, softmax_scale) -> int:

@@ -614,6 +614,165 @@ void prompt_attention_out(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10
         "prompt_attention_out");
 }
 
+// ------------------------------------------------------------------ pages ---
+
+// The layers' caches, checked once and kept alive; calls take their addresses from here.
+struct KV8Layers {
+  std::vector<torch::Tensor> held;
+  std::vector<lb_kv8_layer> at;
+  int64_t pages = 0, heads = 0, page_size = 0, head_dim = 0;
+
+  KV8Layers(std::vector<torch::Tensor> k_caches, std::vector<torch::Tensor> v_caches,
+            std::vector<torch::Tensor> k_scales, std::vector<torch::Tensor> v_scales) {
+    const size_t n = k_caches.size();
+    TORCH_CHECK(n > 0, "at least one layer");
+    TORCH_CHECK(v_caches.size() == n && k_scales.size() == n && v_scales.size() == n,
+                "k_caches, v_caches, k_scales and v_scales must name the same layers");
+    for (size_t i = 0; i < n; ++i) {
+      const torch::Tensor &k_cache = k_caches[i], &v_cache = v_caches[i], &k_scale = k_scales[i], &v_scale = v_scales[i];
+      LB_CHECK_DEV(k_cache); LB_CHECK_DEV(v_cache); LB_CHECK_DEV(k_scale); LB_CHECK_DEV(v_scale);
+      LB_CHECK_CONTIG(k_cache); LB_CHECK_CONTIG(v_cache); LB_CHECK_CONTIG(k_scale); LB_CHECK_CONTIG(v_scale);
+      LB_CHECK_FLOAT(k_scale); LB_CHECK_FLOAT(v_scale);
+      TORCH_CHECK(k_cache.scalar_type() == at::kChar && v_cache.scalar_type() == at::kChar,
+                  "k_cache and v_cache must be int8");
+      TORCH_CHECK(k_cache.dim() == 4, "k_cache must be [pages, heads, page_size, head_dim]");
+      TORCH_CHECK(k_cache.sizes() == k_caches[0].sizes(), "the layers' caches must have the same shape");
+      TORCH_CHECK(v_cache.dim() == 4 && v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1) &&
+                      v_cache.size(2) == k_cache.size(3) && v_cache.size(3) == k_cache.size(2),
+                  "v_cache must be [pages, heads, head_dim, page_size]");
+      TORCH_CHECK(k_scale.dim() == 2 && k_scale.size(0) == k_cache.size(0) && k_scale.size(1) == k_cache.size(1),
+                  "k_scale must be [pages, heads]");
+      TORCH_CHECK(v_scale.sizes() == k_scale.sizes(), "v_scale must be [pages, heads]");
+      for (const torch::Tensor* t : {&k_cache, &v_cache, &k_scale, &v_scale}) {
+        TORCH_CHECK(t->device() == k_caches[0].device(), "the layers' caches must be on the same device");
+        held.push_back(*t);
+      }
+      at.push_back({k_cache.data_ptr<int8_t>(), v_cache.data_ptr<int8_t>(), k_scale.data_ptr<float>(),
+                    v_scale.data_ptr<float>()});
+    }
+    pages = k_caches[0].size(0), heads = k_caches[0].size(1);
+    page_size = k_caches[0].size(2), head_dim = k_caches[0].size(3);
+    TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim must be 64, 128 or 256");
+    TORCH_CHECK(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128,
+                "page_size must be 16, 32, 64 or 128");
+  }
+};
+
+constexpr int64_t kMaxPageRows = 4096;  // rows that one call names
+
+struct TableView {
+  int32_t *table, *refs;
+  int64_t rows, width, stride, pages;
+};
+
+TableView check_pages(const torch::Tensor& page_table, const torch::Tensor& refs) {
+  LB_CHECK_DEV(page_table); LB_CHECK_DEV(refs); LB_CHECK_CONTIG(refs); LB_CHECK_I32(page_table); LB_CHECK_I32(refs);
+  TORCH_CHECK(page_table.device() == refs.device(), "page_table and refs must be on the same device");
+  TORCH_CHECK(refs.dim() == 1, "refs must be [pages]");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(refs.data_ptr()) % 16 == 0, "refs must be 16-byte aligned");
+  TORCH_CHECK(page_table.dim() == 2, "page_table must be [rows, max_pages]");
+  TableView v;
+  v.table = page_table.data_ptr<int32_t>(), v.refs = refs.data_ptr<int32_t>();
+  v.rows = page_table.size(0), v.width = page_table.size(1), v.pages = refs.size(0);
+  TORCH_CHECK(page_table.stride(1) == 1 || v.width <= 1, "page_table must be contiguous along the pages");
+  v.stride = v.rows <= 1 ? v.width : page_table.stride(0);
+  TORCH_CHECK(v.stride >= v.width, "page_table rows must not overlap");
+  return v;
+}
+
+int32_t* check_lens(const torch::Tensor& seq_lens, const TableView& v, const torch::Tensor& like) {
+  LB_CHECK_DEV(seq_lens); LB_CHECK_CONTIG(seq_lens); LB_CHECK_I32(seq_lens);
+  TORCH_CHECK(seq_lens.device() == like.device(), "seq_lens must be on the same device as the other tensors");
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == v.rows, "seq_lens must be [rows] of page_table");
+  return seq_lens.data_ptr<int32_t>();
+}
+
+// int32 [n] of a call's rows (n < 0: any number); null where it is not given.
+int32_t* check_list(const c10::optional<torch::Tensor>& list, const char* name, int64_t n, const torch::Tensor& like) {
+  if (!list.has_value()) return nullptr;
+  const torch::Tensor& t = *list;
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on the same device as the other tensors");
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous(), name, " must be contiguous int32 [rows of the call]");
+  TORCH_CHECK(n < 0 || t.size(0) == n, name, " must have ", n, " entries");
+  return t.data_ptr<int32_t>();
+}
+
+void check_count(int64_t n) { TORCH_CHECK(n <= kMaxPageRows, "at most ", kMaxPageRows, " rows in a call, got ", n); }
+
+void kv8_pages_free_out(torch::Tensor page_table, torch::Tensor seq_lens, torch::Tensor refs, int64_t page_size,
+                        torch::Tensor rows, c10::optional<torch::Tensor> keep) {
+  const TableView v = check_pages(page_table, refs);
+  int32_t* lens = check_lens(seq_lens, v, refs);
+  const int32_t* which = check_list(rows, "rows", -1, refs);
+  const int32_t* kept = check_list(keep, "keep", rows.size(0), refs);
+  check_count(rows.size(0));
+  const c10::DeviceGuard guard(refs.device());
+  lb_ok(lb_kv8_pages_free(v.table, v.rows, v.width, v.stride, lens, v.refs, v.pages, page_size, which, kept,
+                          rows.size(0), stream_of(refs)),
+        "kv8_pages_free_out");
+}
+
+void kv8_pages_fork_out(torch::Tensor page_table, torch::Tensor seq_lens, torch::Tensor refs, int64_t page_size,
+                        torch::Tensor parents, torch::Tensor children, c10::optional<torch::Tensor> lens,
+                        c10::optional<torch::Tensor> done) {
+  const TableView v = check_pages(page_table, refs);
+  int32_t* own = check_lens(seq_lens, v, refs);
+  const int32_t* from = check_list(parents, "parents", -1, refs);
+  const int64_t n = parents.size(0);
+  const int32_t* to = check_list(children, "children", n, refs);
+  const int32_t* most = check_list(lens, "lens", n, refs);
+  int32_t* said = check_list(done, "done", n, refs);
+  check_count(n);
+  const c10::DeviceGuard guard(refs.device());
+  lb_ok(lb_kv8_pages_fork(v.table, v.rows, v.width, v.stride, own, v.refs, v.pages, page_size, from, to, most, said, n,
+                          stream_of(refs)),
+        "kv8_pages_fork_out");
+}
+
+void kv8_pages_extend_out(torch::Tensor page_table, torch::Tensor seq_lens, torch::Tensor refs, int64_t page_size,
+                          torch::Tensor rows, torch::Tensor add, torch::Tensor status, const KV8Layers* layers) {
+  const TableView v = check_pages(page_table, refs);
+  int32_t* lens = check_lens(seq_lens, v, refs);
+  const int32_t* which = check_list(rows, "rows", -1, refs);
+  const int32_t* more = check_list(add, "add", rows.size(0), refs);
+  int32_t* said = check_list(status, "status", 1, refs);
+  check_count(rows.size(0));
+  TORCH_CHECK(!layers || layers->held[0].device() == refs.device(), "the layers must be on the same device as the other tensors");
+  TORCH_CHECK(!layers || (layers->pages == v.pages && layers->page_size == page_size),
+              "the layers' caches must have the pages that refs counts");
+  const c10::DeviceGuard guard(refs.device());
+  auto scratch = op_scratch(lb_kv8_pages_extend_scratch_bytes(v.pages), refs);
+  lb_ok(lb_kv8_pages_extend(v.table, v.rows, v.width, v.stride, lens, v.refs, v.pages, page_size, which, more,
+                            rows.size(0), said, layers ? layers->at.data() : nullptr, layers ? layers->at.size() : 0,
+                            layers ? layers->heads : 0, layers ? layers->head_dim : 0, scratch.ptr, scratch.bytes,
+                            stream_of(refs)),
+        "kv8_pages_extend_out");
+}
+
+void kv8_pages_compact_out(torch::Tensor page_table, torch::Tensor refs, torch::Tensor used, const KV8Layers* layers) {
+  const TableView v = check_pages(page_table, refs);
+  int32_t* said = check_list(used, "used", 1, refs);
+  TORCH_CHECK(!layers || layers->held[0].device() == refs.device(), "the layers must be on the same device as the other tensors");
+  TORCH_CHECK(!layers || layers->pages == v.pages, "the layers' caches must have the pages that refs counts");
+  const c10::DeviceGuard guard(refs.device());
+  auto scratch = op_scratch(lb_kv8_pages_compact_scratch_bytes(v.pages), refs);
+  lb_ok(lb_kv8_pages_compact(v.table, v.rows, v.width, v.stride, v.refs, v.pages, said,
+                             layers ? layers->at.data() : nullptr, layers ? layers->at.size() : 0,
+                             layers ? layers->heads : 0, layers ? layers->page_size : 16, layers ? layers->head_dim : 0,
+                             scratch.ptr, scratch.bytes, stream_of(refs)),
+        "kv8_pages_compact_out");
+}
+
+void kv8_copy_pages(const KV8Layers& layers, torch::Tensor src, torch::Tensor dst) {
+  const torch::Tensor& like = layers.held[0];
+  const int32_t* from = check_list(src, "src", -1, like);
+  const int32_t* to = check_list(dst, "dst", src.size(0), like);
+  const c10::DeviceGuard guard(like.device());
+  lb_ok(lb_kv8_copy_pages(layers.at.data(), layers.at.size(), layers.pages, layers.heads, layers.page_size,
+                          layers.head_dim, from, to, src.size(0), stream_of(like)),
+        "kv8_copy_pages");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(langburst_cuda, m) {
@@ -677,6 +836,25 @@ PYBIND11_MODULE(langburst_cuda, m) {
   m.def("prompt_attention_out", &prompt_attention_out,
         "Causal attention inside each of the packed sequences of a batch of prompts", py::arg("q"), py::arg("k"),
         py::arg("v"), py::arg("cu_seqlens"), py::arg("out"), py::arg("softmax_scale"));
+  py::class_<KV8Layers>(m, "KV8Layers", "The layers' 8-bit caches, as the operators on pages take them")
+      .def(py::init<std::vector<torch::Tensor>, std::vector<torch::Tensor>, std::vector<torch::Tensor>,
+                    std::vector<torch::Tensor>>(),
+           py::arg("k_caches"), py::arg("v_caches"), py::arg("k_scales"), py::arg("v_scales"))
+      .def("__len__", [](const KV8Layers& l) { return l.at.size(); });
+  m.def("kv8_pages_free_out", &kv8_pages_free_out, "Rows keep their first tokens and give up the pages behind them",
+        py::arg("page_table"), py::arg("seq_lens"), py::arg("refs"), py::arg("page_size"), py::arg("rows"),
+        py::arg("keep") = py::none());
+  m.def("kv8_pages_fork_out", &kv8_pages_fork_out, "Empty rows get the first tokens of others, by holding their pages too",
+        py::arg("page_table"), py::arg("seq_lens"), py::arg("refs"), py::arg("page_size"), py::arg("parents"),
+        py::arg("children"), py::arg("lens") = py::none(), py::arg("done") = py::none());
+  m.def("kv8_pages_extend_out", &kv8_pages_extend_out,
+        "Pages for new tokens of rows; a shared page that is not full is copied first", py::arg("page_table"),
+        py::arg("seq_lens"), py::arg("refs"), py::arg("page_size"), py::arg("rows"), py::arg("add"), py::arg("status"),
+        py::arg("layers") = py::none());
+  m.def("kv8_pages_compact_out", &kv8_pages_compact_out, "Moves the pages in use to the front of the pool",
+        py::arg("page_table"), py::arg("refs"), py::arg("used"), py::arg("layers") = py::none());
+  m.def("kv8_copy_pages", &kv8_copy_pages, "Copies pages in every layer", py::arg("layers"), py::arg("src"),
+        py::arg("dst"));
   m.def("abi_version", []() { return lb_abi_version(); });
   m.attr("__provides__") = py::make_tuple("lowbit_gemv", "lowbit_row_dequant", "lowbit_gemv_pair", "lowbit_gemm",
                                           "lowbit_marlin_gemm", "lowbit_marlin_gemm_out",

@@ -13,6 +13,8 @@
 // key/value head.  Four waves of 32 rows go through tiles of 64 keys together: the
 // codes of a tile come into registers while the tile before is computed, become fp16
 // (exactly) and lie in LDS for all four.
+#include <type_traits>
+
 #include "attn_common.hpp"
 
 namespace lb {
@@ -38,10 +40,10 @@ constexpr int kRows = 128, kKeys = 64, kWaves = 4;
 constexpr float kNoMax = -1e30f;
 // The running maximum is that of weight times value scale.  It moves only when
 // exceeded by 2^kSlack, and the weights carry 2^kLift more: at most 2^15, inside
-// fp16, and 2^7 farther from its subnormals.  Value scales count from 2^-kScales to
-// 2^kScales; where all of a tile's are within 2^kNear of one, the scale is part of
-// the exponent, and a weight without it the exponential divided by it.
-constexpr float kSlack = 8.0f, kLift = 7.0f, kScales = 80.0f, kNear = 32.0f;
+// fp16, and 2^7 farther from its subnormals.  A value scale is part of its weights'
+// exponent, between 2^-kScales and 2^kScales (fp16 values give 2^-31 to 2^9), so that
+// no weight that counts in the sum falls below fp32's normal numbers.
+constexpr float kSlack = 8.0f, kLift = 7.0f, kScales = 32.0f;
 // A piece of a row block's keys is this many tiles at least.
 constexpr int kMinTiles = 4;
 
@@ -154,31 +156,38 @@ __device__ __forceinline__ int k_swizzle(int row) {
   return D == 64 ? (row >> 1) & 7 : row & 15;
 }
 
-// The pages of a tile, lane l those of its 16 tokens l % 4, and the next tile's codes.
+// The tiles of a piece on their way: pages two tiles ahead of the codes that become
+// fp16, codes one.  Lane l knows the page of the 16 tokens l % 4 of a tile.
 template <int D>
 struct Tiles {
-  static constexpr int N = D / 64;  // loads of keys (and of values) of a thread
+  static constexpr int N = D / 64;  // loads of keys (and of values) of a thread and tile
   const ChunkArgs& a;
   const int32_t* table;
   int head, len, lane, wave;
-  int groups_shift;  // log2 of the groups of 16 tokens that a page's row holds, of a tile's four
-  uint32_t k_off[N], v_off[N];
-  int page;       // of the tile after the one whose codes are loaded
+  int groups;      // log2 of the groups of 16 tokens, of a tile's four, that lie side by side in a page
+  int per, in;     // channels of a load of values, loads of all channels
+  uint32_t k_off, v_off;   // the thread's place in a load
+  int k_lds, v_lds[N];     // and in LDS
+  int page;        // of the tile after the ones whose codes are loaded
   bool held;
-  float ks, vs;   // of the tile whose codes are loaded
-  bool held_codes;
-  u32x4 kc[N], vc[N];
+  // of the tile whose codes are loaded last, and of the one before
+  float ks[2], vs[2];
+  uint32_t held_codes[2];  // bit g: of its 16 tokens g some are held
+  u32x4 codes[2 * N];
 
-  __device__ __forceinline__ Tiles(const ChunkArgs& args, const Piece& p, int kv_head, int w) : a(args), head(kv_head), len(p.s.len), lane(lane_id()), wave(w) {
+  __device__ __forceinline__ Tiles(const ChunkArgs& args, const Piece& p, int kv_head, int w)
+      : a(args), head(kv_head), len(p.s.len), lane(lane_id()), wave(w) {
     table = a.page_table + (int64_t)p.b * a.table_stride;
-    groups_shift = min(a.page_shift - 4, 2);
-    const int per = kWave >> groups_shift;  // channels of a load
+    groups = min(a.page_shift - 4, 2), per = kWave >> groups, in = D / per;
+    const int row = (wave * kWave + lane) / (D / 16), col = 2 * (lane % (D / 16));
+    k_off = (row & 15) * D + col * 8;
+    k_lds = row * D + 8 * (col ^ k_swizzle<D>(row));
+    v_off = (((wave % in) * per + (lane >> groups)) << a.page_shift) + (lane & ((1 << groups) - 1)) * 16;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int x = (i * kWaves + wave) * kWave + lane;
-      k_off[i] = ((x / (D / 16)) & 15) * D + (x % (D / 16)) * 16;
-      const int y = i * kWaves + wave, in = D / per;
-      v_off[i] = (((y % in) * per + (lane >> groups_shift)) << a.page_shift) + (lane & ((1 << groups_shift) - 1)) * 16;
+      const int y = i * kWaves + wave, g = (y / in << groups) + (lane & ((1 << groups) - 1));
+      const int ch = (y % in) * per + (lane >> groups);
+      v_lds[i] = ch * kKeys + 8 * ((2 * g) ^ (ch & 7));
     }
   }
   __device__ __forceinline__ void load_page(int tile) {
@@ -186,62 +195,68 @@ struct Tiles {
     page = table[min(t, len - 1) >> a.page_shift];
     held = t < len;
   }
-  // Codes and scales of `tile`, whose pages are known.
-  __device__ __forceinline__ void load_codes(int tile) {
+  // Scales of a tile whose pages are known, and where its codes are; none of `!real`.
+  int cell;
+  __device__ __forceinline__ void begin(int set) {
+    const bool real = held && (unsigned)page < (unsigned)a.num_pages;
+    held_codes[set] = (uint32_t)__ballot(real) & 15;
+    cell = (real ? page : 0) * a.heads_kv + head;
+    ks[set] = a.k_scale[cell], vs[set] = a.v_scale[cell];
+  }
+  // Load j of the tile: of its keys, then of its values.
+  __device__ __forceinline__ void load(int j, int tile, bool real) {
     const int mask = (1 << a.page_shift) - 1;
-    held_codes = held && (unsigned)page < (unsigned)a.num_pages;
-    const int safe = held_codes ? page : 0;
-    const int cell = safe * a.heads_kv + head;
-    ks = a.k_scale[cell], vs = a.v_scale[cell];
-    const int in = D / (kWave >> groups_shift);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int g = (i * kWaves + wave) * (kWave * 16 / D) / 16;  // the load's 16 tokens
+    const uint32_t bytes = real ? (uint32_t)D << a.page_shift : 0u;
+    if (j < N) {
+      const int g = (j * kWaves + wave) * (kWave * 16 / D) / 16;  // the load's 16 tokens
       const int64_t c = __builtin_amdgcn_readlane(cell, g);
-      const int8_t* from = a.k_cache + ((c << a.page_shift) + ((tile * kKeys + 16 * g) & mask)) * D;
-      kc[i] = *reinterpret_cast<const u32x4*>(from + k_off[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int g = (i * kWaves + wave) / in << groups_shift;
+      const uint32_t at = (uint32_t)((tile * kKeys + 16 * g) & mask) * D;
+      codes[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer_of(a.k_cache + (c << a.page_shift) * D, bytes), k_off, at, 0));
+    } else {
+      const int y = (j - N) * kWaves + wave, g = y / in << groups;
       const int64_t c = __builtin_amdgcn_readlane(cell, g);
-      const int8_t* from = a.v_cache + ((c * D) << a.page_shift) + ((tile * kKeys + 16 * g) & mask);
-      vc[i] = *reinterpret_cast<const u32x4*>(from + v_off[i]);
+      const uint32_t at = ((uint32_t)(((j - N) * kWaves % in) * per) << a.page_shift) + ((tile * kKeys + 16 * g) & mask);
+      codes[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer_of(a.v_cache + ((c * D) << a.page_shift), bytes), v_off, at, 0));
     }
   }
   // As fp16 into LDS: keys [token][channel], values [channel][token], the tokens of a
   // group in the order of the second product's operand (of 4 h .. 4 h + 3 and 8 more
   // the half h); chunks of 16 bytes change places so that reads use every bank.
-  __device__ __forceinline__ void store(uint16_t* kl, uint16_t* vl) const {
-    const int in = D / (kWave >> groups_shift);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      f16x8 x, y;
-      codes_to_half(kc[i], x, y);
-      const int c = (i * kWaves + wave) * kWave + lane, row = c / (D / 16), col = 2 * (c % (D / 16)), swz = k_swizzle<D>(row);
-      *reinterpret_cast<f16x8*>(kl + row * D + 8 * (col ^ swz)) = x;
-      *reinterpret_cast<f16x8*>(kl + row * D + 8 * ((col + 1) ^ swz)) = y;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      f16x8 x, y;
-      codes_to_half((u32x4){vc[i][0], vc[i][2], vc[i][1], vc[i][3]}, x, y);
-      const int w = i * kWaves + wave;
-      const int g = ((w / in) << groups_shift) + (lane & ((1 << groups_shift) - 1));
-      const int ch = (w % in) * (kWave >> groups_shift) + (lane >> groups_shift);
-      *reinterpret_cast<f16x8*>(vl + ch * kKeys + 8 * ((2 * g) ^ (ch & 7))) = x;
-      *reinterpret_cast<f16x8*>(vl + ch * kKeys + 8 * ((2 * g + 1) ^ (ch & 7))) = y;
+  __device__ __forceinline__ void store(int j, uint16_t* kl, uint16_t* vl) const {
+    f16x8 x, y;
+    if (j < N) {
+      codes_to_half(codes[j], x, y);
+      constexpr int kRowStep = kWaves * kWave / (D / 16);
+      static_assert(N == 1 || kRowStep % 16 == 0, "rows of a thread's loads change places alike");
+      uint16_t* to = kl + k_lds + j * kRowStep * D;
+      *reinterpret_cast<f16x8*>(to) = x;
+      *reinterpret_cast<f16x8*>(kl + (k_lds ^ 8) + j * kRowStep * D) = y;
+    } else {
+      const u32x4 w = codes[j];
+      codes_to_half((u32x4){w[0], w[2], w[1], w[3]}, x, y);
+      *reinterpret_cast<f16x8*>(vl + v_lds[j - N]) = x;
+      *reinterpret_cast<f16x8*>(vl + (v_lds[j - N] ^ 8)) = y;
     }
   }
 };
 
-// What the scores of a tile's four groups of 16 tokens are multiplied with, and their
-// values' scales.
+// What the scores of a tile's four groups of 16 tokens are multiplied with, their
+// values' scales as exponents, and the inverse of these.
 struct Scales {
-  float k[4], log[4], inverse[4], v[4];
+  float k[4], log[4], inverse[4];
   uint32_t held;  // bit g
-  bool plain;     // nothing special about any of them
+  bool usual;     // both scales of all four finite, above zero and inside the range
 };
+
+// At 256 channels the output fills half of a wave's accumulation registers, which only
+// the matrix products reach; without these marks the compiler copies all of it into
+// vector registers in every tile, for the rare tile that scales it.
+template <int D, int N>
+__device__ __forceinline__ void stay_in_accumulators(f32x16 (&o)[N]) {
+  if constexpr (D == 256)
+#pragma unroll
+    for (int d = 0; d < N; ++d) asm volatile("" : "+a"(o[d]));
+}
 
 template <int D>
 __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(ChunkArgs a) {
@@ -260,10 +275,9 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
   const int rows = p.s.n * a.group, wave_row = p.block * kRows + wave * 32;
   const int row = wave_row + r, token = row / a.group, q_head = kvh * a.group + row - token * a.group;
   const bool real = row < rows;
-  // the wave's rows see the keys up to `seen`, all of them those up to `all_see`
+  // the lane's row sees the keys up to `seen`, all of the wave's those up to `all_see`
   const int seen = real ? min(p.s.at + token, p.s.len - 1) : -1;
   const int all_see = min(p.s.at + wave_row / a.group, p.s.len - 1);
-  const int any_see = wave_row < rows ? min(p.s.at + min(rows - 1, wave_row + 31) / a.group, p.s.len - 1) : -1;
 
   f16x8 qf[KK];
   {
@@ -279,124 +293,175 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = (f32x16)(0.0f);
 
-  Tiles<D> tiles(a, p, kvh, wave);
+  typedef Tiles<D> T;
+  T tiles(a, p, kvh, wave);
   if (p.t0 < p.t1) {
     tiles.load_page(p.t0);
-    tiles.load_codes(p.t0);
+    tiles.begin(0);
+#pragma unroll
+    for (int j = 0; j < 2 * T::N; ++j) tiles.load(j, p.t0, true);
     tiles.load_page(p.t0 + 1);
-    tiles.store(k0, v0);
+#pragma unroll
+    for (int j = 0; j < 2 * T::N; ++j) tiles.store(j, k0, v0);
+    tiles.begin(1);
+#pragma unroll
+    for (int j = 0; j < 2 * T::N; ++j) tiles.load(j, p.t0 + 1, p.t0 + 1 < p.t1);
+    tiles.load_page(p.t0 + 2);
   }
 
-  // Tile kt from (kl, vl); the next tile's codes go to (kn, vn).
   Scales sc;
-  auto scales = [&]() {
-    const float k = tiles.held_codes ? tiles.ks * a.scale + (tiles.ks - tiles.ks) : 0.0f;
-    const float lg = __builtin_fmaxf(__builtin_fminf(__builtin_amdgcn_logf(__builtin_fabsf(tiles.vs)), kScales), -kScales);
+  float fix;  // lane g: what is left of a value scale outside its exponent's range
+  auto scales = [&](int set) {
+    sc.held = tiles.held_codes[set];
+    const bool held = sc.held >> (lane & 3) & 1;
+    const float ks = tiles.ks[set], vs = held ? tiles.vs[set] : 1.0f;
+    const float k = held ? ks * a.scale + (ks - ks) : 1.0f;
+    const float lg = __builtin_fmaxf(__builtin_fminf(__builtin_amdgcn_logf(__builtin_fabsf(vs)), kScales), -kScales);
     const float inv = __builtin_amdgcn_exp2f(-lg - kLift);
-    const bool plain = tiles.held_codes && k > 0.0f && k < __builtin_inff() && tiles.vs > 0.0f && __builtin_fabsf(lg) <= kNear;
-    sc.held = (uint32_t)__ballot(tiles.held_codes) & 15;
-    sc.plain = ((uint32_t)__ballot(plain) & 15) == 15;
+    fix = vs * __builtin_amdgcn_exp2f(-lg);
+    const bool usual = k > 0.0f && k < __builtin_inff() && vs > 0.0f && __builtin_fabsf(lg) < kScales;
+    sc.usual = ((uint32_t)__ballot(usual) & 15) == 15;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       auto at = [&](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), g)); };
-      sc.k[g] = at(k), sc.log[g] = at(lg), sc.inverse[g] = at(inv), sc.v[g] = at(tiles.vs);
+      sc.k[g] = at(k), sc.log[g] = at(lg), sc.inverse[g] = at(inv);
     }
   };
-  auto take = [&](int kt, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
-    scales();
+  // Tile kt from (kl, vl).  Between the products of the scores the next tile's codes
+  // become fp16 in (kn, vn), and the loads of the one after take their registers.
+  auto take = [&](int kt, auto parity, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
+    constexpr int set = decltype(parity)::value;
+    scales(set);
     lds_barrier();
-    if (kt + 1 < p.t1) {
-      tiles.load_codes(kt + 1);
-      tiles.load_page(kt + 2);
-    }
-    if (kt * kKeys <= any_see) {
-      f32x16 s[ST];
+    const bool more = kt + 2 < p.t1;
+    tiles.begin(set);
+    tiles.load_page(kt + 3);
+    auto feed = [&](int j) {
+      tiles.store(j, kn, vn);
+      tiles.load(j, kt + 2, more);
+    };
+    // the lane's places in the rows; out of the compiler's sight, or it keeps one register
+    // for each of their uses
+    int from_k = r * D + 8 * (h ^ k_swizzle<D>(r)), from_v = r * kKeys + 8 * (h ^ (r & 7));
+    asm volatile("" : "+v"(from_k), "+v"(from_v));
+    f32x16 s[ST];
 #pragma unroll
-      for (int t = 0; t < ST; ++t) s[t] = (f32x16)(0.0f);
+    for (int t = 0; t < ST; ++t) s[t] = (f32x16)(0.0f);
+    constexpr int CH = KK / 4;  // channel steps of a quarter
+    f16x8 kf[2][CH][ST];
+    auto read_k = [&](int q) {
 #pragma unroll
-      for (int k = 0; k < KK; ++k)
+      for (int k = 0; k < CH; ++k)
 #pragma unroll
         for (int t = 0; t < ST; ++t) {
-          const int key = 32 * t + r;
-          const f16x8 kf = *reinterpret_cast<const f16x8*>(kl + key * D + 8 * ((2 * k + h) ^ k_swizzle<D>(key)));
-          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[k], s[t], 0, 0, 0);
+          kf[q & 1][k][t] = *reinterpret_cast<const f16x8*>(kl + 32 * t * D + (from_k ^ 16 * (q * CH + k)));
         }
-      const bool plain = sc.plain && kt * kKeys + kKeys - 1 <= all_see;
-      float peak = kNoMax;
-      if (plain) {
+    };
+    read_k(0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float x = s[g / 2][8 * (g % 2)];
+    for (int q = 0; q < 4; ++q) {
+      if (q < 3) read_k(q + 1);
 #pragma unroll
-          for (int i = 1; i < 8; ++i) x = __builtin_fmaxf(x, s[g / 2][8 * (g % 2) + i]);
-          peak = __builtin_fmaxf(peak, x * sc.k[g] + sc.log[g]);
-        }
-      } else {
-        const int past = seen - kt * kKeys - 4 * h;  // keys of the lane up to here are seen
+      for (int k = 0; k < CH; ++k)
 #pragma unroll
-        for (int t = 0; t < ST; ++t)
+        for (int t = 0; t < ST; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[q & 1][k][t], qf[q * CH + k], s[t], 0, 0, 0);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int g = 2 * t + i / 8;
-            float x = s[t][i] * sc.k[g];
-            if (32 * t + 8 * (i >> 2) + (i & 3) > past || !(sc.held >> g & 1)) x = -__builtin_inff();
-            s[t][i] = x;
-            peak = __builtin_fmaxf(peak, x + sc.log[g]);
-          }
-      }
-      if (__any(peak > m + kSlack)) {
-        // row by row: what other rows of the wave see changes no bit of a row
-        float up = __builtin_fmaxf(peak, from_lane(peak, lane ^ 32));
-        if (!(up > m + kSlack)) up = m;
-        const float f = __builtin_amdgcn_exp2f(m - up);
-        m = up;
-        l *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= f;
-      }
-      f16x8 pf[2 * ST];
-      if (plain) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float lift = sc.log[g] + kLift - m;
-          float sum = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float w = __builtin_amdgcn_exp2f(s[g / 2][8 * (g % 2) + i] * sc.k[g] + lift);
-            sum += w;
-            pf[g][i] = (f16)w;
-          }
-          l += sum * sc.inverse[g];
-        }
-      } else {
-        const int past = seen - kt * kKeys - 4 * h;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float lifted = sc.v[g] * __builtin_exp2f(kLift);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float w = __builtin_amdgcn_exp2f(s[g / 2][8 * (g % 2) + i] - m);
-            l += w;
-            // no weight, and none of a value scale that is not finite either
-            const bool sees = 16 * g + 8 * (i >> 2) + (i & 3) <= past && (sc.held >> g & 1);
-            pf[g][i] = (f16)(sees ? w * lifted : 0.0f);
-          }
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 2 * ST; ++c)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const int ch = 32 * d + r;
-          const f16x8 vf = *reinterpret_cast<const f16x8*>(vl + ch * kKeys + 8 * ((2 * c + h) ^ (ch & 7)));
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[c], o[d], 0, 0, 0);
-        }
+      for (int j = 0; j < 2 * T::N; ++j)
+        if (j * 4 / (2 * T::N) == q) feed(j);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (kt + 1 < p.t1) tiles.store(kn, vn);
+    const int past = seen - kt * kKeys - 4 * h;  // keys of the lane up to here are seen
+    if (__builtin_expect(!sc.usual, 0)) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[g / 2][8 * (g % 2) + i] *= sc.k[g];
+        sc.k[g] = 1.0f;
+      }
+    }
+    if (kt * kKeys + kKeys - 1 > all_see || sc.held != 15) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int last = sc.held >> g & 1 ? past - 16 * g : -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (8 * (i >> 2) + (i & 3) > last) s[g / 2][8 * (g % 2) + i] = -__builtin_inff();
+      }
+    }
+    float peak = kNoMax;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float x = s[g / 2][8 * (g % 2)];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) x = __builtin_fmaxf(x, s[g / 2][8 * (g % 2) + i]);
+      peak = __builtin_fmaxf(peak, x * sc.k[g] + sc.log[g]);
+    }
+    stay_in_accumulators<D>(o);
+    if (__any(peak > m + kSlack)) {
+      // row by row: what other rows of the wave see changes no bit of a row
+      float up = __builtin_fmaxf(peak, from_lane(peak, lane ^ 32));
+      if (!(up > m + kSlack)) up = m;
+      const float f = __builtin_amdgcn_exp2f(m - up);
+      m = up;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+      stay_in_accumulators<D>(o);
+    }
+    f16x8 pf[2 * ST];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float lift = sc.log[g] + kLift - m;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __builtin_amdgcn_exp2f(s[g / 2][8 * (g % 2) + i] * sc.k[g] + lift);
+        sum += w;
+        pf[g][i] = (f16)w;
+      }
+      l += sum * sc.inverse[g];
+    }
+    if (__builtin_expect(!sc.usual, 0)) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f16 x = (f16)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, fix), g));
+        const int last = sc.held >> g & 1 ? past - 16 * g : -1;
+        // a key that is not seen has no weight, and none of a scale that is not finite either
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pf[g][i] = 8 * (i >> 2) + (i & 3) > last ? (f16)0.0f : pf[g][i] * x;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2 * ST; ++c)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const f16x8 vf = *reinterpret_cast<const f16x8*>(vl + 32 * d * kKeys + (from_v ^ 16 * c));
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[c], o[d], 0, 0, 0);
+      }
   };
+  if (wave_row >= rows) {
+    // a wave without rows brings the tiles for the others
+    auto bring = [&](int kt, auto parity, uint16_t* kn, uint16_t* vn) {
+      constexpr int set = decltype(parity)::value;
+      lds_barrier();
+      tiles.begin(set);
+      tiles.load_page(kt + 3);
+#pragma unroll
+      for (int j = 0; j < 2 * T::N; ++j) {
+        tiles.store(j, kn, vn);
+        tiles.load(j, kt + 2, kt + 2 < p.t1);
+      }
+    };
+    for (int kt = p.t0; kt < p.t1; kt += 2) {
+      bring(kt, std::integral_constant<int, 0>(), k1, v1);
+      if (kt + 1 < p.t1) bring(kt + 1, std::integral_constant<int, 1>(), k0, v0);
+    }
+  } else
   for (int kt = p.t0; kt < p.t1; kt += 2) {
-    take(kt, k0, v0, k1, v1);
-    if (kt + 1 < p.t1) take(kt + 1, k1, v1, k0, v0);
+    take(kt, std::integral_constant<int, 0>(), k0, v0, k1, v1);
+    if (kt + 1 < p.t1) take(kt + 1, std::integral_constant<int, 1>(), k1, v1, k0, v0);
+    stay_in_accumulators<D>(o);
   }
 
   l += from_lane(l, lane ^ 32);
@@ -419,7 +484,10 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
   lds_barrier();
   uint16_t* mine = wave < 2 ? (wave == 0 ? k0 : k1) : (wave == 2 ? v0 : v1);
   const float inv = l > 0.0f ? __builtin_exp2f(-kLift) / l : l == 0.0f ? 0.0f : l;
-  const int64_t place = (int64_t)(p.s.first + token) * a.o_token + (int64_t)q_head * a.o_head;
+  int again = wave_row + r;  // the row's place once more: kept over the loop it would take registers
+  asm volatile("" : "+v"(again));
+  const int to_token = again / a.group, to_head = kvh * a.group + again - to_token * a.group;
+  const int64_t place = (int64_t)(p.s.first + to_token) * a.o_token + (int64_t)to_head * a.o_head;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll

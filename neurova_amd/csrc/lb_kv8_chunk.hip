@@ -13,8 +13,6 @@
 // key/value head.  Four waves of 32 rows go through tiles of 64 keys together: the
 // codes of a tile come into registers while the tile before is computed, become fp16
 // (exactly) and lie in LDS for all four.
-#include <type_traits>
-
 #include "attn_common.hpp"
 
 namespace lb {
@@ -43,12 +41,12 @@ constexpr float kNoMax = -1e30f;
 // fp16, and 2^7 farther from its subnormals.  A value scale is part of its weights'
 // exponent, between 2^-kScales and 2^kScales (fp16 values give 2^-31 to 2^9), so that
 // no weight that counts in the sum falls below fp32's normal numbers.
-constexpr float kSlack = 8.0f, kLift = 7.0f, kScales = 32.0f;
+constexpr float kSlack = 8.0f, kLift = 7.0f, kScales = 32.0f, kMost = 32768.0f;  // 2^(kSlack + kLift)
 // A piece of a row block's keys is this many tiles at least.
 constexpr int kMinTiles = 4;
 
 template <int D>
-constexpr int kPerSimd = D == 64 ? 3 : D == 128 ? 2 : 1;
+constexpr int kPerSimd = D == 256 ? 1 : 2;
 
 // ------------------------------------------------------------- the work ---
 
@@ -151,32 +149,40 @@ constexpr int kPartFloats = kRows * (D + 2);
 
 // ------------------------------------------------------------- a tile ---
 
+// The 16-byte chunks of a key's row change places so that reads use every bank: of the
+// keys 0 to 3 and 16 to 19 and so on, which the lanes of a product's operand read.
 template <int D>
-__device__ __forceinline__ int k_swizzle(int row) {
-  return D == 64 ? (row >> 1) & 7 : row & 15;
+__device__ __forceinline__ int k_swizzle(int key) {
+  const int b2 = key >> 2 & 1, b4 = key >> 4 & 1;
+  return D == 64 ? (key >> 1 & 1) | b4 << 1 | b2 << 2 : (key & 3) | b4 << 2 | b2 << 3;
 }
 
-// The tiles of a piece on their way: pages two tiles ahead of the codes that become
-// fp16, codes one.  Lane l knows the page of the 16 tokens l % 4 of a tile.
+// Sixteen tiles' pages and scales are looked up together, lane l those of the 16 tokens
+// l % 4 of tile l / 4, and what the products need of them lies in LDS for all waves: the
+// factor of the scores, the value scale as an exponent, the inverse of that (2^-kLift
+// times), and what is left of a value scale outside the exponent's range.
+constexpr int kBatch = 16;
+typedef f32x4 Info[2][kBatch * 4];
+
+// The tiles of a piece on their way: pages and scales a batch ahead, codes a tile ahead.
 template <int D>
 struct Tiles {
   static constexpr int N = D / 64;  // loads of keys (and of values) of a thread and tile
   const ChunkArgs& a;
+  Info& info;
   const int32_t* table;
-  int head, len, lane, wave;
-  int groups;      // log2 of the groups of 16 tokens, of a tile's four, that lie side by side in a page
-  int per, in;     // channels of a load of values, loads of all channels
-  uint32_t k_off, v_off;   // the thread's place in a load
-  int k_lds, v_lds[N];     // and in LDS
-  int page;        // of the tile after the ones whose codes are loaded
-  bool held;
-  // of the tile whose codes are loaded last, and of the one before
-  float ks[2], vs[2];
-  uint32_t held_codes[2];  // bit g: of its 16 tokens g some are held
+  int head, len, first, lane, wave;
+  int groups;     // log2 of the groups of 16 tokens, of a tile's four, that lie side by side in a page
+  int per, in;    // channels of a load of values, loads of all channels
+  uint32_t k_off, v_off;  // the thread's place in a load
+  int k_lds, v_lds[N];    // and in LDS
+  int cell, next_cell, page;  // page and head: of the batch whose codes are loaded, of the next; page of the one after
+  float ks, vs;               // scales of the next batch
+  uint64_t held, usual, next_held, next_usual;  // bit l: page there; scales finite, above zero, inside the range
   u32x4 codes[2 * N];
 
-  __device__ __forceinline__ Tiles(const ChunkArgs& args, const Piece& p, int kv_head, int w)
-      : a(args), head(kv_head), len(p.s.len), lane(lane_id()), wave(w) {
+  __device__ __forceinline__ Tiles(const ChunkArgs& args, Info& shared, const Piece& p, int kv_head, int w)
+      : a(args), info(shared), head(kv_head), len(p.s.len), first(p.t0), lane(lane_id()), wave(w) {
     table = a.page_table + (int64_t)p.b * a.table_stride;
     groups = min(a.page_shift - 4, 2), per = kWave >> groups, in = D / per;
     const int row = (wave * kWave + lane) / (D / 16), col = 2 * (lane % (D / 16));
@@ -190,62 +196,65 @@ struct Tiles {
       v_lds[i] = ch * kKeys + 8 * ((2 * g) ^ (ch & 7));
     }
   }
-  __device__ __forceinline__ void load_page(int tile) {
-    const int t = tile * kKeys + 16 * (lane & 3);
-    page = table[min(t, len - 1) >> a.page_shift];
-    held = t < len;
+  __device__ __forceinline__ int token(int batch) const { return (first + batch * kBatch) * kKeys + 16 * lane; }
+  __device__ __forceinline__ void load_pages(int batch) { page = table[min(token(batch), len - 1) >> a.page_shift]; }
+  __device__ __forceinline__ void load_scales(int batch) {
+    const bool real = token(batch) < len && (unsigned)page < (unsigned)a.num_pages;
+    next_held = __ballot(real);
+    next_cell = (real ? page : 0) * a.heads_kv + head;
+    ks = a.k_scale[next_cell], vs = a.v_scale[next_cell];
   }
-  // Scales of a tile whose pages are known, and where its codes are; none of `!real`.
-  int cell;
-  __device__ __forceinline__ void begin(int set) {
-    const bool real = held && (unsigned)page < (unsigned)a.num_pages;
-    held_codes[set] = (uint32_t)__ballot(real) & 15;
-    cell = (real ? page : 0) * a.heads_kv + head;
-    ks[set] = a.k_scale[cell], vs[set] = a.v_scale[cell];
+  __device__ __forceinline__ void tell(int batch) {
+    const bool real = next_held >> lane & 1;
+    const float v = real ? vs : 1.0f;
+    // a scale of infinity has no scores: ks - ks makes it NaN and is zero otherwise
+    const float k = real ? ks * a.scale + (ks - ks) : 1.0f;
+    const float lg = __builtin_fmaxf(__builtin_fminf(__builtin_amdgcn_logf(__builtin_fabsf(v)), kScales), -kScales);
+    next_usual = __ballot(k > 0.0f && k < __builtin_inff() && v > 0.0f && __builtin_fabsf(lg) < kScales);
+    if (lane / kBatch == wave) info[batch & 1][lane] = (f32x4){k, lg, __builtin_amdgcn_exp2f(-lg - kLift), v * __builtin_amdgcn_exp2f(-lg)};
   }
-  // Load j of the tile: of its keys, then of its values.
-  __device__ __forceinline__ void load(int j, int tile, bool real) {
-    const int mask = (1 << a.page_shift) - 1;
+  __device__ __forceinline__ void turn() { held = next_held, usual = next_usual; }
+  // Tile i of the piece is about to be computed, the loads of tile i + 2 to be sent off
+  // (i even).  A batch's places are written at least a barrier after their last readers.
+  __device__ __forceinline__ void step(int i) {
+    const int c = i % kBatch, batch = i / kBatch;
+    if (c == 0 && i > 0) turn();
+    else if (c == 2) load_scales(batch + 1);
+    else if (c == 8) tell(batch + 1);
+    else if (c == 10) load_pages(batch + 2);
+    else if (c == kBatch - 2) cell = next_cell;
+  }
+  // Load j of tile i: of its keys, then of its values; none of one that is not `real`.
+  __device__ __forceinline__ void load(int j, int i, bool real) {
+    const int mask = (1 << a.page_shift) - 1, at_lane = i % kBatch * 4, token = (first + i) * kKeys;
     const uint32_t bytes = real ? (uint32_t)D << a.page_shift : 0u;
     if (j < N) {
       const int g = (j * kWaves + wave) * (kWave * 16 / D) / 16;  // the load's 16 tokens
-      const int64_t c = __builtin_amdgcn_readlane(cell, g);
-      const uint32_t at = (uint32_t)((tile * kKeys + 16 * g) & mask) * D;
+      const int64_t c = __builtin_amdgcn_readlane(cell, at_lane + g);
+      const uint32_t at = (uint32_t)((token + 16 * g) & mask) * D;
       codes[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer_of(a.k_cache + (c << a.page_shift) * D, bytes), k_off, at, 0));
     } else {
       const int y = (j - N) * kWaves + wave, g = y / in << groups;
-      const int64_t c = __builtin_amdgcn_readlane(cell, g);
-      const uint32_t at = ((uint32_t)(((j - N) * kWaves % in) * per) << a.page_shift) + ((tile * kKeys + 16 * g) & mask);
+      const int64_t c = __builtin_amdgcn_readlane(cell, at_lane + g);
+      const uint32_t at = ((uint32_t)(((j - N) * kWaves % in) * per) << a.page_shift) + ((token + 16 * g) & mask);
       codes[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer_of(a.v_cache + ((c * D) << a.page_shift), bytes), v_off, at, 0));
     }
   }
-  // As fp16 into LDS: keys [token][channel], values [channel][token], the tokens of a
-  // group in the order of the second product's operand (of 4 h .. 4 h + 3 and 8 more
-  // the half h); chunks of 16 bytes change places so that reads use every bank.
+  // As fp16 into LDS: keys [token][channel], values [channel][token].
   __device__ __forceinline__ void store(int j, uint16_t* kl, uint16_t* vl) const {
     f16x8 x, y;
+    codes_to_half(codes[j], x, y);
     if (j < N) {
-      codes_to_half(codes[j], x, y);
       constexpr int kRowStep = kWaves * kWave / (D / 16);
-      static_assert(N == 1 || kRowStep % 16 == 0, "rows of a thread's loads change places alike");
-      uint16_t* to = kl + k_lds + j * kRowStep * D;
-      *reinterpret_cast<f16x8*>(to) = x;
-      *reinterpret_cast<f16x8*>(kl + (k_lds ^ 8) + j * kRowStep * D) = y;
+      static_assert(N == 1 || kRowStep == 32 || kRowStep == 16, "the rows of a thread's loads change places alike, or as 16 says");
+      const int at = k_lds ^ (kRowStep == 16 && (j & 1) ? 8 << 2 : 0);
+      *reinterpret_cast<f16x8*>(kl + at + j * kRowStep * D) = x;
+      *reinterpret_cast<f16x8*>(kl + (at ^ 8) + j * kRowStep * D) = y;
     } else {
-      const u32x4 w = codes[j];
-      codes_to_half((u32x4){w[0], w[2], w[1], w[3]}, x, y);
       *reinterpret_cast<f16x8*>(vl + v_lds[j - N]) = x;
       *reinterpret_cast<f16x8*>(vl + (v_lds[j - N] ^ 8)) = y;
     }
   }
-};
-
-// What the scores of a tile's four groups of 16 tokens are multiplied with, their
-// values' scales as exponents, and the inverse of these.
-struct Scales {
-  float k[4], log[4], inverse[4];
-  uint32_t held;  // bit g
-  bool usual;     // both scales of all four finite, above zero and inside the range
 };
 
 // At 256 channels the output fills half of a wave's accumulation registers, which only
@@ -261,8 +270,10 @@ __device__ __forceinline__ void stay_in_accumulators(f32x16 (&o)[N]) {
 template <int D>
 __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(ChunkArgs a) {
   constexpr int DT = D / 32, KK = D / 16, ST = kKeys / 32;
+  constexpr int VN = DT < 4 ? DT : 4;  // fragments of values read ahead
   // four arrays and not one: reads of a tile then need not wait for writes of the next
   __shared__ __align__(16) uint16_t k0[kKeys * D], k1[kKeys * D], v0[kKeys * D], v1[kKeys * D];
+  __shared__ Info info;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 31, h = lane >> 5;
   const int kvh = blockIdx.x % a.heads_kv, item = blockIdx.x / a.heads_kv;
@@ -294,55 +305,40 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
   for (int d = 0; d < DT; ++d) o[d] = (f32x16)(0.0f);
 
   typedef Tiles<D> T;
-  T tiles(a, p, kvh, wave);
-  if (p.t0 < p.t1) {
-    tiles.load_page(p.t0);
-    tiles.begin(0);
+  T tiles(a, info, p, kvh, wave);
+  const int count = p.t1 - p.t0;
+  if (count > 0) {
+    tiles.load_pages(0);
+    tiles.load_scales(0);
+    tiles.cell = tiles.next_cell;
+    tiles.load_pages(1);
 #pragma unroll
-    for (int j = 0; j < 2 * T::N; ++j) tiles.load(j, p.t0, true);
-    tiles.load_page(p.t0 + 1);
+    for (int j = 0; j < 2 * T::N; ++j) tiles.load(j, 0, true);
+    tiles.tell(0);
+    tiles.turn();
 #pragma unroll
     for (int j = 0; j < 2 * T::N; ++j) tiles.store(j, k0, v0);
-    tiles.begin(1);
 #pragma unroll
-    for (int j = 0; j < 2 * T::N; ++j) tiles.load(j, p.t0 + 1, p.t0 + 1 < p.t1);
-    tiles.load_page(p.t0 + 2);
+    for (int j = 0; j < 2 * T::N; ++j) tiles.load(j, 1, 1 < count);
   }
 
-  Scales sc;
-  float fix;  // lane g: what is left of a value scale outside its exponent's range
-  auto scales = [&](int set) {
-    sc.held = tiles.held_codes[set];
-    const bool held = sc.held >> (lane & 3) & 1;
-    const float ks = tiles.ks[set], vs = held ? tiles.vs[set] : 1.0f;
-    const float k = held ? ks * a.scale + (ks - ks) : 1.0f;
-    const float lg = __builtin_fmaxf(__builtin_fminf(__builtin_amdgcn_logf(__builtin_fabsf(vs)), kScales), -kScales);
-    const float inv = __builtin_amdgcn_exp2f(-lg - kLift);
-    fix = vs * __builtin_amdgcn_exp2f(-lg);
-    const bool usual = k > 0.0f && k < __builtin_inff() && vs > 0.0f && __builtin_fabsf(lg) < kScales;
-    sc.usual = ((uint32_t)__ballot(usual) & 15) == 15;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      auto at = [&](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), g)); };
-      sc.k[g] = at(k), sc.log[g] = at(lg), sc.inverse[g] = at(inv);
-    }
-  };
-  // Tile kt from (kl, vl).  Between the products of the scores the next tile's codes
-  // become fp16 in (kn, vn), and the loads of the one after take their registers.
-  auto take = [&](int kt, auto parity, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
-    constexpr int set = decltype(parity)::value;
-    scales(set);
+  // Tile i of the piece from (kl, vl).  Between the products of the scores the next
+  // tile's codes become fp16 in (kn, vn), and the loads of the one after take their
+  // registers.
+  auto take = [&](int i, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
     lds_barrier();
-    const bool more = kt + 2 < p.t1;
-    tiles.begin(set);
-    tiles.load_page(kt + 3);
+    if (i % 2 == 0) tiles.step(i);
     auto feed = [&](int j) {
       tiles.store(j, kn, vn);
-      tiles.load(j, kt + 2, more);
+      tiles.load(j, i + 2, i + 2 < count);
     };
+    const int place = i % kBatch * 4;
+    const int key = (p.t0 + i) * kKeys;
     // the lane's places in the rows; out of the compiler's sight, or it keeps one register
-    // for each of their uses
-    int from_k = r * D + 8 * (h ^ k_swizzle<D>(r)), from_v = r * kKeys + 8 * (h ^ (r & 7));
+    // for each of their uses.  Row 8 x + 4 h + y of the scores is key 16 h + 4 x + y of
+    // its 32: a lane holds 16 keys side by side, of one page.
+    const int row_key = 16 * (r >> 2 & 1) + 4 * (r >> 3) + (r & 3);
+    int from_k = row_key * D + 8 * (h ^ k_swizzle<D>(row_key)), from_v = r * kKeys + 8 * (2 * h ^ (r & 7));
     asm volatile("" : "+v"(from_k), "+v"(from_v));
     f32x16 s[ST];
 #pragma unroll
@@ -371,36 +367,63 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
         if (j * 4 / (2 * T::N) == q) feed(j);
       __builtin_amdgcn_sched_barrier(0);
     }
-    const int past = seen - kt * kKeys - 4 * h;  // keys of the lane up to here are seen
-    if (__builtin_expect(!sc.usual, 0)) {
+    f32x4 say[ST];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+    for (int t = 0; t < ST; ++t) say[t] = info[i / kBatch & 1][place + 2 * t + h];
+    const uint32_t held = (uint32_t)(tiles.held >> place) & 15, usual = (uint32_t)(tiles.usual >> place) & 15;
+    const int past = seen - key - 16 * h;  // keys of the lane up to here are seen
+    if (__builtin_expect(usual != 15, 0)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[g / 2][8 * (g % 2) + i] *= sc.k[g];
-        sc.k[g] = 1.0f;
+      for (int t = 0; t < ST; ++t) {
+        s[t] *= say[t][0];
+        say[t][0] = 1.0f;
       }
     }
-    if (kt * kKeys + kKeys - 1 > all_see || sc.held != 15) {
+    if (key + kKeys - 1 > all_see || held != 15) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int last = sc.held >> g & 1 ? past - 16 * g : -1;
+      for (int t = 0; t < ST; ++t) {
+        const int last = held >> (2 * t + h) & 1 ? past - 32 * t : -1;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (8 * (i >> 2) + (i & 3) > last) s[g / 2][8 * (g % 2) + i] = -__builtin_inff();
+        for (int x = 0; x < 16; ++x)
+          if (x > last) s[t][x] = -__builtin_inff();
       }
     }
-    float peak = kNoMax;
+    f16x8 vf[2][VN], pf[2 * ST];
+    auto read_v = [&](int c) {  // group c of fragments: of 16 tokens, or half their channels
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float x = s[g / 2][8 * (g % 2)];
+      for (int d = 0; d < VN; ++d)
+        vf[c & 1][d] = *reinterpret_cast<const f16x8*>(vl + 32 * (c * VN % DT + d) * kKeys + (from_v ^ 8 * (c * VN / DT / 2 * 4 + c * VN / DT % 2)));
+    };
+    float sum;
+    auto weigh = [&]() {
+      sum = 0.0f;
 #pragma unroll
-      for (int i = 1; i < 8; ++i) x = __builtin_fmaxf(x, s[g / 2][8 * (g % 2) + i]);
-      peak = __builtin_fmaxf(peak, x * sc.k[g] + sc.log[g]);
-    }
-    stay_in_accumulators<D>(o);
-    if (__any(peak > m + kSlack)) {
+      for (int t = 0; t < ST; ++t) {
+        const float lift = say[t][1] + kLift - m;
+        float part = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const float w = __builtin_amdgcn_exp2f(s[t][x] * say[t][0] + lift);
+          part += w;
+          pf[2 * t + x / 8][x % 8] = (f16)w;
+        }
+        sum += part * say[t][2];
+      }
+    };
+    auto highest = [&]() {
+      float up = kNoMax;
+#pragma unroll
+      for (int t = 0; t < ST; ++t) {
+        float x = s[t][0];
+#pragma unroll
+        for (int y = 1; y < 16; ++y) x = __builtin_fmaxf(x, s[t][y]);
+        up = __builtin_fmaxf(up, x * say[t][0] + say[t][1]);
+      }
+      return up;
+    };
+    auto raise = [&](float up) {
       // row by row: what other rows of the wave see changes no bit of a row
-      float up = __builtin_fmaxf(peak, from_lane(peak, lane ^ 32));
+      up = __builtin_fmaxf(up, from_lane(up, lane ^ 32));
       if (!(up > m + kSlack)) up = m;
       const float f = __builtin_amdgcn_exp2f(m - up);
       m = up;
@@ -408,60 +431,70 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= f;
       stay_in_accumulators<D>(o);
-    }
-    f16x8 pf[2 * ST];
+    };
+    stay_in_accumulators<D>(o);
+    if constexpr (D == 256) {
+      // the scores beside their weights do not fit the registers
+      const float up = highest();
+      if (__any(up > m + kSlack)) raise(up);
+      weigh();
+    } else {
+      // with the maximum as it is; a weight that leaves its range shows it to be too low
+      weigh();
+      f16x8 top = pf[0];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float lift = sc.log[g] + kLift - m;
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = __builtin_amdgcn_exp2f(s[g / 2][8 * (g % 2) + i] * sc.k[g] + lift);
-        sum += w;
-        pf[g][i] = (f16)w;
+      for (int g = 1; g < 4; ++g) top = __builtin_elementwise_max(top, pf[g]);
+      const f16x4 top4 = __builtin_elementwise_max(__builtin_shufflevector(top, top, 0, 1, 2, 3), __builtin_shufflevector(top, top, 4, 5, 6, 7));
+      const f16x2 top2 = __builtin_elementwise_max(__builtin_shufflevector(top4, top4, 0, 1), __builtin_shufflevector(top4, top4, 2, 3));
+      if (__any(top2[0] > (f16)kMost || top2[1] > (f16)kMost)) {
+        raise(highest());
+        weigh();
       }
-      l += sum * sc.inverse[g];
     }
-    if (__builtin_expect(!sc.usual, 0)) {
+    l += sum;
+    read_v(0);
+    if (__builtin_expect(usual != 15, 0)) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f16 x = (f16)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, fix), g));
-        const int last = sc.held >> g & 1 ? past - 16 * g : -1;
+      for (int t = 0; t < ST; ++t) {
+        const int last = held >> (2 * t + h) & 1 ? past - 32 * t : -1;
         // a key that is not seen has no weight, and none of a scale that is not finite either
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pf[g][i] = 8 * (i >> 2) + (i & 3) > last ? (f16)0.0f : pf[g][i] * x;
+        for (int x = 0; x < 16; ++x) pf[2 * t + x / 8][x % 8] = x > last ? (f16)0.0f : pf[2 * t + x / 8][x % 8] * (f16)say[t][3];
       }
     }
 #pragma unroll
-    for (int c = 0; c < 2 * ST; ++c)
+    for (int c = 0; c < 2 * ST * DT / VN; ++c) {
+      if (c + 1 < 2 * ST * DT / VN) read_v(c + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const f16x8 vf = *reinterpret_cast<const f16x8*>(vl + 32 * d * kKeys + (from_v ^ 16 * c));
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[c], o[d], 0, 0, 0);
+      for (int d = 0; d < VN; ++d) {
+        f32x16& to = o[c * VN % DT + d];
+        to = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c & 1][d], pf[c * VN / DT], to, 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   if (wave_row >= rows) {
     // a wave without rows brings the tiles for the others
-    auto bring = [&](int kt, auto parity, uint16_t* kn, uint16_t* vn) {
-      constexpr int set = decltype(parity)::value;
+    auto bring = [&](int i, uint16_t* kn, uint16_t* vn) {
       lds_barrier();
-      tiles.begin(set);
-      tiles.load_page(kt + 3);
+      if (i % 2 == 0) tiles.step(i);
 #pragma unroll
       for (int j = 0; j < 2 * T::N; ++j) {
         tiles.store(j, kn, vn);
-        tiles.load(j, kt + 2, kt + 2 < p.t1);
+        tiles.load(j, i + 2, i + 2 < count);
       }
     };
-    for (int kt = p.t0; kt < p.t1; kt += 2) {
-      bring(kt, std::integral_constant<int, 0>(), k1, v1);
-      if (kt + 1 < p.t1) bring(kt + 1, std::integral_constant<int, 1>(), k0, v0);
+    for (int i = 0; i < count; i += 2) {
+      bring(i, k1, v1);
+      if (i + 1 < count) bring(i + 1, k0, v0);
     }
-  } else
-  for (int kt = p.t0; kt < p.t1; kt += 2) {
-    take(kt, std::integral_constant<int, 0>(), k0, v0, k1, v1);
-    if (kt + 1 < p.t1) take(kt + 1, std::integral_constant<int, 1>(), k1, v1, k0, v0);
-    stay_in_accumulators<D>(o);
+  } else {
+    for (int i = 0; i < count; i += 2) {
+      take(i, k0, v0, k1, v1);
+      if (i + 1 < count) take(i + 1, k1, v1, k0, v0);
+      stay_in_accumulators<D>(o);
+    }
   }
 
   l += from_lane(l, lane ^ 32);

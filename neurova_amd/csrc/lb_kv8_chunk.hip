@@ -18,6 +18,19 @@
 namespace lb {
 namespace {
 
+// x / d for 0 <= x < 2^31 by a product: with 2^(s - 1) < d <= 2^s and m = ceil(2^(31 + s) / d)
+// the product is off by less than x 2^s / 2^(31 + s) < 1 / d of a quotient.
+struct Divisor {
+  uint32_t m;
+  int shift, d;
+  explicit Divisor(int by = 1) : m(0), shift(0), d(by) {
+    if (by <= 1) return;
+    while ((1ll << (shift + 1)) < by) ++shift;
+    m = (uint32_t)(((1ll << (32 + shift)) + by - 1) / by);
+  }
+  __device__ __forceinline__ int of(int x) const { return m ? (int)(__umulhi((uint32_t)x, m) >> shift) : x; }
+};
+
 struct ChunkArgs {
   const uint16_t* q;
   int64_t q_token, q_head;
@@ -27,9 +40,11 @@ struct ChunkArgs {
   uint16_t* out;
   int64_t o_token, o_head;
   float* parts;
+  struct Work* plan;  // behind the parts: how the keys were cut
   int64_t table_stride;
   int num_pages, page_shift, max_tokens;
-  int batch, tokens, heads_kv, group;
+  int batch, tokens;
+  Divisor heads_kv, group;
   int workers, slots;  // workgroups that run at once; parts that the scratch holds
   float scale;         // softmax scale * log2(e)
 };
@@ -43,7 +58,12 @@ constexpr float kNoMax = -1e30f;
 // no weight that counts in the sum falls below fp32's normal numbers.
 constexpr float kSlack = 8.0f, kLift = 7.0f, kScales = 32.0f, kMost = 32768.0f;  // 2^(kSlack + kLift)
 // A piece of a row block's keys is this many tiles at least.
-constexpr int kMinTiles = 4;
+constexpr int kMinTiles = 2;
+constexpr int kCuts = 24;
+// In tiles: what a piece takes beside its own, the launch that joins cut ones, and for
+// each round of these what their parts take to write and read.
+constexpr float kPiece = 3.0f, kCut = 2.0f, kPart = 5.0f;
+constexpr int kPartRounds = 4;  // of parts that the scratch holds
 
 template <int D>
 constexpr int kPerSimd = D == 256 ? 1 : 2;
@@ -64,7 +84,7 @@ __device__ __forceinline__ Seq seq_of(const ChunkArgs& a, int b) {
   s.len = min(full, a.max_tokens), s.at = full - s.n;
   return s;
 }
-__device__ __forceinline__ int blocks_of(const ChunkArgs& a, const Seq& s) { return (s.n * a.group + kRows - 1) / kRows; }
+__device__ __forceinline__ int blocks_of(const ChunkArgs& a, const Seq& s) { return (s.n * a.group.d + kRows - 1) / kRows; }
 __device__ __forceinline__ int tiles_of(const Seq& s) { return max((s.len + kKeys - 1) / kKeys, 1); }
 // Pieces of each of a sequence's row blocks.  The float quotient is exact enough:
 // (x + 1/2) / most is 1 / (2 most) away from an integer, more than its error.
@@ -72,28 +92,68 @@ __device__ __forceinline__ int pieces_in(int tiles, int most, float inverse) {
   return (int)(((float)(tiles + most - 1) + 0.5f) * inverse);
 }
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), kWave - 1); }
+// The lane with the smallest v (above zero), the lowest of several.
+__device__ __forceinline__ int wave_least(float v) {
+  uint32_t x = (__builtin_bit_cast(uint32_t, v) & ~63u) | lane_id();
+  auto least = [&](uint32_t other) { x = min(x, other); };
+  least(__builtin_amdgcn_update_dpp(~0, x, 0x111, 0xf, 0xf, false));  // as in wave_scan
+  least(__builtin_amdgcn_update_dpp(~0, x, 0x112, 0xf, 0xf, false));
+  least(__builtin_amdgcn_update_dpp(~0, x, 0x114, 0xf, 0xf, false));
+  least(__builtin_amdgcn_update_dpp(~0, x, 0x118, 0xf, 0xf, false));
+  least(__builtin_amdgcn_update_dpp(~0, x, 0x142, 0xa, 0xf, false));
+  least(__builtin_amdgcn_update_dpp(~0, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, kWave - 1) & 63;
+}
 
-// Every row block's keys are cut into pieces of at most `most` tiles, a workgroup
-// each: about as many as run at once, where there are fewer row blocks than that.
+// Every row block's keys are cut into pieces of at most `most` tiles, a workgroup each.
 struct Work {
-  int most, total;
+  int most, total;  // pieces of all sequences, of one head
 };
+// A lane tries one length of the pieces: the longest row block's keys cut into one to
+// kCuts, or what all workers have in all and somewhat more, so that all run at once.  What
+// has the least rounds of pieces times their mean length, and the time that a piece takes
+// besides, is taken.  (Above 64 sequences: what the workers have in all.)
 __device__ __forceinline__ Work work_of(const ChunkArgs& a, const Seq& own) {
-  const int lane = lane_id();
-  auto sum = [&](auto of) {
-    int n = wave_total(of(own));
-    for (int c = kWave; c < a.batch; c += kWave) n += wave_total(of(seq_of(a, c + lane)));
-    return n;
-  };
-  const int tiles = sum([&](const Seq& s) { return blocks_of(a, s) * tiles_of(s); }) * a.heads_kv;
-  Work w;
-  w.most = max((tiles + a.workers - 1) / a.workers, kMinTiles);
-  for (int tries = 0;; ++tries) {
-    const float inverse = __builtin_amdgcn_rcpf((float)w.most);
-    w.total = sum([&](const Seq& s) { return blocks_of(a, s) * pieces_in(tiles_of(s), w.most, inverse); });
-    if (tries == 8 || w.total * a.heads_kv <= a.workers) return w;
-    w.most += max(w.most / 16, 1);
+  const int lane = lane_id(), blocks = blocks_of(a, own), tiles = tiles_of(own);
+  const float heads = (float)a.heads_kv.d, slots = __builtin_amdgcn_rcpf((float)a.workers);
+  if (a.batch > kWave) {
+    int all = wave_total(blocks * tiles);
+    for (int c = kWave; c < a.batch; c += kWave) {
+      const Seq s = seq_of(a, c + lane);
+      all += wave_total(blocks_of(a, s) * tiles_of(s));
+    }
+    const int most = max((int)((float)all * heads * slots) + 1, kMinTiles);
+    const float inverse = __builtin_amdgcn_rcpf((float)most);
+    int n = wave_total(blocks * pieces_in(tiles, most, inverse));
+    for (int c = kWave; c < a.batch; c += kWave) {
+      const Seq s = seq_of(a, c + lane);
+      n += wave_total(blocks_of(a, s) * pieces_in(tiles_of(s), most, inverse));
+    }
+    return {most, n};
   }
+  int all = 0, longest = 1;
+  for (int b = 0; b < a.batch; ++b) {
+    const int n = __builtin_amdgcn_readlane(blocks, b), t = __builtin_amdgcn_readlane(tiles, b);
+    all += n * t;
+    if (n) longest = max(longest, t);
+  }
+  const float work = (float)all * heads, share = work * slots;
+  const int cuts = lane + 1;
+  int most = lane < kCuts ? (int)((float)(longest + lane) * __builtin_amdgcn_rcpf((float)cuts) + 0.5f) : (int)(share * (1.0f + (lane - kCuts) * 0.02f)) + 1;
+  most = max(min(most, longest), kMinTiles);
+  const float inverse = __builtin_amdgcn_rcpf((float)most);
+  int n = 0, cut = 0;
+  for (int b = 0; b < a.batch; ++b) {
+    const int each = pieces_in(__builtin_amdgcn_readlane(tiles, b), most, inverse), x = __builtin_amdgcn_readlane(blocks, b) * each;
+    n += x, cut += each > 1 ? x : 0;
+  }
+  const float count = (float)n * heads, rounds = __builtin_ceilf(count * slots);
+  const float mean = __builtin_fmaxf(work * __builtin_amdgcn_rcpf(count), rounds <= 1.0f ? (float)min(most, longest) : 0.0f);
+  float cost = rounds * (mean + kPiece);
+  if (cut) cost += kCut + kPart * (float)cut * heads * slots;
+  if (cut * a.heads_kv.d > a.slots) cost = 3e38f;
+  const int best = wave_least(cost);
+  return {__builtin_amdgcn_readlane(most, best), __builtin_amdgcn_readlane(n, best)};
 }
 
 // A row block's piece of keys, tiles [t0, t1).
@@ -103,38 +163,63 @@ struct Piece {
   Seq s;
 };
 __device__ __forceinline__ int block_tiles(const ChunkArgs& a, const Seq& s, int block) {
-  const int last = min(s.n - 1, ((block + 1) * kRows - 1) / a.group);  // token of the last row
+  const int last = min(s.n - 1, a.group.of((block + 1) * kRows - 1));  // token of the last row
   return max((min(s.at + last + 1, s.len) + kKeys - 1) / kKeys, 0);
 }
 __device__ __forceinline__ Seq seq_from(const Seq& s, int lane) {
   return {__builtin_amdgcn_readlane(s.first, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.len, lane),
           __builtin_amdgcn_readlane(s.at, lane)};
 }
-// Piece i of all, in the order of the sequences and the last row block first.
+// Piece i of all, the last row block of a sequence first.  With more pieces than run at
+// once the sequences with the longest come first (of up to 64 sequences): short ones last
+// fill the ends.
 // JOIN: row block i of those that have several pieces, and its first.
 template <bool JOIN>
 __device__ __forceinline__ bool piece_of(const ChunkArgs& a, const Seq& own, const Work& w, int i, Piece& p) {
   const int lane = lane_id();
   const float inverse = __builtin_amdgcn_rcpf((float)w.most);
+  // x-th piece (row block) of the sequence in lane `at`, which has `blocks` cut into `pieces`
+  auto found = [&](const Seq& s, int b, int at, int x, int blocks, int pieces, int slots) {
+    p.s = seq_from(s, at), p.b = b, p.pieces = pieces;
+    int q = JOIN ? x : (int)(((float)x + 0.5f) * __builtin_amdgcn_rcpf((float)pieces));
+    p.piece = JOIN ? 0 : x - q * pieces;
+    if (!JOIN && p.piece < 0) --q, p.piece += pieces;
+    if (!JOIN && p.piece >= pieces) ++q, p.piece -= pieces;
+    p.block = blocks - 1 - q;
+    p.slot = slots + q * pieces + p.piece;
+    const int tiles = block_tiles(a, p.s, p.block);
+    const float each = (float)tiles * __builtin_amdgcn_rcpf((float)pieces);
+    p.t0 = min((int)(each * (float)p.piece), tiles);
+    p.t1 = p.piece + 1 == pieces ? tiles : min((int)(each * (float)(p.piece + 1)), tiles);
+  };
+  if (a.batch == 1) {
+    const int blocks = __builtin_amdgcn_readlane(blocks_of(a, own), 0);
+    const int pieces = __builtin_amdgcn_readlane(pieces_in(tiles_of(own), w.most, inverse), 0);
+    if (i >= (JOIN ? (pieces > 1 ? blocks : 0) : blocks * pieces)) return false;
+    found(own, 0, 0, i, blocks, pieces, 0);
+    return true;
+  }
   int base = 0, slots = 0;
   for (int c = 0; c < a.batch; c += kWave) {
     const Seq s = c ? seq_of(a, c + lane) : own;
     const int blocks = blocks_of(a, s), pieces = pieces_in(tiles_of(s), w.most, inverse);
     const int split = pieces > 1 ? blocks * pieces : 0;
     const int size = JOIN ? (pieces > 1 ? blocks : 0) : blocks * pieces;
-    const int upto = wave_scan(size), all = __builtin_amdgcn_readlane(upto, kWave - 1);
+    int upto = wave_scan(size);
+    const int all = __builtin_amdgcn_readlane(upto, kWave - 1);
     const int split_upto = wave_scan(split);
     if (base + all > i) {
-      const int at = __builtin_ctzll(__ballot(base + upto > i));
-      const int x = i - base - __builtin_amdgcn_readlane(upto - size, at);
-      p.s = seq_from(s, at);
-      p.b = c + at, p.pieces = __builtin_amdgcn_readlane(pieces, at);
-      const int from_last = JOIN ? x : x / p.pieces;
-      p.block = __builtin_amdgcn_readlane(blocks, at) - 1 - from_last;
-      p.piece = JOIN ? 0 : x - from_last * p.pieces;
-      p.slot = slots + __builtin_amdgcn_readlane(split_upto - split, at) + from_last * p.pieces + p.piece;
-      const uint32_t tiles = block_tiles(a, p.s, p.block);
-      p.t0 = tiles * p.piece / p.pieces, p.t1 = tiles * (p.piece + 1) / p.pieces;
+      if (!JOIN && a.batch <= kWave && w.total * a.heads_kv.d > a.workers) {
+        const int length = pieces > 1 ? w.most : tiles_of(s);
+        upto = size;
+        for (int b = 0; b < a.batch; ++b) {
+          const int other = __builtin_amdgcn_readlane(length, b);
+          if (other > length || (other == length && b < lane)) upto += __builtin_amdgcn_readlane(size, b);
+        }
+      }
+      const int at = __builtin_ctzll(__ballot(base + upto > i && base + upto - size <= i));
+      found(s, c + at, at, i - base - __builtin_amdgcn_readlane(upto - size, at), __builtin_amdgcn_readlane(blocks, at),
+            __builtin_amdgcn_readlane(pieces, at), slots + __builtin_amdgcn_readlane(split_upto - split, at));
       return true;
     }
     base += all, slots += __builtin_amdgcn_readlane(split_upto, kWave - 1);
@@ -201,7 +286,7 @@ struct Tiles {
   __device__ __forceinline__ void load_scales(int batch) {
     const bool real = token(batch) < len && (unsigned)page < (unsigned)a.num_pages;
     next_held = __ballot(real);
-    next_cell = (real ? page : 0) * a.heads_kv + head;
+    next_cell = (real ? page : 0) * a.heads_kv.d + head;
     ks = a.k_scale[next_cell], vs = a.v_scale[next_cell];
   }
   __device__ __forceinline__ void tell(int batch) {
@@ -276,19 +361,20 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
   __shared__ Info info;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 31, h = lane >> 5;
-  const int kvh = blockIdx.x % a.heads_kv, item = blockIdx.x / a.heads_kv;
+  const int item = a.heads_kv.of(blockIdx.x), kvh = blockIdx.x - item * a.heads_kv.d;
   Piece p;
   {
     const Seq own = seq_of(a, lane);
     const Work w = work_of(a, own);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.slots > 0) *a.plan = w;  // for the join
     if (!piece_of<false>(a, own, w, item, p)) return;
   }
-  const int rows = p.s.n * a.group, wave_row = p.block * kRows + wave * 32;
-  const int row = wave_row + r, token = row / a.group, q_head = kvh * a.group + row - token * a.group;
+  const int rows = p.s.n * a.group.d, wave_row = p.block * kRows + wave * 32;
+  const int row = wave_row + r, token = a.group.of(row), q_head = kvh * a.group.d + row - token * a.group.d;
   const bool real = row < rows;
   // the lane's row sees the keys up to `seen`, all of the wave's those up to `all_see`
   const int seen = real ? min(p.s.at + token, p.s.len - 1) : -1;
-  const int all_see = min(p.s.at + wave_row / a.group, p.s.len - 1);
+  const int all_see = min(p.s.at + a.group.of(wave_row), p.s.len - 1);
 
   f16x8 qf[KK];
   {
@@ -366,6 +452,10 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
       for (int j = 0; j < 2 * T::N; ++j)
         if (j * 4 / (2 * T::N) == q) feed(j);
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (D == 256) {  // in vector registers from here, not brought there for each use
+#pragma unroll
+      for (int t = 0; t < ST; ++t) asm volatile("" : "+v"(s[t]));
     }
     f32x4 say[ST];
 #pragma unroll
@@ -499,7 +589,7 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
 
   l += from_lane(l, lane ^ 32);
   if (p.pieces > 1) {
-    const int slot = p.slot * a.heads_kv + kvh;
+    const int slot = p.slot * a.heads_kv.d + kvh;
     if (slot >= a.slots) return;
     float* part = a.parts + (int64_t)slot * kPartFloats<D>;
     if (real) {
@@ -519,7 +609,7 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
   const float inv = l > 0.0f ? __builtin_exp2f(-kLift) / l : l == 0.0f ? 0.0f : l;
   int again = wave_row + r;  // the row's place once more: kept over the loop it would take registers
   asm volatile("" : "+v"(again));
-  const int to_token = again / a.group, to_head = kvh * a.group + again - to_token * a.group;
+  const int to_token = a.group.of(again), to_head = kvh * a.group.d + again - to_token * a.group.d;
   const int64_t place = (int64_t)(p.s.first + to_token) * a.o_token + (int64_t)to_head * a.o_head;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -551,22 +641,21 @@ __global__ __launch_bounds__(kWave * kWaves) void kv8_chunk_join_kernel(ChunkArg
   const int r = lane & 31, h = lane >> 5;
   constexpr int DT = D / 32;
   const Seq own = seq_of(a, lane);
-  const Work w = work_of(a, own);
+  const Work w = *a.plan;
   for (int x = blockIdx.x;; x += gridDim.x) {
-    int y = x / a.heads_kv;
-    const int kvh = x - y * a.heads_kv, d = y % DT, quarter = y / DT % kWaves;
+    const int y = a.heads_kv.of(x), kvh = x - y * a.heads_kv.d, d = y % DT, quarter = y / DT % kWaves;
     Piece p;
     if (!piece_of<true>(a, own, w, y / (DT * kWaves), p)) return;
-    const int rows = p.s.n * a.group, first_row = p.block * kRows + quarter * 32;
+    const int rows = p.s.n * a.group.d, first_row = p.block * kRows + quarter * 32;
     if (first_row >= rows) continue;
-    const int row = first_row + r, token = row / a.group, q_head = kvh * a.group + row - token * a.group;
+    const int row = first_row + r, token = a.group.of(row), q_head = kvh * a.group.d + row - token * a.group.d;
     float m = kNoMax, l = 0.0f;
     f32x4 o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = (f32x4)(0.0f);
     if (row < rows)
       for (int j = wave; j < p.pieces; j += kWaves) {
-        const int slot = (p.slot + j) * a.heads_kv + kvh;
+        const int slot = (p.slot + j) * a.heads_kv.d + kvh;
         if (slot >= a.slots) break;
         const float* part = a.parts + (int64_t)slot * kPartFloats<D>;
         const float pm = part[quarter * 32 + r], pl = part[kRows + quarter * 32 + r];
@@ -607,8 +696,8 @@ struct Plan {
   size_t scratch;
 };
 
-// Row blocks that are cut have more than `most` tiles each, of workers * most in all:
-// at most as many as the workers, and their pieces twice that.
+// Above 64 sequences the row blocks that are cut have more than `most` tiles each, of
+// workers * most in all: at most as many as the workers, and their pieces twice that.
 Plan plan_of(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv, int64_t head_dim, int64_t max_tokens) {
   Plan p;
   p.workers = (head_dim == 64 ? kPerSimd<64> : head_dim == 128 ? kPerSimd<128> : kPerSimd<256>) * (int64_t)lbh::device_cus();
@@ -617,9 +706,9 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv, i
   p.joined = tiles > kMinTiles;
   // no more pieces than all row blocks have of the smallest size
   const int64_t pieces = blocks * ((tiles + kMinTiles - 1) / kMinTiles);
-  p.slots = !p.joined ? 0 : pieces < 2 * p.workers ? pieces : 2 * p.workers;
+  p.slots = !p.joined ? 0 : pieces < kPartRounds * p.workers ? pieces : kPartRounds * p.workers;
   p.grid = blocks + p.slots;
-  p.scratch = ((size_t)p.slots * kRows * (head_dim + 2) * 4 + 255) & ~(size_t)255;
+  p.scratch = p.slots ? (((size_t)p.slots * kRows * (head_dim + 2) * 4 + 255) & ~(size_t)255) + 256 : 0;
   return p;
 }
 
@@ -683,10 +772,11 @@ extern "C" int lb_kv8_chunk_attention(const uint16_t* q, int64_t q_token_stride,
   a.k_cache = k_cache, a.v_cache = v_cache, a.k_scale = k_scale, a.v_scale = v_scale;
   a.page_table = page_table, a.seq_lens = seq_lens, a.starts = cu_seqlens;
   a.out = out, a.o_token = o_token_stride, a.o_head = o_head_stride;
-  a.parts = static_cast<float*>(scratch), a.table_stride = table_stride;
+  a.parts = static_cast<float*>(scratch), a.plan = p.slots ? reinterpret_cast<Work*>(static_cast<char*>(scratch) + p.scratch - 256) : nullptr;
+  a.table_stride = table_stride;
   a.num_pages = (int)num_pages, a.page_shift = __builtin_ctzll((unsigned long long)page_size);
   a.max_tokens = (int)max_tokens;
-  a.batch = (int)batch, a.tokens = (int)tokens, a.heads_kv = (int)heads_kv, a.group = (int)(heads_q / heads_kv);
+  a.batch = (int)batch, a.tokens = (int)tokens, a.heads_kv = Divisor((int)heads_kv), a.group = Divisor((int)(heads_q / heads_kv));
   a.workers = (int)p.workers, a.slots = (int)p.slots;
   a.scale = softmax_scale * kLog2e;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);

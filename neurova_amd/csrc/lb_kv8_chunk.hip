@@ -108,6 +108,7 @@ __device__ __forceinline__ int wave_least(float v) {
 // Every row block's keys are cut into pieces of at most `most` tiles, a workgroup each.
 struct Work {
   int most, total;  // pieces of all sequences, of one head
+  int tail, cuts;   // of a single sequence: so many first row blocks are cut into `cuts`, the others not at all (tail 0: all alike)
 };
 // A lane tries one length of the pieces: the longest row block's keys cut into one to
 // kCuts, or what all workers have in all and somewhat more, so that all run at once.  What
@@ -129,7 +130,7 @@ __device__ __forceinline__ Work work_of(const ChunkArgs& a, const Seq& own) {
       const Seq s = seq_of(a, c + lane);
       n += wave_total(blocks_of(a, s) * pieces_in(tiles_of(s), most, inverse));
     }
-    return {most, n};
+    return {most, n, 0, 1};
   }
   int all = 0, longest = 1;
   for (int b = 0; b < a.batch; ++b) {
@@ -153,7 +154,19 @@ __device__ __forceinline__ Work work_of(const ChunkArgs& a, const Seq& own) {
   if (cut) cost += kCut + kPart * (float)cut * heads * slots;
   if (cut * a.heads_kv.d > a.slots) cost = 3e38f;
   const int best = wave_least(cost);
-  return {__builtin_amdgcn_readlane(most, best), __builtin_amdgcn_readlane(n, best)};
+  Work w = {__builtin_amdgcn_readlane(most, best), __builtin_amdgcn_readlane(n, best), 0, 1};
+  if (a.batch == 1) {
+    // whole row blocks for some rounds, and what is left of them, the shortest, cut so that it
+    // fills one more
+    const int count = __builtin_amdgcn_readlane(blocks, 0), full = (int)((float)(count * a.heads_kv.d) * slots + 0.001f);
+    const int tail = count - (int)((float)(full * a.workers) * __builtin_amdgcn_rcpf(heads) + 0.001f);
+    const int cuts = tail > 0 ? (int)((float)a.workers * __builtin_amdgcn_rcpf((float)tail * heads) + 0.001f) : 1;
+    const float least = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, cost), best));
+    const float one = (float)longest, tailed = (float)full * (one + kPiece) + one * __builtin_amdgcn_rcpf((float)cuts) + kPiece + kCut + kPart;
+    if (full > 0 && cuts > 1 && longest >= cuts * kMinTiles && tail * cuts * a.heads_kv.d <= a.slots && tailed < least)
+      w = {longest, count - tail + tail * cuts, tail, cuts};
+  }
+  return w;
 }
 
 // A row block's piece of keys, tiles [t0, t1).
@@ -194,6 +207,14 @@ __device__ __forceinline__ bool piece_of(const ChunkArgs& a, const Seq& own, con
   };
   if (a.batch == 1) {
     const int blocks = __builtin_amdgcn_readlane(blocks_of(a, own), 0);
+    if (w.tail) {
+      const int whole = blocks - w.tail;
+      if (i >= (JOIN ? w.tail : w.total)) return false;
+      if (JOIN) found(own, 0, 0, i, w.tail, w.cuts, 0);
+      else if (i < whole) found(own, 0, 0, i, blocks, 1, 0);
+      else found(own, 0, 0, i - whole, w.tail, w.cuts, 0);
+      return true;
+    }
     const int pieces = __builtin_amdgcn_readlane(pieces_in(tiles_of(own), w.most, inverse), 0);
     if (i >= (JOIN ? (pieces > 1 ? blocks : 0) : blocks * pieces)) return false;
     found(own, 0, 0, i, blocks, pieces, 0);
@@ -272,13 +293,13 @@ struct Tiles {
     groups = min(a.page_shift - 4, 2), per = kWave >> groups, in = D / per;
     const int row = (wave * kWave + lane) / (D / 16), col = 2 * (lane % (D / 16));
     k_off = (row & 15) * D + col * 8;
-    k_lds = row * D + 8 * (col ^ k_swizzle<D>(row));
+    k_lds = row * D + 8 * (col ^ (col >> 4) ^ k_swizzle<D>(row));
     v_off = (((wave % in) * per + (lane >> groups)) << a.page_shift) + (lane & ((1 << groups) - 1)) * 16;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int y = i * kWaves + wave, g = (y / in << groups) + (lane & ((1 << groups) - 1));
       const int ch = (y % in) * per + (lane >> groups);
-      v_lds[i] = ch * kKeys + 8 * ((2 * g) ^ (ch & 7));
+      v_lds[i] = ch * kKeys + 8 * ((2 * g) ^ (ch >> 1 & 7));
     }
   }
   __device__ __forceinline__ int token(int batch) const { return (first + batch * kBatch) * kKeys + 16 * lane; }
@@ -424,7 +445,7 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
     // for each of their uses.  Row 8 x + 4 h + y of the scores is key 16 h + 4 x + y of
     // its 32: a lane holds 16 keys side by side, of one page.
     const int row_key = 16 * (r >> 2 & 1) + 4 * (r >> 3) + (r & 3);
-    int from_k = row_key * D + 8 * (h ^ k_swizzle<D>(row_key)), from_v = r * kKeys + 8 * (2 * h ^ (r & 7));
+    int from_k = row_key * D + 8 * (h ^ k_swizzle<D>(row_key)), from_v = r * kKeys + 8 * (2 * h ^ (r >> 1 & 7));
     asm volatile("" : "+v"(from_k), "+v"(from_v));
     f32x16 s[ST];
 #pragma unroll
@@ -436,10 +457,11 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
       for (int k = 0; k < CH; ++k)
 #pragma unroll
         for (int t = 0; t < ST; ++t) {
-          kf[q & 1][k][t] = *reinterpret_cast<const f16x8*>(kl + 32 * t * D + (from_k ^ 16 * (q * CH + k)));
+          kf[q & 1][k][t] = *reinterpret_cast<const f16x8*>(kl + 32 * t * D + (from_k ^ 16 * (q * CH + k) ^ (q * CH + k >= 8 ? 8 : 0)));
         }
     };
     read_k(0);
+    __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -453,6 +475,7 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
         if (j * 4 / (2 * T::N) == q) feed(j);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     if constexpr (D == 256) {  // in vector registers from here, not brought there for each use
 #pragma unroll
       for (int t = 0; t < ST; ++t) asm volatile("" : "+v"(s[t]));
@@ -552,6 +575,7 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
         for (int x = 0; x < 16; ++x) pf[2 * t + x / 8][x % 8] = x > last ? (f16)0.0f : pf[2 * t + x / 8][x % 8] * (f16)say[t][3];
       }
     }
+    __builtin_amdgcn_s_setprio(2);
 #pragma unroll
     for (int c = 0; c < 2 * ST * DT / VN; ++c) {
       if (c + 1 < 2 * ST * DT / VN) read_v(c + 1);

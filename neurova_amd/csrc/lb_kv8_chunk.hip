@@ -373,24 +373,129 @@ __device__ __forceinline__ void stay_in_accumulators(f32x16 (&o)[N]) {
     for (int d = 0; d < N; ++d) asm volatile("" : "+a"(o[d]));
 }
 
-template <int D>
-__global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(ChunkArgs a) {
-  constexpr int DT = D / 32, KK = D / 16, ST = kKeys / 32;
-  constexpr int VN = DT < 4 ? DT : 4;  // fragments of values read ahead
-  // four arrays and not one: reads of a tile then need not wait for writes of the next
-  __shared__ __align__(16) uint16_t k0[kKeys * D], k1[kKeys * D], v0[kKeys * D], v1[kKeys * D];
-  __shared__ Info info;
+// The end of a piece of up to 32 rows: waves 0 and 1 hold the first half of the channels,
+// of 32 keys of every tile each, 2 and 3 the second.  `sums` (fp16 of 32 rows and more),
+// `states` and `lines` are places in LDS that no wave reads any more after a barrier.
+template <int D, int N>
+__device__ __forceinline__ void finish_thin(const ChunkArgs& a, const Piece& p, int kvh, int wave, int lane, f32x16 (&o)[N], float m, float l,
+                                            uint16_t* sums, float* states, uint16_t* lines) {
+  constexpr int DB = D / 64;
+  const int r = lane & 31, h = lane >> 5, half = wave >> 1, rows = p.s.n * a.group.d, first = p.block * kRows;
+  f32x4* to = reinterpret_cast<f32x4*>(sums) + lane;
+  lds_barrier();
+  if (wave & 1) {
+    if (h == 0) states[half * 64 + r] = m, states[half * 64 + 32 + r] = l;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[(4 * d + i) * kWave] = (f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+  }
+  lds_barrier();
+  if (!(wave & 1)) {
+    const float m1 = states[half * 64 + r], l1 = states[half * 64 + 32 + r], up = __builtin_fmaxf(m, m1);
+    const float f = __builtin_amdgcn_exp2f(m - up), f1 = __builtin_amdgcn_exp2f(m1 - up);
+    m = up, l = l * f + l1 * f1;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 x = to[(4 * d + i) * kWave];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[d][4 * i + j] = o[d][4 * i + j] * f + x[j] * f1;
+      }
+  }
+  if (p.pieces > 1) {
+    const int slot = p.slot * a.heads_kv.d + kvh;
+    if (slot >= a.slots || (wave & 1) || first + r >= rows) return;
+    float* part = a.parts + (int64_t)slot * kPartFloats<D>;
+    if (lane == r && half == 0) part[r] = m, part[kRows + r] = l;
+    f32x4* out = reinterpret_cast<f32x4*>(part + 2 * kRows) + lane;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[(4 * (half * DB + d) + i) * kWave] = (f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+    return;
+  }
+  if (!(wave & 1)) {
+    const float inv = l > 0.0f ? __builtin_exp2f(-kLift) / l : l == 0.0f ? 0.0f : l;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        u32x2 w;
+        w[0] = as_u32((f16x2){(f16)(o[d][i] * inv), (f16)(o[d][i + 1] * inv)});
+        w[1] = as_u32((f16x2){(f16)(o[d][i + 2] * inv), (f16)(o[d][i + 3] * inv)});
+        *reinterpret_cast<u32x2*>(lines + r * D + 8 * ((4 * (half * DB + d) + i / 4) ^ k_swizzle<D>(r)) + 4 * h) = w;
+      }
+  }
+  lds_barrier();
+#pragma unroll
+  for (int j = 0; j < 32 * D / 8 / (kWave * kWaves); ++j) {
+    const int x = (j * kWaves + wave) * kWave + lane, rr = x / (D / 8), chunk = x % (D / 8);
+    const int row = first + rr, token = a.group.of(row), head = kvh * a.group.d + row - token * a.group.d;
+    const u32x4 w = *reinterpret_cast<const u32x4*>(lines + rr * D + 8 * (chunk ^ k_swizzle<D>(rr)));
+    if (row < rows) *reinterpret_cast<u32x4*>(a.out + (int64_t)(p.s.first + token) * a.o_token + (int64_t)head * a.o_head + 8 * chunk) = w;
+  }
+}
+
+// The end of a piece of more rows: each wave's 32, through `mine`, where no wave reads any
+// more after a barrier.  (The row's place is found once more: kept over the loop it would
+// take registers.)
+template <int D, int N>
+__device__ __forceinline__ void finish(const ChunkArgs& a, const Piece& p, int kvh, int wave, int lane, f32x16 (&o)[N], float m, float l, uint16_t* mine) {
+  constexpr int DT = D / 32;
+  const int r = lane & 31, h = lane >> 5, rows = p.s.n * a.group.d, wave_row = p.block * kRows + wave * 32;
+  int row = wave_row + r;
+  asm volatile("" : "+v"(row));
+  if (p.pieces > 1) {
+    const int slot = p.slot * a.heads_kv.d + kvh;
+    if (slot >= a.slots) return;
+    float* part = a.parts + (int64_t)slot * kPartFloats<D>;
+    if (row < rows) {
+      if (h == 0) part[wave * 32 + r] = m, part[kRows + wave * 32 + r] = l;
+      f32x4* to = reinterpret_cast<f32x4*>(part + 2 * kRows + wave * 32 * D) + lane;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          to[(4 * d + i) * kWave] = (f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+    }
+    return;
+  }
+  // the rows leave through LDS, a wave's 32 x D in an array that no wave reads any more
+  lds_barrier();
+  const float inv = l > 0.0f ? __builtin_exp2f(-kLift) / l : l == 0.0f ? 0.0f : l;
+  const int to_token = a.group.of(row), to_head = kvh * a.group.d + row - to_token * a.group.d;
+  const int64_t place = (int64_t)(p.s.first + to_token) * a.o_token + (int64_t)to_head * a.o_head;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      u32x2 w;
+      w[0] = as_u32((f16x2){(f16)(o[d][i] * inv), (f16)(o[d][i + 1] * inv)});
+      w[1] = as_u32((f16x2){(f16)(o[d][i + 2] * inv), (f16)(o[d][i + 3] * inv)});
+      const int chunk = (4 * d + i / 4) ^ k_swizzle<D>(r);
+      *reinterpret_cast<u32x2*>(mine + r * D + 8 * chunk + 4 * h) = w;
+    }
+#pragma unroll
+  for (int j = 0; j < 32 * D / 8 / kWave; ++j) {
+    const int x = j * kWave + lane, rr = x / (D / 8), chunk = x % (D / 8);
+    const uint32_t lo = from_lane((uint32_t)place, rr), hi = from_lane((uint32_t)(place >> 32), rr);
+    const u32x4 w = *reinterpret_cast<const u32x4*>(mine + rr * D + 8 * (chunk ^ k_swizzle<D>(rr)));
+    if (wave_row + rr < rows)
+      *reinterpret_cast<u32x4*>(a.out + (int64_t)(((uint64_t)hi << 32) | lo) + 8 * chunk) = w;
+  }
+}
+
+// A piece, by the waves of a workgroup.  THIN: a row block of up to 32 rows, which the waves
+// share: each takes half of the keys and half of the channels.
+template <int D, bool THIN>
+__device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh, uint16_t* k0, uint16_t* k1, uint16_t* v0, uint16_t* v1, Info& info) {
+  constexpr int DT = D / 32, KK = D / 16, ST = kKeys / 32, OB = THIN ? DT / 2 : DT;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 31, h = lane >> 5;
-  const int item = a.heads_kv.of(blockIdx.x), kvh = blockIdx.x - item * a.heads_kv.d;
-  Piece p;
-  {
-    const Seq own = seq_of(a, lane);
-    const Work w = work_of(a, own);
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.slots > 0) *a.plan = w;  // for the join
-    if (!piece_of<false>(a, own, w, item, p)) return;
-  }
-  const int rows = p.s.n * a.group.d, wave_row = p.block * kRows + wave * 32;
+  const int rows = p.s.n * a.group.d;
+  const int wave_row = p.block * kRows + (THIN ? 0 : wave * 32);
   const int row = wave_row + r, token = a.group.of(row), q_head = kvh * a.group.d + row - token * a.group.d;
   const bool real = row < rows;
   // the lane's row sees the keys up to `seen`, all of the wave's those up to `all_see`
@@ -406,10 +511,10 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
       if (real) qf[k] = *reinterpret_cast<const f16x8*>(from + 16 * k + 8 * h);
     }
   }
-  f32x16 o[DT];
+  f32x16 o[OB];
   float m = kNoMax, l = 0.0f;
 #pragma unroll
-  for (int d = 0; d < DT; ++d) o[d] = (f32x16)(0.0f);
+  for (int d = 0; d < OB; ++d) o[d] = (f32x16)(0.0f);
 
   typedef Tiles<D> T;
   T tiles(a, info, p, kvh, wave);
@@ -431,8 +536,10 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
 
   // Tile i of the piece from (kl, vl).  Between the products of the scores the next
   // tile's codes become fp16 in (kn, vn), and the loads of the one after take their
-  // registers.
+  // registers.  Of a thin row block a wave takes 32 of the keys and half of the channels.
   auto take = [&](int i, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
+    constexpr int SB = THIN ? 1 : ST, DB = THIN ? DT / 2 : DT, VN = DB < 4 ? DB : 4;  // VN: fragments of values read ahead
+    const int tb = THIN ? wave & 1 : 0;
     lds_barrier();
     if (i % 2 == 0) tiles.step(i);
     auto feed = [&](int j) {
@@ -446,17 +553,18 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
     // its 32: a lane holds 16 keys side by side, of one page.
     const int row_key = 16 * (r >> 2 & 1) + 4 * (r >> 3) + (r & 3);
     int from_k = row_key * D + 8 * (h ^ k_swizzle<D>(row_key)), from_v = r * kKeys + 8 * (2 * h ^ (r >> 1 & 7));
+    if (THIN) from_k += 32 * tb * D, from_v = (from_v ^ 32 * tb) + 32 * (wave >> 1) * DB * kKeys;
     asm volatile("" : "+v"(from_k), "+v"(from_v));
-    f32x16 s[ST];
+    f32x16 s[SB];
 #pragma unroll
-    for (int t = 0; t < ST; ++t) s[t] = (f32x16)(0.0f);
+    for (int t = 0; t < SB; ++t) s[t] = (f32x16)(0.0f);
     constexpr int CH = KK / 4;  // channel steps of a quarter
-    f16x8 kf[2][CH][ST];
+    f16x8 kf[2][CH][SB];
     auto read_k = [&](int q) {
 #pragma unroll
       for (int k = 0; k < CH; ++k)
 #pragma unroll
-        for (int t = 0; t < ST; ++t) {
+        for (int t = 0; t < SB; ++t) {
           kf[q & 1][k][t] = *reinterpret_cast<const f16x8*>(kl + 32 * t * D + (from_k ^ 16 * (q * CH + k) ^ (q * CH + k >= 8 ? 8 : 0)));
         }
     };
@@ -469,49 +577,49 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
 #pragma unroll
       for (int k = 0; k < CH; ++k)
 #pragma unroll
-        for (int t = 0; t < ST; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[q & 1][k][t], qf[q * CH + k], s[t], 0, 0, 0);
+        for (int t = 0; t < SB; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[q & 1][k][t], qf[q * CH + k], s[t], 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < 2 * T::N; ++j)
         if (j * 4 / (2 * T::N) == q) feed(j);
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
-    if constexpr (D == 256) {  // in vector registers from here, not brought there for each use
+    if constexpr (D == 256 && !THIN) {  // in vector registers from here, not brought there for each use
 #pragma unroll
-      for (int t = 0; t < ST; ++t) asm volatile("" : "+v"(s[t]));
+      for (int t = 0; t < SB; ++t) asm volatile("" : "+v"(s[t]));
     }
-    f32x4 say[ST];
+    f32x4 say[SB];
 #pragma unroll
-    for (int t = 0; t < ST; ++t) say[t] = info[i / kBatch & 1][place + 2 * t + h];
+    for (int t = 0; t < SB; ++t) say[t] = info[i / kBatch & 1][place + 2 * (tb + t) + h];
     const uint32_t held = (uint32_t)(tiles.held >> place) & 15, usual = (uint32_t)(tiles.usual >> place) & 15;
     const int past = seen - key - 16 * h;  // keys of the lane up to here are seen
     if (__builtin_expect(usual != 15, 0)) {
 #pragma unroll
-      for (int t = 0; t < ST; ++t) {
+      for (int t = 0; t < SB; ++t) {
         s[t] *= say[t][0];
         say[t][0] = 1.0f;
       }
     }
     if (key + kKeys - 1 > all_see || held != 15) {
 #pragma unroll
-      for (int t = 0; t < ST; ++t) {
-        const int last = held >> (2 * t + h) & 1 ? past - 32 * t : -1;
+      for (int t = 0; t < SB; ++t) {
+        const int last = held >> (2 * (tb + t) + h) & 1 ? past - 32 * (tb + t) : -1;
 #pragma unroll
         for (int x = 0; x < 16; ++x)
           if (x > last) s[t][x] = -__builtin_inff();
       }
     }
-    f16x8 vf[2][VN], pf[2 * ST];
+    f16x8 vf[2][VN], pf[2 * SB];
     auto read_v = [&](int c) {  // group c of fragments: of 16 tokens, or half their channels
 #pragma unroll
       for (int d = 0; d < VN; ++d)
-        vf[c & 1][d] = *reinterpret_cast<const f16x8*>(vl + 32 * (c * VN % DT + d) * kKeys + (from_v ^ 8 * (c * VN / DT / 2 * 4 + c * VN / DT % 2)));
+        vf[c & 1][d] = *reinterpret_cast<const f16x8*>(vl + 32 * (c * VN % DB + d) * kKeys + (from_v ^ 8 * (c * VN / DB / 2 * 4 + c * VN / DB % 2)));
     };
     float sum;
     auto weigh = [&]() {
       sum = 0.0f;
 #pragma unroll
-      for (int t = 0; t < ST; ++t) {
+      for (int t = 0; t < SB; ++t) {
         const float lift = say[t][1] + kLift - m;
         float part = 0.0f;
 #pragma unroll
@@ -526,7 +634,7 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
     auto highest = [&]() {
       float up = kNoMax;
 #pragma unroll
-      for (int t = 0; t < ST; ++t) {
+      for (int t = 0; t < SB; ++t) {
         float x = s[t][0];
 #pragma unroll
         for (int y = 1; y < 16; ++y) x = __builtin_fmaxf(x, s[t][y]);
@@ -542,11 +650,11 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
       m = up;
       l *= f;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= f;
-      stay_in_accumulators<D>(o);
+      for (int d = 0; d < DB; ++d) o[d] *= f;
+      if constexpr (!THIN) stay_in_accumulators<D>(o);
     };
-    stay_in_accumulators<D>(o);
-    if constexpr (D == 256) {
+    if constexpr (!THIN) stay_in_accumulators<D>(o);
+    if constexpr (D == 256 && !THIN) {
       // the scores beside their weights do not fit the registers
       const float up = highest();
       if (__any(up > m + kSlack)) raise(up);
@@ -556,7 +664,7 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
       weigh();
       f16x8 top = pf[0];
 #pragma unroll
-      for (int g = 1; g < 4; ++g) top = __builtin_elementwise_max(top, pf[g]);
+      for (int g = 1; g < 2 * SB; ++g) top = __builtin_elementwise_max(top, pf[g]);
       const f16x4 top4 = __builtin_elementwise_max(__builtin_shufflevector(top, top, 0, 1, 2, 3), __builtin_shufflevector(top, top, 4, 5, 6, 7));
       const f16x2 top2 = __builtin_elementwise_max(__builtin_shufflevector(top4, top4, 0, 1), __builtin_shufflevector(top4, top4, 2, 3));
       if (__any(top2[0] > (f16)kMost || top2[1] > (f16)kMost)) {
@@ -568,8 +676,8 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
     read_v(0);
     if (__builtin_expect(usual != 15, 0)) {
 #pragma unroll
-      for (int t = 0; t < ST; ++t) {
-        const int last = held >> (2 * t + h) & 1 ? past - 32 * t : -1;
+      for (int t = 0; t < SB; ++t) {
+        const int last = held >> (2 * (tb + t) + h) & 1 ? past - 32 * (tb + t) : -1;
         // a key that is not seen has no weight, and none of a scale that is not finite either
 #pragma unroll
         for (int x = 0; x < 16; ++x) pf[2 * t + x / 8][x % 8] = x > last ? (f16)0.0f : pf[2 * t + x / 8][x % 8] * (f16)say[t][3];
@@ -577,18 +685,18 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
     }
     __builtin_amdgcn_s_setprio(2);
 #pragma unroll
-    for (int c = 0; c < 2 * ST * DT / VN; ++c) {
-      if (c + 1 < 2 * ST * DT / VN) read_v(c + 1);
+    for (int c = 0; c < 2 * SB * DB / VN; ++c) {
+      if (c + 1 < 2 * SB * DB / VN) read_v(c + 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int d = 0; d < VN; ++d) {
-        f32x16& to = o[c * VN % DT + d];
-        to = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c & 1][d], pf[c * VN / DT], to, 0, 0, 0);
+        f32x16& to = o[c * VN % DB + d];
+        to = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c & 1][d], pf[c * VN / DB], to, 0, 0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  if (wave_row >= rows) {
+  if (!THIN && wave_row >= rows) {
     // a wave without rows brings the tiles for the others
     auto bring = [&](int i, uint16_t* kn, uint16_t* vn) {
       lds_barrier();
@@ -607,52 +715,33 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
     for (int i = 0; i < count; i += 2) {
       take(i, k0, v0, k1, v1);
       if (i + 1 < count) take(i + 1, k1, v1, k0, v0);
-      stay_in_accumulators<D>(o);
+      if constexpr (!THIN) stay_in_accumulators<D>(o);
     }
   }
 
   l += from_lane(l, lane ^ 32);
-  if (p.pieces > 1) {
-    const int slot = p.slot * a.heads_kv.d + kvh;
-    if (slot >= a.slots) return;
-    float* part = a.parts + (int64_t)slot * kPartFloats<D>;
-    if (real) {
-      if (h == 0) part[wave * 32 + r] = m, part[kRows + wave * 32 + r] = l;
-      f32x4* to = reinterpret_cast<f32x4*>(part + 2 * kRows + wave * 32 * D) + lane;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          to[(4 * d + i) * kWave] = (f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-    }
-    return;
+  if constexpr (THIN) {
+    finish_thin<D>(a, p, kvh, wave, lane, o, m, l, wave < 2 ? k0 : k1, reinterpret_cast<float*>(v0), v1);
+  } else {
+    finish<D>(a, p, kvh, wave, lane, o, m, l, wave < 2 ? (wave == 0 ? k0 : k1) : (wave == 2 ? v0 : v1));
   }
-  // the rows leave through LDS, a wave's 32 x D in an array that no wave reads any more
-  lds_barrier();
-  uint16_t* mine = wave < 2 ? (wave == 0 ? k0 : k1) : (wave == 2 ? v0 : v1);
-  const float inv = l > 0.0f ? __builtin_exp2f(-kLift) / l : l == 0.0f ? 0.0f : l;
-  int again = wave_row + r;  // the row's place once more: kept over the loop it would take registers
-  asm volatile("" : "+v"(again));
-  const int to_token = a.group.of(again), to_head = kvh * a.group.d + again - to_token * a.group.d;
-  const int64_t place = (int64_t)(p.s.first + to_token) * a.o_token + (int64_t)to_head * a.o_head;
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      u32x2 w;
-      w[0] = as_u32((f16x2){(f16)(o[d][i] * inv), (f16)(o[d][i + 1] * inv)});
-      w[1] = as_u32((f16x2){(f16)(o[d][i + 2] * inv), (f16)(o[d][i + 3] * inv)});
-      const int chunk = (4 * d + i / 4) ^ k_swizzle<D>(r);
-      *reinterpret_cast<u32x2*>(mine + r * D + 8 * chunk + 4 * h) = w;
-    }
-#pragma unroll
-  for (int j = 0; j < 32 * D / 8 / kWave; ++j) {
-    const int x = j * kWave + lane, rr = x / (D / 8), chunk = x % (D / 8);
-    const uint32_t lo = from_lane((uint32_t)place, rr), hi = from_lane((uint32_t)(place >> 32), rr);
-    const u32x4 w = *reinterpret_cast<const u32x4*>(mine + rr * D + 8 * (chunk ^ k_swizzle<D>(rr)));
-    if (wave_row + rr < rows)
-      *reinterpret_cast<u32x4*>(a.out + (int64_t)(((uint64_t)hi << 32) | lo) + 8 * chunk) = w;
+}
+
+template <int D>
+__global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(ChunkArgs a) {
+  // four arrays and not one: reads of a tile then need not wait for writes of the next
+  __shared__ __align__(16) uint16_t k0[kKeys * D], k1[kKeys * D], v0[kKeys * D], v1[kKeys * D];
+  __shared__ Info info;
+  const int item = a.heads_kv.of(blockIdx.x), kvh = blockIdx.x - item * a.heads_kv.d;
+  Piece p;
+  {
+    const Seq own = seq_of(a, lane_id());
+    const Work w = work_of(a, own);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.slots > 0) *a.plan = w;  // for the join
+    if (!piece_of<false>(a, own, w, item, p)) return;
   }
+  if (p.s.n * a.group.d - p.block * kRows <= 32) run<D, true>(a, p, kvh, k0, k1, v0, v1, info);
+  else run<D, false>(a, p, kvh, k0, k1, v0, v1, info);
 }
 
 // Joins the parts of the row blocks that were cut: 32 rows and 32 channels a

@@ -13,6 +13,8 @@
 // key/value head.  Four waves of 32 rows go through tiles of 64 keys together: the
 // codes of a tile come into registers while the tile before is computed, become fp16
 // (exactly) and lie in LDS for all four.
+#include <type_traits>
+
 #include "attn_common.hpp"
 
 namespace lb {
@@ -270,8 +272,8 @@ __device__ __forceinline__ int k_swizzle(int key) {
 constexpr int kBatch = 16;
 typedef f32x4 Info[2][kBatch * 4];
 
-// The tiles of a piece on their way: pages and scales a batch ahead, codes a tile ahead.
-template <int D>
+// The tiles of a piece on their way: pages and scales a batch ahead, codes DEPTH tiles.
+template <int D, int DEPTH>
 struct Tiles {
   static constexpr int N = D / 64;  // loads of keys (and of values) of a thread and tile
   const ChunkArgs& a;
@@ -282,10 +284,12 @@ struct Tiles {
   int per, in;    // channels of a load of values, loads of all channels
   uint32_t k_off, v_off;  // the thread's place in a load
   int k_lds, v_lds[N];    // and in LDS
-  int cell, next_cell, page;  // page and head: of the batch whose codes are loaded, of the next; page of the one after
+  uint32_t k_at[2], v_at[2];  // lane l: where the codes of its 16 tokens are, of the batch that is loaded
+  int cell, page;             // page and head, of the next batch; page of the one after
   float ks, vs;               // scales of the next batch
-  uint64_t held, usual, next_held, next_usual;  // bit l: page there; scales finite, above zero, inside the range
-  u32x4 codes[2 * N];
+  uint64_t held, odd, next_held, next_odd;  // bit l: page there; scales not finite, not above zero or outside the range
+  uint64_t strange;                         // bit 4 i: tile i has a group without a page, or odd
+  u32x4 codes[DEPTH][2 * N];
 
   __device__ __forceinline__ Tiles(const ChunkArgs& args, Info& shared, const Piece& p, int kv_head, int w)
       : a(args), info(shared), head(kv_head), len(p.s.len), first(p.t0), lane(lane_id()), wave(w) {
@@ -307,8 +311,8 @@ struct Tiles {
   __device__ __forceinline__ void load_scales(int batch) {
     const bool real = token(batch) < len && (unsigned)page < (unsigned)a.num_pages;
     next_held = __ballot(real);
-    next_cell = (real ? page : 0) * a.heads_kv.d + head;
-    ks = a.k_scale[next_cell], vs = a.v_scale[next_cell];
+    cell = (real ? page : 0) * a.heads_kv.d + head;
+    ks = a.k_scale[cell], vs = a.v_scale[cell];
   }
   __device__ __forceinline__ void tell(int batch) {
     const bool real = next_held >> lane & 1;
@@ -316,40 +320,50 @@ struct Tiles {
     // a scale of infinity has no scores: ks - ks makes it NaN and is zero otherwise
     const float k = real ? ks * a.scale + (ks - ks) : 1.0f;
     const float lg = __builtin_fmaxf(__builtin_fminf(__builtin_amdgcn_logf(__builtin_fabsf(v)), kScales), -kScales);
-    next_usual = __ballot(k > 0.0f && k < __builtin_inff() && v > 0.0f && __builtin_fabsf(lg) < kScales);
+    next_odd = __ballot(!(k > 0.0f && k < __builtin_inff() && v > 0.0f && __builtin_fabsf(lg) < kScales));
     if (lane / kBatch == wave) info[batch & 1][lane] = (f32x4){k, lg, __builtin_amdgcn_exp2f(-lg - kLift), v * __builtin_amdgcn_exp2f(-lg)};
   }
-  __device__ __forceinline__ void turn() { held = next_held, usual = next_usual; }
-  // Tile i of the piece is about to be computed, the loads of tile i + 2 to be sent off
-  // (i even).  A batch's places are written at least a barrier after their last readers.
+  __device__ __forceinline__ void turn() {
+    held = next_held, odd = next_odd;
+    strange = ~held | odd;
+    strange |= strange >> 1;
+    strange |= strange >> 2;
+  }
+  __device__ __forceinline__ void locate(int batch) {
+    const int in_page = token(batch) & ((1 << a.page_shift) - 1);
+    const uint64_t k = (uint64_t)(uintptr_t)a.k_cache + (uint64_t)((((int64_t)cell << a.page_shift) + in_page) * D);
+    const uint64_t v = (uint64_t)(uintptr_t)a.v_cache + (uint64_t)(((int64_t)cell * D << a.page_shift) + in_page);
+    k_at[0] = (uint32_t)k, k_at[1] = (uint32_t)(k >> 32), v_at[0] = (uint32_t)v, v_at[1] = (uint32_t)(v >> 32);
+  }
+  // Tile i of the piece is about to be computed, the loads of tile i + 1 + DEPTH to be sent
+  // off.  A batch's places in LDS are written at least a barrier after their last readers.
   __device__ __forceinline__ void step(int i) {
     const int c = i % kBatch, batch = i / kBatch;
+    if (c == kBatch - 1 - DEPTH) locate(batch + 1);
+    if (i % 2) return;
     if (c == 0 && i > 0) turn();
     else if (c == 2) load_scales(batch + 1);
     else if (c == 8) tell(batch + 1);
-    else if (c == 10) load_pages(batch + 2);
-    else if (c == kBatch - 2) cell = next_cell;
+  }
+  // After the last use of the pages' numbers: the batch after the next one's.
+  __device__ __forceinline__ void step_after(int i) {
+    if (i % kBatch == 4) load_pages(i / kBatch + 2);
   }
   // Load j of tile i: of its keys, then of its values; none of one that is not `real`.
-  __device__ __forceinline__ void load(int j, int i, bool real) {
-    const int mask = (1 << a.page_shift) - 1, at_lane = i % kBatch * 4, token = (first + i) * kKeys;
+  __device__ __forceinline__ void load(int set, int j, int i, bool real) {
+    const int at_lane = i % kBatch * 4;
+    const int y = (j - N) * kWaves + wave;
+    const int l = at_lane + (j < N ? (j * kWaves + wave) * (kWave * 16 / D) / 16 : y / in << groups);  // the load's 16 tokens
+    const uint32_t* at = j < N ? k_at : v_at;
+    const uint64_t base = (uint32_t)__builtin_amdgcn_readlane(at[0], l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at[1], l) << 32;
     const uint32_t bytes = real ? (uint32_t)D << a.page_shift : 0u;
-    if (j < N) {
-      const int g = (j * kWaves + wave) * (kWave * 16 / D) / 16;  // the load's 16 tokens
-      const int64_t c = __builtin_amdgcn_readlane(cell, at_lane + g);
-      const uint32_t at = (uint32_t)((token + 16 * g) & mask) * D;
-      codes[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer_of(a.k_cache + (c << a.page_shift) * D, bytes), k_off, at, 0));
-    } else {
-      const int y = (j - N) * kWaves + wave, g = y / in << groups;
-      const int64_t c = __builtin_amdgcn_readlane(cell, at_lane + g);
-      const uint32_t at = ((uint32_t)(((j - N) * kWaves % in) * per) << a.page_shift) + ((token + 16 * g) & mask);
-      codes[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer_of(a.v_cache + ((c * D) << a.page_shift), bytes), v_off, at, 0));
-    }
+    codes[set][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+        buffer_of(reinterpret_cast<const void*>(base), bytes), j < N ? k_off : v_off, j < N ? 0 : ((j - N) * kWaves % in * per) << a.page_shift, 0));
   }
   // As fp16 into LDS: keys [token][channel], values [channel][token].
-  __device__ __forceinline__ void store(int j, uint16_t* kl, uint16_t* vl) const {
+  __device__ __forceinline__ void store(int set, int j, uint16_t* kl, uint16_t* vl) const {
     f16x8 x, y;
-    codes_to_half(codes[j], x, y);
+    codes_to_half(codes[set][j], x, y);
     if (j < N) {
       constexpr int kRowStep = kWaves * kWave / (D / 16);
       static_assert(N == 1 || kRowStep == 32 || kRowStep == 16, "the rows of a thread's loads change places alike, or as 16 says");
@@ -516,35 +530,43 @@ __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh,
 #pragma unroll
   for (int d = 0; d < OB; ++d) o[d] = (f32x16)(0.0f);
 
-  typedef Tiles<D> T;
+  // a thin block's tile is done before the next one's codes can arrive; it has registers
+  // to spare
+  constexpr int DEPTH = THIN ? 2 : 1;
+  typedef Tiles<D, DEPTH> T;
   T tiles(a, info, p, kvh, wave);
   const int count = p.t1 - p.t0;
   if (count > 0) {
     tiles.load_pages(0);
     tiles.load_scales(0);
-    tiles.cell = tiles.next_cell;
+    tiles.locate(0);
     tiles.load_pages(1);
 #pragma unroll
-    for (int j = 0; j < 2 * T::N; ++j) tiles.load(j, 0, true);
+    for (int j = 0; j < 2 * T::N; ++j) tiles.load(0, j, 0, true);
+#pragma unroll
+    for (int j = 0; j < 2 * T::N; ++j)
+      if (DEPTH == 2) tiles.load(DEPTH - 1, j, 1, 1 < count);
     tiles.tell(0);
     tiles.turn();
 #pragma unroll
-    for (int j = 0; j < 2 * T::N; ++j) tiles.store(j, k0, v0);
+    for (int j = 0; j < 2 * T::N; ++j) tiles.store(0, j, k0, v0);
 #pragma unroll
-    for (int j = 0; j < 2 * T::N; ++j) tiles.load(j, 1, 1 < count);
+    for (int j = 0; j < 2 * T::N; ++j) tiles.load(0, j, DEPTH, DEPTH < count);
   }
 
   // Tile i of the piece from (kl, vl).  Between the products of the scores the next
   // tile's codes become fp16 in (kn, vn), and the loads of the one after take their
   // registers.  Of a thin row block a wave takes 32 of the keys and half of the channels.
-  auto take = [&](int i, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
+  auto take = [&](int i, auto parity, const uint16_t* kl, const uint16_t* vl, uint16_t* kn, uint16_t* vn) {
     constexpr int SB = THIN ? 1 : ST, DB = THIN ? DT / 2 : DT, VN = DB < 4 ? DB : 4;  // VN: fragments of values read ahead
     const int tb = THIN ? wave & 1 : 0;
+    constexpr int next = DEPTH == 1 ? 0 : 1 - decltype(parity)::value;  // the registers of tile i + 1, and of i + 1 + DEPTH
     lds_barrier();
-    if (i % 2 == 0) tiles.step(i);
+    tiles.step(i);
+    const bool more = i + 1 + DEPTH < count;
     auto feed = [&](int j) {
-      tiles.store(j, kn, vn);
-      tiles.load(j, i + 2, i + 2 < count);
+      tiles.store(next, j, kn, vn);
+      tiles.load(next, j, i + 1 + DEPTH, more);
     };
     const int place = i % kBatch * 4;
     const int key = (p.t0 + i) * kKeys;
@@ -591,18 +613,13 @@ __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh,
     f32x4 say[SB];
 #pragma unroll
     for (int t = 0; t < SB; ++t) say[t] = info[i / kBatch & 1][place + 2 * (tb + t) + h];
-    const uint32_t held = (uint32_t)(tiles.held >> place) & 15, usual = (uint32_t)(tiles.usual >> place) & 15;
     const int past = seen - key - 16 * h;  // keys of the lane up to here are seen
-    if (__builtin_expect(usual != 15, 0)) {
+    const bool strange = tiles.strange >> place & 1;
+    if (__builtin_expect(strange || key + kKeys - 1 > all_see, 0)) {
+      const uint32_t held = (uint32_t)(tiles.held >> place) & 15, odd = (uint32_t)(tiles.odd >> place) & 15;
 #pragma unroll
       for (int t = 0; t < SB; ++t) {
-        s[t] *= say[t][0];
-        say[t][0] = 1.0f;
-      }
-    }
-    if (key + kKeys - 1 > all_see || held != 15) {
-#pragma unroll
-      for (int t = 0; t < SB; ++t) {
+        if (odd) s[t] *= say[t][0], say[t][0] = 1.0f;
         const int last = held >> (2 * (tb + t) + h) & 1 ? past - 32 * (tb + t) : -1;
 #pragma unroll
         for (int x = 0; x < 16; ++x)
@@ -674,7 +691,8 @@ __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh,
     }
     l += sum;
     read_v(0);
-    if (__builtin_expect(usual != 15, 0)) {
+    if (__builtin_expect(strange, 0)) {
+      const uint32_t held = (uint32_t)(tiles.held >> place) & 15;
 #pragma unroll
       for (int t = 0; t < SB; ++t) {
         const int last = held >> (2 * (tb + t) + h) & 1 ? past - 32 * (tb + t) : -1;
@@ -695,17 +713,19 @@ __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh,
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    tiles.step_after(i);
   };
   if (!THIN && wave_row >= rows) {
     // a wave without rows brings the tiles for the others
     auto bring = [&](int i, uint16_t* kn, uint16_t* vn) {
       lds_barrier();
-      if (i % 2 == 0) tiles.step(i);
+      tiles.step(i);
 #pragma unroll
       for (int j = 0; j < 2 * T::N; ++j) {
-        tiles.store(j, kn, vn);
-        tiles.load(j, i + 2, i + 2 < count);
+        tiles.store(0, j, kn, vn);
+        tiles.load(0, j, i + 2, i + 2 < count);
       }
+      tiles.step_after(i);
     };
     for (int i = 0; i < count; i += 2) {
       bring(i, k1, v1);
@@ -713,9 +733,14 @@ __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh,
     }
   } else {
     for (int i = 0; i < count; i += 2) {
-      take(i, k0, v0, k1, v1);
-      if (i + 1 < count) take(i + 1, k1, v1, k0, v0);
-      if constexpr (!THIN) stay_in_accumulators<D>(o);
+      take(i, std::integral_constant<int, 0>(), k0, v0, k1, v1);
+      if (i + 1 < count) take(i + 1, std::integral_constant<int, 1>(), k1, v1, k0, v0);
+      if constexpr (!THIN) {
+        stay_in_accumulators<D>(o);
+        if constexpr (D == 256)  // and the queries, so that the codes need not be brought from there
+#pragma unroll
+          for (int k = 0; k < KK; ++k) asm volatile("" : "+a"(qf[k]));
+      }
     }
   }
 

@@ -16,15 +16,18 @@ namespace {
 struct Pages {
   int32_t *table, *lens, *refs;
   int64_t stride;
-  int rows, width, pages, page_size;
+  int rows, width, pages, shift;  // shift: log2 of a page's tokens
 };
 
 // Rows of one call: a workgroup goes through all of them.
 constexpr int kMaxRows = 4096;
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / kWave;
 constexpr int kEach = kMaxRows / kPlanThreads;
+constexpr int kClaims = 8192;  // rows of a table in which a row's first mention is found by its number, not by a search
 
-__device__ __forceinline__ int pages_of(int tokens, int page_size) { return (int)(((int64_t)tokens + page_size - 1) / page_size); }
+// Pages of `tokens` (not below 0).
+__device__ __forceinline__ int pages_of(int tokens, const Pages& p) { return (int)(((uint32_t)tokens + (1u << p.shift) - 1) >> p.shift); }
+__device__ __forceinline__ int64_t capacity(const Pages& p) { return (int64_t)p.width << p.shift; }
 
 // Exclusive prefix sum over the workgroup's threads; `total` of all.
 __device__ __forceinline__ int block_scan(int v, int* lds, int& total) {
@@ -46,7 +49,7 @@ __global__ __launch_bounds__(256) void free_kernel(Pages p, const int32_t* rows,
   const int i = blockIdx.x, row = rows[i];
   if ((unsigned)row >= (unsigned)p.rows) return;
   const int tokens = keep ? max(keep[i], 0) : 0;
-  const int first = max(pages_of(tokens, p.page_size), (int)blockIdx.y * kFreeCols), last = min(p.width, ((int)blockIdx.y + 1) * kFreeCols);
+  const int first = max(pages_of(tokens, p), (int)blockIdx.y * kFreeCols), last = min(p.width, ((int)blockIdx.y + 1) * kFreeCols);
   int32_t* mine = p.table + (int64_t)row * p.stride;
   for (int c = first + threadIdx.x; c < last; c += 256) {
     if (mine[c] < 0) continue;
@@ -65,7 +68,7 @@ __device__ __forceinline__ int forked(const Pages& p, const int32_t* parents, co
   const int parent = parents[i], child = children[i];
   if ((unsigned)parent >= (unsigned)p.rows || (unsigned)child >= (unsigned)p.rows || named || p.lens[child] > 0) return -1;
   int n = min(max(p.lens[parent], 0), lens ? max(lens[i], 0) : 0x7fffffff);
-  return (int)min((int64_t)n, (int64_t)p.width * p.page_size);
+  return (int)min((int64_t)n, capacity(p));
 }
 
 __global__ __launch_bounds__(256) void fork_kernel(Pages p, const int32_t* parents, const int32_t* children, const int32_t* lens) {
@@ -76,7 +79,7 @@ __global__ __launch_bounds__(256) void fork_kernel(Pages p, const int32_t* paren
   if (n <= 0) return;
   const int32_t* from = p.table + (int64_t)parents[i] * p.stride;
   int32_t* to = p.table + (int64_t)child * p.stride;
-  const int first = blockIdx.y * kFreeCols, last = min(pages_of(n, p.page_size), first + kFreeCols);
+  const int first = blockIdx.y * kFreeCols, last = min(pages_of(n, p), first + kFreeCols);
   for (int c = first + threadIdx.x; c < last; c += 256) {
     const int page = from[c];
     const bool real = (unsigned)page < (unsigned)p.pages;
@@ -88,17 +91,27 @@ __global__ __launch_bounds__(256) void fork_kernel(Pages p, const int32_t* paren
 // The children's lengths, once their tables are written (which goes by the old ones).
 __global__ __launch_bounds__(kPlanThreads) void fork_lens_kernel(Pages p, const int32_t* parents, const int32_t* children, const int32_t* lens,
                                                                 int32_t* done, int count) {
-  __shared__ int32_t names[kMaxRows];
-  for (int i = threadIdx.x; i < count; i += kPlanThreads) names[i] = children[i];
-  __syncthreads();
+  __shared__ int32_t names[kMaxRows], claims[kClaims];
   int n[kEach];
+  const bool few = p.rows <= kClaims;
+  for (int i = threadIdx.x; i < count; i += kPlanThreads) {
+    names[i] = children[i];
+    if (few && (unsigned)names[i] < (unsigned)p.rows) claims[names[i]] = 0x7fffffff;
+  }
+  __syncthreads();
+  if (few)
+    for (int i = threadIdx.x; i < count; i += kPlanThreads)
+      if ((unsigned)names[i] < (unsigned)p.rows) atomicMin(&claims[names[i]], i);
+  __syncthreads();
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const int i = e * kPlanThreads + threadIdx.x;
     n[e] = -1;
-    if (i >= count) continue;
+    if (i >= count || (unsigned)names[i] >= (unsigned)p.rows) continue;
     bool named = false;
-    for (int j = 0; j < i; ++j) named |= names[j] == names[i];
+    if (few) named = claims[names[i]] != i;
+    else
+      for (int j = 0; j < i; ++j) named |= names[j] == names[i];
     n[e] = forked(p, parents, children, lens, i, named);
   }
   __syncthreads();
@@ -137,45 +150,65 @@ struct Held {
 };
 constexpr int kLook = 16 * kPlanThreads;  // pages looked at together
 
+constexpr int kFresh = 4096;   // new pages that stay in LDS
+
 __global__ __launch_bounds__(kPlanThreads) void extend_kernel(Pages p, const int32_t* rows, const int32_t* add, int32_t* status, int count, int layers,
-                                                             Copies* copies, int32_t* fresh) {
-  __shared__ int32_t names[kMaxRows], shared_page[kMaxRows], before[kMaxRows + 1];
+                                                             Copies* copies, int32_t* many) {
+  __shared__ int32_t names[kMaxRows], shared_page[kMaxRows], before[kMaxRows + 1], claims[kClaims];
   __shared__ int lds[kPlanWaves];
   const int each = (count + kPlanThreads - 1) / kPlanThreads;  // consecutive rows of a thread
   const int i0 = threadIdx.x * each;
+  int need[kEach], tail[kEach], name[kEach], more[kEach], holders[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = i0 + e;
+    need[e] = 0, tail[e] = -1, name[e] = -1, more[e] = 0, holders[e] = 0;
+    if (e < each && i < count) name[e] = rows[i], more[e] = max(add[i], 0);
+  }
   Held held;
   held.load(p, (int64_t)threadIdx.x * 16);
-  for (int i = threadIdx.x; i < count; i += kPlanThreads) names[i] = rows[i];
+  const bool few = p.rows <= kClaims;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (e >= each || i0 + e >= count) continue;
+    names[i0 + e] = name[e], shared_page[i0 + e] = -1;
+    if (few && (unsigned)name[e] < (unsigned)p.rows) claims[name[e]] = 0x7fffffff;
+  }
   __syncthreads();
-  int need[kEach], tail[kEach];
+  if (few) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (e < each && i0 + e < count && (unsigned)name[e] < (unsigned)p.rows) atomicMin(&claims[name[e]], i0 + e);
+    __syncthreads();
+  }
   bool too_long = false, any_shared = false;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    need[e] = 0, tail[e] = -1;
-    const int i = i0 + e;
-    if (e >= each || i >= count) continue;
-    shared_page[i] = -1;
-    const int row = names[i], n = max(add[i], 0);
-    if ((unsigned)row >= (unsigned)p.rows || n == 0) continue;
+    const int i = i0 + e, row = name[e];
+    if (e >= each || i >= count || (unsigned)row >= (unsigned)p.rows || more[e] == 0) continue;
     bool again = false;
-    for (int j = 0; j < i; ++j) again |= names[j] == row;
+    if (few) again = claims[row] != i;
+    else
+      for (int j = 0; j < i; ++j) again |= names[j] == row;
     if (again) continue;
     const int len = max(p.lens[row], 0);
-    const int64_t now = (int64_t)len + n;
-    if (now > (int64_t)p.width * p.page_size) {
+    const int64_t now = (int64_t)len + more[e];
+    if (now > capacity(p)) {
       too_long = true;
       continue;
     }
-    need[e] = pages_of((int)now, p.page_size) - pages_of(len, p.page_size);
+    need[e] = pages_of((int)now, p) - pages_of(len, p);
     tail[e] = len;
-    if (len % p.page_size) {
-      const int page = p.table[(int64_t)row * p.stride + len / p.page_size];
-      if ((unsigned)page < (unsigned)p.pages && p.refs[page] > 1) shared_page[i] = page, any_shared = true;
+    if (len & ((1 << p.shift) - 1)) {
+      const int page = p.table[(int64_t)row * p.stride + (len >> p.shift)];
+      if ((unsigned)page < (unsigned)p.pages) holders[e] = p.refs[page];
+      if (holders[e] > 1) shared_page[i] = page, any_shared = true;
     }
   }
   too_long = __syncthreads_or(too_long);
+  any_shared = __syncthreads_or(any_shared);
   int copied = 0;  // bit e
-  if (__syncthreads_or(any_shared)) {
+  if (any_shared) {
     // all but the last of a page's holders take a copy
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
@@ -183,7 +216,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_kernel(Pages p, const int
       if (e >= each || i >= count || shared_page[i] < 0) continue;
       int rank = 0;
       for (int j = 0; j < i; ++j) rank += shared_page[j] == shared_page[i];
-      if (rank < p.refs[shared_page[i]] - 1) copied |= 1 << e;
+      if (rank < holders[e] - 1) copied |= 1 << e;
     }
   }
   int sum = 0;
@@ -192,16 +225,17 @@ __global__ __launch_bounds__(kPlanThreads) void extend_kernel(Pages p, const int
     need[e] += copied >> e & 1;
     sum += need[e];
   }
-  int total, all_copies;
-  int at = block_scan(sum, lds, total);
-  int copy_at = block_scan(__builtin_popcount(copied), lds, all_copies);
+  int total, all_copies = 0;
+  int at = block_scan(sum, lds, total), copy_at = 0;
+  if (any_shared) copy_at = block_scan(__builtin_popcount(copied), lds, all_copies);
 #pragma unroll
   for (int e = 0; e < kEach; ++e)
     if (e < each && i0 + e < count) {
       before[i0 + e] = at | (copied >> e & 1) << 31;
       at += need[e];
     }
-  // the lowest free pages
+  // the lowest free pages; the claims are read no more
+  int32_t* fresh = total <= kFresh ? claims : many;
   int found = 0;
   for (int64_t base = 0; found < total && base < p.pages; base += kLook) {
     const Held now = held;
@@ -211,12 +245,14 @@ __global__ __launch_bounds__(kPlanThreads) void extend_kernel(Pages p, const int
     for (int j = 0; j < 16; ++j) n += !now.is(j);
     int rank = found + block_scan(n, lds, all);
     found += all;
+    if (rank < total) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (!now.is(j)) {
-        if (rank < total) fresh[rank] = (int32_t)(base + threadIdx.x * 16 + j);
-        ++rank;
-      }
+      for (int j = 0; j < 16; ++j)
+        if (!now.is(j)) {
+          if (rank < total) fresh[rank] = (int32_t)(base + threadIdx.x * 16 + j);
+          ++rank;
+        }
+    }
   }
   const int say = too_long ? -1 : all_copies && !layers ? -2 : max(total - found, 0);
   if (threadIdx.x == 0) *status = say, copies->count = say ? 0 : all_copies;
@@ -226,18 +262,16 @@ __global__ __launch_bounds__(kPlanThreads) void extend_kernel(Pages p, const int
   for (int e = 0; e < kEach; ++e) {
     const int i = i0 + e;
     if (e >= each || i >= count || tail[e] < 0) continue;
-    const int row = names[i];
     if (copied >> e & 1) {
       const int to = fresh[before[i] & 0x7fffffff], from = shared_page[i];
       copies->src[copy_at] = from, copies->dst[copy_at] = to;
       ++copy_at;
-      p.table[(int64_t)row * p.stride + tail[e] / p.page_size] = to;
+      p.table[(int64_t)name[e] * p.stride + (tail[e] >> p.shift)] = to;
       p.refs[to] = 1;
       __hip_atomic_fetch_add(p.refs + from, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    names[i] = pages_of(tail[e], p.page_size) - (copied >> e & 1);  // the column of its first page
-    shared_page[i] = row;
-    p.lens[row] = tail[e] + max(add[i], 0);
+    shared_page[i] = pages_of(tail[e], p) - (copied >> e & 1);  // the column of its first page
+    p.lens[name[e]] = tail[e] + more[e];
   }
   __syncthreads();
   for (int k = threadIdx.x; k < total; k += kPlanThreads) {
@@ -249,7 +283,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_kernel(Pages p, const int
     const int at = k - (before[lo] & 0x7fffffff);
     if (before[lo] < 0 && at == 0) continue;  // the copy
     const int page = fresh[k];
-    p.table[(int64_t)shared_page[lo] * p.stride + names[lo] + at] = page;
+    p.table[(int64_t)names[lo] * p.stride + shared_page[lo] + at] = page;
     p.refs[page] = 1;
   }
 }
@@ -401,7 +435,8 @@ int check_pages(const int32_t* table, int64_t rows, int64_t max_pages, int64_t s
 Pages pages_at(int32_t* table, int64_t rows, int64_t max_pages, int64_t stride, int32_t* lens, int32_t* refs, int64_t num_pages, int64_t page_size) {
   Pages p;
   p.table = table, p.lens = lens, p.refs = refs, p.stride = stride;
-  p.rows = (int)rows, p.width = (int)max_pages, p.pages = (int)num_pages, p.page_size = (int)page_size;
+  p.rows = (int)rows, p.width = (int)max_pages, p.pages = (int)num_pages;
+  p.shift = page_size > 0 ? __builtin_ctzll((unsigned long long)page_size) : 0;
   return p;
 }
 

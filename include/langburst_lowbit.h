@@ -325,8 +325,9 @@ int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_s
  * one that sees none (padding before position 0) is zero, and rows of tokens that
  * belong to no sequence are left as they are.  Scores, softmax and sums are fp32;
  * a weight times its value scale enters the second product as one fp16 number
- * (2^-11, and 2^-32 of the row's largest; value scales from 2^-80 to 2^80).  A
- * page's scale that is not finite reaches the rows that see a token of the page.
+ * (2^-11, and 2^-32 of the row's largest; value scales of any size up to 2^32, and
+ * fp16 values give 2^9 at most).  A page's scale that is not finite reaches the rows
+ * that see a token of the page.
  * One launch, or a second one that joins the parts of rows whose keys were cut,
  * which tables of more than a few hundred tokens take.  scratch:
  * lb_kv8_chunk_attention_scratch_bytes() bytes, 16-byte aligned, no

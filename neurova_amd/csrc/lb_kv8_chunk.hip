@@ -93,6 +93,26 @@ __device__ __forceinline__ int tiles_of(const Seq& s) { return max((s.len + kKey
 __device__ __forceinline__ int pieces_in(int tiles, int most, float inverse) {
   return (int)(((float)(tiles + most - 1) + 0.5f) * inverse);
 }
+// Up to kSorted sequences' row blocks and tiles stay in registers, lane l those of sequence
+// 64 c + l.
+constexpr int kChunks = 4, kSorted = kChunks * kWave;
+struct Sizes {
+  Seq own;  // of the first 64
+  int blocks[kChunks], tiles[kChunks];
+};
+__device__ __forceinline__ Sizes sizes_of(const ChunkArgs& a) {
+  Sizes z;
+  z.own = seq_of(a, lane_id());
+  z.blocks[0] = blocks_of(a, z.own), z.tiles[0] = tiles_of(z.own);
+#pragma unroll
+  for (int c = 1; c < kChunks; ++c) {
+    z.blocks[c] = 0, z.tiles[c] = 1;
+    if (c * kWave >= a.batch || a.batch > kSorted) continue;
+    const Seq s = seq_of(a, c * kWave + lane_id());
+    z.blocks[c] = blocks_of(a, s), z.tiles[c] = tiles_of(s);
+  }
+  return z;
+}
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), kWave - 1); }
 // The lane with the smallest v (above zero), the lowest of several.
 __device__ __forceinline__ int wave_least(float v) {
@@ -115,10 +135,21 @@ struct Work {
 // A lane tries one length of the pieces: the longest row block's keys cut into one to
 // kCuts, or what all workers have in all and somewhat more, so that all run at once.  What
 // has the least rounds of pieces times their mean length, and the time that a piece takes
-// besides, is taken.  (Above 64 sequences: what the workers have in all.)
-__device__ __forceinline__ Work work_of(const ChunkArgs& a, const Seq& own) {
-  const int lane = lane_id(), blocks = blocks_of(a, own), tiles = tiles_of(own);
+// besides, is taken.  (Above 64 sequences: what
+// the workers have in all.)
+__device__ __forceinline__ Work work_of(const ChunkArgs& a, const Sizes& z) {
+  const int lane = lane_id(), blocks = z.blocks[0], tiles = z.tiles[0];
   const float heads = (float)a.heads_kv.d, slots = __builtin_amdgcn_rcpf((float)a.workers);
+  if (a.batch > kWave && a.batch <= kSorted) {
+    int all = 0, n = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) all += z.blocks[c] * z.tiles[c];
+    const int most = max((int)((float)wave_total(all) * heads * slots) + 1, kMinTiles);
+    const float inverse = __builtin_amdgcn_rcpf((float)most);
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) n += z.blocks[c] * pieces_in(z.tiles[c], most, inverse);
+    return {most, wave_total(n), 0, 1};
+  }
   if (a.batch > kWave) {
     int all = wave_total(blocks * tiles);
     for (int c = kWave; c < a.batch; c += kWave) {
@@ -186,12 +217,14 @@ __device__ __forceinline__ Seq seq_from(const Seq& s, int lane) {
           __builtin_amdgcn_readlane(s.at, lane)};
 }
 // Piece i of all, the last row block of a sequence first.  With more pieces than run at
-// once the sequences with the longest come first (of up to 64 sequences): short ones last
-// fill the ends.
+// once the sequences with the longest come first (of up to kSorted): short ones last fill
+// the ends (128 decoding sequences of 500 to 8192 tokens, 8 heads of 128: 193 us in the
+// order of the sequences).
 // JOIN: row block i of those that have several pieces, and its first.
 template <bool JOIN>
-__device__ __forceinline__ bool piece_of(const ChunkArgs& a, const Seq& own, const Work& w, int i, Piece& p) {
+__device__ __forceinline__ bool piece_of(const ChunkArgs& a, const Sizes& z, const Work& w, int i, Piece& p) {
   const int lane = lane_id();
+  const Seq& own = z.own;
   const float inverse = __builtin_amdgcn_rcpf((float)w.most);
   // x-th piece (row block) of the sequence in lane `at`, which has `blocks` cut into `pieces`
   auto found = [&](const Seq& s, int b, int at, int x, int blocks, int pieces, int slots) {
@@ -208,7 +241,7 @@ __device__ __forceinline__ bool piece_of(const ChunkArgs& a, const Seq& own, con
     p.t1 = p.piece + 1 == pieces ? tiles : min((int)(each * (float)(p.piece + 1)), tiles);
   };
   if (a.batch == 1) {
-    const int blocks = __builtin_amdgcn_readlane(blocks_of(a, own), 0);
+    const int blocks = __builtin_amdgcn_readlane(z.blocks[0], 0);
     if (w.tail) {
       const int whole = blocks - w.tail;
       if (i >= (JOIN ? w.tail : w.total)) return false;
@@ -217,30 +250,64 @@ __device__ __forceinline__ bool piece_of(const ChunkArgs& a, const Seq& own, con
       else found(own, 0, 0, i - whole, w.tail, w.cuts, 0);
       return true;
     }
-    const int pieces = __builtin_amdgcn_readlane(pieces_in(tiles_of(own), w.most, inverse), 0);
+    const int pieces = __builtin_amdgcn_readlane(pieces_in(z.tiles[0], w.most, inverse), 0);
     if (i >= (JOIN ? (pieces > 1 ? blocks : 0) : blocks * pieces)) return false;
     found(own, 0, 0, i, blocks, pieces, 0);
     return true;
   }
-  int base = 0, slots = 0;
+  int slots = 0;
+  if (a.batch <= kSorted) {
+    int pieces[kChunks], size[kChunks], length[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      pieces[c] = pieces_in(z.tiles[c], w.most, inverse);
+      size[c] = JOIN ? (pieces[c] > 1 ? z.blocks[c] : 0) : z.blocks[c] * pieces[c];
+      length[c] = pieces[c] > 1 ? w.most : z.tiles[c];  // at most w.most
+    }
+    auto from = [&](int t) {  // pieces of t tiles or more
+      int n = 0;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) n += length[c] >= t ? size[c] : 0;
+      return wave_total(n);
+    };
+    int lo = 0;
+    if (!JOIN && w.total * a.heads_kv.d > a.workers) {
+      if (i >= w.total) return false;
+      lo = 1;
+      int hi = w.most + 1;  // from(lo) > i >= from(hi)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (from(mid) > i) lo = mid; else hi = mid;
+      }
+      i -= from(lo + 1);
+    }
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      if (c * kWave >= a.batch) break;
+      const int mine = lo == 0 || length[c] == lo ? size[c] : 0;
+      const int upto = wave_scan(mine), all = __builtin_amdgcn_readlane(upto, kWave - 1);
+      const int split = pieces[c] > 1 ? z.blocks[c] * pieces[c] : 0, split_upto = wave_scan(split);
+      if (i < all) {
+        const int at = __builtin_ctzll(__ballot(upto > i));
+        const Seq s = c ? seq_of(a, c * kWave + lane) : own;
+        found(s, c * kWave + at, at, i - __builtin_amdgcn_readlane(upto - mine, at), __builtin_amdgcn_readlane(z.blocks[c], at),
+              __builtin_amdgcn_readlane(pieces[c], at), slots + __builtin_amdgcn_readlane(split_upto - split, at));
+        return true;
+      }
+      i -= all, slots += __builtin_amdgcn_readlane(split_upto, kWave - 1);
+    }
+    return false;
+  }
+  int base = 0;
   for (int c = 0; c < a.batch; c += kWave) {
     const Seq s = c ? seq_of(a, c + lane) : own;
     const int blocks = blocks_of(a, s), pieces = pieces_in(tiles_of(s), w.most, inverse);
     const int split = pieces > 1 ? blocks * pieces : 0;
     const int size = JOIN ? (pieces > 1 ? blocks : 0) : blocks * pieces;
-    int upto = wave_scan(size);
-    const int all = __builtin_amdgcn_readlane(upto, kWave - 1);
+    const int upto = wave_scan(size), all = __builtin_amdgcn_readlane(upto, kWave - 1);
     const int split_upto = wave_scan(split);
     if (base + all > i) {
-      if (!JOIN && a.batch <= kWave && w.total * a.heads_kv.d > a.workers) {
-        const int length = pieces > 1 ? w.most : tiles_of(s);
-        upto = size;
-        for (int b = 0; b < a.batch; ++b) {
-          const int other = __builtin_amdgcn_readlane(length, b);
-          if (other > length || (other == length && b < lane)) upto += __builtin_amdgcn_readlane(size, b);
-        }
-      }
-      const int at = __builtin_ctzll(__ballot(base + upto > i && base + upto - size <= i));
+      const int at = __builtin_ctzll(__ballot(base + upto > i));
       found(s, c + at, at, i - base - __builtin_amdgcn_readlane(upto - size, at), __builtin_amdgcn_readlane(blocks, at),
             __builtin_amdgcn_readlane(pieces, at), slots + __builtin_amdgcn_readlane(split_upto - split, at));
       return true;
@@ -760,10 +827,10 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
   const int item = a.heads_kv.of(blockIdx.x), kvh = blockIdx.x - item * a.heads_kv.d;
   Piece p;
   {
-    const Seq own = seq_of(a, lane_id());
-    const Work w = work_of(a, own);
+    const Sizes z = sizes_of(a);
+    const Work w = work_of(a, z);
     if (blockIdx.x == 0 && threadIdx.x == 0 && a.slots > 0) *a.plan = w;  // for the join
-    if (!piece_of<false>(a, own, w, item, p)) return;
+    if (!piece_of<false>(a, z, w, item, p)) return;
   }
   if (p.s.n * a.group.d - p.block * kRows <= 32) run<D, true>(a, p, kvh, k0, k1, v0, v1, info);
   else run<D, false>(a, p, kvh, k0, k1, v0, v1, info);
@@ -778,12 +845,12 @@ __global__ __launch_bounds__(kWave * kWaves) void kv8_chunk_join_kernel(ChunkArg
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 31, h = lane >> 5;
   constexpr int DT = D / 32;
-  const Seq own = seq_of(a, lane);
+  const Sizes z = sizes_of(a);
   const Work w = *a.plan;
   for (int x = blockIdx.x;; x += gridDim.x) {
     const int y = a.heads_kv.of(x), kvh = x - y * a.heads_kv.d, d = y % DT, quarter = y / DT % kWaves;
     Piece p;
-    if (!piece_of<true>(a, own, w, y / (DT * kWaves), p)) return;
+    if (!piece_of<true>(a, z, w, y / (DT * kWaves), p)) return;
     const int rows = p.s.n * a.group.d, first_row = p.block * kRows + quarter * 32;
     if (first_row >= rows) continue;
     const int row = first_row + r, token = a.group.of(row), q_head = kvh * a.group.d + row - token * a.group.d;

@@ -388,13 +388,13 @@ struct LayerShape {
   int64_t count, heads, page_bytes;
 };
 
-int check_layers(const lb_kv8_layer* at, int64_t count, int64_t heads, int64_t page_size, int64_t head_dim) {
+int check_layers(const lb_kv8_layer* at, int64_t count, int64_t num_pages, int64_t heads, int64_t page_size, int64_t head_dim) {
   if (count < 0) return LB_ERR_ARG;
   if (count == 0) return LB_OK;
   if (!at || heads <= 0 || heads > 4096) return LB_ERR_ARG;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return LB_ERR_PROB_SHAPE;
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return LB_ERR_PROB_SHAPE;
-  for (int64_t i = 0; i < count; ++i) {
+  for (int64_t i = 0; i < count && num_pages > 0; ++i) {
     if (!at[i].k_cache || !at[i].v_cache || !at[i].k_scale || !at[i].v_scale) return LB_ERR_ARG;
     if (!lbh::aligned(at[i].k_cache, 16) || !lbh::aligned(at[i].v_cache, 16) || !lbh::aligned(at[i].k_scale, 4) || !lbh::aligned(at[i].v_scale, 4))
       return LB_ERR_ALIGN;
@@ -484,7 +484,7 @@ extern "C" int lb_kv8_pages_extend(int32_t* page_table, int64_t rows, int64_t ma
                                    size_t scratch_bytes, lb_stream_t stream) {
   using namespace lb;
   int err = check_pages(page_table, rows, max_pages, table_stride, seq_lens, refs, num_pages, page_size);
-  if (err == LB_OK) err = check_layers(layers, num_layers, heads_kv, page_size, head_dim);
+  if (err == LB_OK) err = check_layers(layers, num_layers, num_pages, heads_kv, page_size, head_dim);
   if (err != LB_OK) return err;
   if (count < 0 || count > kMaxRows || (count > 0 && (!which || !add)) || !status) return LB_ERR_ARG;
   if (count * max_pages > (1 << 30)) return LB_ERR_PROB_SHAPE;  // new pages are numbered in 32 bits
@@ -506,7 +506,7 @@ extern "C" int lb_kv8_pages_compact(int32_t* page_table, int64_t rows, int64_t m
                                     int64_t head_dim, void* scratch, size_t scratch_bytes, lb_stream_t stream) {
   using namespace lb;
   int err = check_pages(page_table, rows, max_pages, table_stride, refs, refs, num_pages, page_size);
-  if (err == LB_OK) err = check_layers(layers, num_layers, heads_kv, page_size, head_dim);
+  if (err == LB_OK) err = check_layers(layers, num_layers, num_pages, heads_kv, page_size, head_dim);
   if (err != LB_OK) return err;
   if (!used) return LB_ERR_ARG;
   if (!lbh::aligned(scratch, 16)) return LB_ERR_ALIGN;
@@ -525,7 +525,7 @@ extern "C" int lb_kv8_pages_compact(int32_t* page_table, int64_t rows, int64_t m
 extern "C" int lb_kv8_copy_pages(const lb_kv8_layer* layers, int64_t num_layers, int64_t num_pages, int64_t heads_kv, int64_t page_size, int64_t head_dim,
                                  const int32_t* src, const int32_t* dst, int64_t count, lb_stream_t stream) {
   using namespace lb;
-  const int err = check_layers(layers, num_layers, heads_kv, page_size, head_dim);
+  const int err = check_layers(layers, num_layers, num_pages, heads_kv, page_size, head_dim);
   if (err != LB_OK) return err;
   if (num_pages < 0 || num_pages > 0x7fffffff - 65536 || count < 0 || count > 0x7fffffff || (count > 0 && (!src || !dst))) return LB_ERR_ARG;
   if (count == 0 || num_layers == 0 || num_pages == 0) return LB_OK;

@@ -118,6 +118,10 @@ CHUNKS = [
     ([129, 260], [1500, 100], 12, 1, 256, 64),
     ([31, 600], [50, 33], 8, 8, 64, 16),
     ([4] * 20, [100, 900, 40, 2000] * 5, 20, 4, 128, 16),
+    # more pieces than run at once: the sequences with the longest come first, whatever their place
+    ([1, 2, 1] * 34, [20, 300, 70, 5, 150, 0] * 17, 8, 8, 64, 32),
+    ([1, 0, 3, 1] * 65, [20, 0, 300, 70] * 65, 3, 3, 64, 16),      # and more sequences than stay in registers
+    ([40] * 12, [300, 100, 200] * 4, 64, 8, 64, 16),
 ]
 
 
@@ -134,7 +138,9 @@ def test_chunks_match_the_definition(dev, case):
 
 
 @pytest.mark.parametrize("news,held,hq,hkv,d,p", [([1500], [700], 40, 8, 128, 16), ([600, 1, 300], [0, 9000, 1000], 24, 4, 256, 64),
-                                                   ([2500, 70], [0, 4000], 8, 8, 64, 32), ([3], [40000], 8, 2, 128, 64)])
+                                                   ([2500, 70], [0, 4000], 8, 8, 64, 32), ([3], [40000], 8, 2, 128, 64),
+                                                   # whole row blocks for a round, and the first ones cut so that they fill one more
+                                                   ([1100], [300], 64, 2, 256, 32), ([2300], [900], 32, 4, 128, 16), ([2300], [0], 32, 4, 64, 64)])
 def test_long_chunks(dev, news, held, hq, hkv, d, p):
     import torch
 

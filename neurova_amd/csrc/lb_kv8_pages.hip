@@ -505,7 +505,7 @@ extern "C" int lb_kv8_pages_compact(int32_t* page_table, int64_t rows, int64_t m
                                     int32_t* used, const lb_kv8_layer* layers, int64_t num_layers, int64_t heads_kv, int64_t page_size,
                                     int64_t head_dim, void* scratch, size_t scratch_bytes, lb_stream_t stream) {
   using namespace lb;
-  int err = check_pages(page_table, rows, max_pages, table_stride, refs, refs, num_pages, page_size);
+  int err = check_pages(page_table, rows, max_pages, table_stride, used, refs, num_pages, page_size);  // no lengths here
   if (err == LB_OK) err = check_layers(layers, num_layers, num_pages, heads_kv, page_size, head_dim);
   if (err != LB_OK) return err;
   if (!used) return LB_ERR_ARG;

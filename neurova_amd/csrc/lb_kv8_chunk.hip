@@ -798,6 +798,8 @@ __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh,
       bring(i, k1, v1);
       if (i + 1 < count) bring(i + 1, k0, v0);
     }
+    // no load is on its way behind this loop, or the compiler waits for it in the other one
+    __builtin_amdgcn_s_waitcnt(0);
   } else {
     for (int i = 0; i < count; i += 2) {
       take(i, std::integral_constant<int, 0>(), k0, v0, k1, v1);
@@ -832,6 +834,7 @@ __global__ __launch_bounds__(kWave * kWaves, kPerSimd<D>) void kv8_chunk_kernel(
     if (blockIdx.x == 0 && threadIdx.x == 0 && a.slots > 0) *a.plan = w;  // for the join
     if (!piece_of<false>(a, z, w, item, p)) return;
   }
+  if (p.block < 0 || p.t0 < 0) return;  // of starts that do not ascend
   if (p.s.n * a.group.d - p.block * kRows <= 32) run<D, true>(a, p, kvh, k0, k1, v0, v1, info);
   else run<D, false>(a, p, kvh, k0, k1, v0, v1, info);
 }

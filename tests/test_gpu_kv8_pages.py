@@ -428,3 +428,20 @@ def test_refusals(dev):
     with pytest.raises(ValueError, match="page_size"):
         KV8Pages(8, 1, 64, page_size=20, device=dev)
     pool.same()
+
+
+@pytest.mark.parametrize("children, width", [(128, 16), (129, 16), (1, 2048), (1, 2049), (2047, 1), (700, 3)])
+def test_forks_of_few_and_many_entries(dev, children, width):
+    """One launch up to 2048 entries, two above; with parts of pages, rows named twice, outside, and holding tokens."""
+    print_case("pages-fork-entries", children, width)
+    rng = random.Random(children + width)
+    pool = Pool(dev, 2 * width + 5, children + 3, width, 16, layers=1, heads=1)
+    assert pool.extend([0, 1], [width * 16, max(width * 16 - 9, 1)]) == 0
+    named = [rng.randrange(2, children + 3) for _ in range(children)]
+    named[0] = rng.choice([-1, children + 3, 1])
+    parents = [rng.choice([0, 1, 1, 2, -1]) for _ in named]
+    pool.fork(parents, named, [rng.choice([0, 1, 15, 16, 17, width * 8, width * 16 + 3]) for _ in named])
+    pool.same("first")
+    pool.free(named[::2])
+    pool.fork(parents[::-1], named[::-1])
+    pool.same("second")

@@ -319,7 +319,7 @@ int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_s
 
 /* The same for any number of new tokens of each sequence, packed one after the
  * other: a sequence's rows are cu_seqlens[b] to cu_seqlens[b + 1], its newest
- * tokens (cu_seqlens int32 [batch + 1], on the device, as seq_lens).  Pieces of
+ * tokens (cu_seqlens int32 [batch + 1], ascending, on the device, as seq_lens).  Pieces of
  * prompts, whole ones, and sequences that decode a token or a few go into one
  * call.  Row i of n sees the keys 0 to seq_lens[b] - n + i that the table holds;
  * one that sees none (padding before position 0) is zero, and rows of tokens that
@@ -328,8 +328,9 @@ int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_s
  * (2^-11, and 2^-32 of the row's largest; value scales of any size up to 2^32, and
  * fp16 values give 2^9 at most).  A page's scale that is not finite reaches the rows
  * that see a token of the page.
- * One launch, or a second one that joins the parts of rows whose keys were cut,
- * which tables of more than a few hundred tokens take.  scratch:
+ * One launch, or with tables of more than 128 tokens a second one, which joins the
+ * parts of rows whose keys were cut: how they are depends on the lengths, on the
+ * device, so the same sequence in another batch may differ in the last bit.  scratch:
  * lb_kv8_chunk_attention_scratch_bytes() bytes, 16-byte aligned, no
  * initialisation; calls that share it must not overlap.  softmax_scale positive
  * and finite. */
@@ -388,7 +389,7 @@ int lb_kv8_pages_free(int32_t* page_table, int64_t rows, int64_t max_pages, int6
  * what that holds, by holding its pages too: nothing is copied.  Every request goes
  * by the tables as they were before the call.  A child that holds tokens, or that an
  * earlier request names, is left as it is; done (may be NULL) int32 [count] says 1
- * for the others.  Two launches. */
+ * for the others.  One launch, or two where count * max_pages is above 2048. */
 int lb_kv8_pages_fork(int32_t* page_table, int64_t rows, int64_t max_pages, int64_t table_stride,
                       int32_t* seq_lens, int32_t* refs, int64_t num_pages, int64_t page_size,
                       const int32_t* parents, const int32_t* children, const int32_t* lens, int32_t* done,

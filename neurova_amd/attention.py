@@ -2,7 +2,7 @@
 
 :class:`KV8Cache` holds one layer's keys and values in 8 bits, in pages of 16
 to 128 tokens with one fp32 scale for each page and key/value head.  Which page
-holds which tokens of which sequence is the caller's: every call takes a
+holds which tokens of which sequence the caller says: every call takes a
 ``page_table`` int32 ``[batch, max_pages]`` and ``seq_lens`` int32 ``[batch]``
 (the new tokens included), both on the GPU, so nothing here waits for the
 device.  A decode step is
@@ -15,10 +15,17 @@ and a batch of prompts, packed one after the other,
     q, k = cache.append(q, k, v, page_table, seq_lens, cu_seqlens, rotation=table, return_k=True)
     out = prompt_attention(q, k, v, cu_seqlens)
 
+A step that mixes pieces of prompts with sequences that decode is
+
+    cache.append(q, k, v, page_table, seq_lens, cu_seqlens, rotation=table, q_out=q)
+    out = cache.attend(q, page_table, seq_lens, cu_seqlens)
+
+and :mod:`neurova_amd.pages` says which row of a table holds which pages.
+
 Rows are fp16 ``[tokens, heads, head_dim]`` and may be views of the fused QKV
 projection's output.  Everything runs on the current stream through the
-``langburst_cuda`` ops ``kv8_append_out``, ``kv8_attention_out`` and
-``prompt_attention_out``; there is no CPU path.  These are this package's own
+``langburst_cuda`` ops ``kv8_append_out``, ``kv8_attention_out``,
+``kv8_chunk_attention_out`` and ``prompt_attention_out``; there is no CPU path.  These are this package's own
 operators, without a counterpart in the reference's projection path.
 """
 from __future__ import annotations
@@ -130,7 +137,7 @@ class KV8Cache:
         With ``cu_seqlens`` int32 ``[batch + 1]`` it says which of the packed
         queries are whose: pieces of prompts, whole ones and single tokens in one
         call.  Without it ``q`` holds the same number for every sequence, a token or
-        a few.  ``scale`` is ``head_dim ** -0.5`` by default.  ``workspace`` (only
+        a few, which for single tokens alone is the faster call.  ``scale`` is ``head_dim ** -0.5`` by default.  ``workspace`` (only
         without ``cu_seqlens``) int32, zeros, of tokens * heads entries, is left zero
         and belongs to calls that run in order; without it the cache keeps one for
         each stream, and a call captured into a graph clears one of its own in every

@@ -13,6 +13,15 @@
 // key/value head.  Four waves of 32 rows go through tiles of 64 keys together: the
 // codes of a tile come into registers while the tile before is computed, become fp16
 // (exactly) and lie in LDS for all four.
+//
+// Bound by what a SIMD issues: of its cycles the products take half and vector instructions
+// somewhat more (the codes to fp16 and the softmax in like shares), at the clock that the
+// load leaves; LDS is busy half of them.  (4096 new tokens on 12288, 40 on 8 heads of 128:
+// 1.22 ms, 986 TFLOP/s at 1.7 GHz.)  At 256 channels a SIMD has one wave, and 476 vector
+// instructions of a tile stand beside 64 products: a third of the cycles each (2048 on 6144:
+// 407 us, 887 TFLOP/s).  128 sequences of one new token: 161 us, 4.5 TB/s, where the operator
+// for single tokens takes 122.  The smallest calls run instructions for the first time (24 on
+// 301: 20 us, about 8 of them before the second tile and 4 for the second launch).
 #include <type_traits>
 
 #include "attn_common.hpp"
@@ -59,14 +68,21 @@ constexpr float kNoMax = -1e30f;
 // exponent, between 2^-kScales and 2^kScales (fp16 values give 2^-31 to 2^9), so that
 // no weight that counts in the sum falls below fp32's normal numbers.
 constexpr float kSlack = 8.0f, kLift = 7.0f, kScales = 32.0f, kMost = 32768.0f;  // 2^(kSlack + kLift)
-// A piece of a row block's keys is this many tiles at least.
+// A piece of a row block's keys is this many tiles at least (with 8 or 16: 24 tokens on 301
+// 25 and 32 us and not 20).
 constexpr int kMinTiles = 2;
 constexpr int kCuts = 24;
 // In tiles: what a piece takes beside its own, the launch that joins cut ones, and for
-// each round of these what their parts take to write and read.
+// each round of these what their parts take to write and read.  (Pieces as long as the
+// workers have on average: 7 of 17 to 900 tokens on up to 5000 311 us and not 243, two of up
+// to 700 beside 40 single ones 234 and 191, 2048 on 6144 at 256 channels 535 and 461.)
 constexpr float kPiece = 3.0f, kCut = 2.0f, kPart = 5.0f;
-constexpr int kPartRounds = 4;  // of parts that the scratch holds
+// Rounds of parts that the scratch holds (with six, and every row block cut: 4096 on 12288
+// 1372 us and not 1348).
+constexpr int kPartRounds = 4;
 
+// Workgroups that run at once on a compute unit, a wave of each on a SIMD.  (256 channels
+// fill the registers with one; 64 with three: 2048 on 2048 tokens 92.8 us and not 83.6.)
 template <int D>
 constexpr int kPerSimd = D == 256 ? 1 : 2;
 
@@ -190,7 +206,7 @@ __device__ __forceinline__ Work work_of(const ChunkArgs& a, const Sizes& z) {
   Work w = {__builtin_amdgcn_readlane(most, best), __builtin_amdgcn_readlane(n, best), 0, 1};
   if (a.batch == 1) {
     // whole row blocks for some rounds, and what is left of them, the shortest, cut so that it
-    // fills one more
+    // fills one more (2048 on 14336 711 us and not 742, 4096 on 12288 1296 and not 1398)
     const int count = __builtin_amdgcn_readlane(blocks, 0), full = (int)((float)(count * a.heads_kv.d) * slots + 0.001f);
     const int tail = count - (int)((float)(full * a.workers) * __builtin_amdgcn_rcpf(heads) + 0.001f);
     const int cuts = tail > 0 ? (int)((float)a.workers * __builtin_amdgcn_rcpf((float)tail * heads) + 0.001f) : 1;
@@ -218,8 +234,9 @@ __device__ __forceinline__ Seq seq_from(const Seq& s, int lane) {
 }
 // Piece i of all, the last row block of a sequence first.  With more pieces than run at
 // once the sequences with the longest come first (of up to kSorted): short ones last fill
-// the ends (128 decoding sequences of 500 to 8192 tokens, 8 heads of 128: 193 us in the
-// order of the sequences).
+// the ends (128 decoding sequences of 500 to 8192 tokens, 8 heads of 128: 161 us, and 193 in
+// the order of the sequences; three of up to 500 new tokens beside 200 single ones 222 and
+// 248).
 // JOIN: row block i of those that have several pieces, and its first.
 template <bool JOIN>
 __device__ __forceinline__ bool piece_of(const ChunkArgs& a, const Sizes& z, const Work& w, int i, Piece& p) {
@@ -332,8 +349,8 @@ __device__ __forceinline__ int k_swizzle(int key) {
   return D == 64 ? (key >> 1 & 1) | b4 << 1 | b2 << 2 : (key & 3) | b4 << 2 | b2 << 3;
 }
 
-// Sixteen tiles' pages and scales are looked up together, lane l those of the 16 tokens
-// l % 4 of tile l / 4, and what the products need of them lies in LDS for all waves: the
+// Sixteen tiles' pages and scales are looked up together (4096 on 12288 1267 us, and 1300 with
+// a tile's at a time), lane l those of the 16 tokens l % 4 of tile l / 4, and what the products need of them lies in LDS for all waves: the
 // factor of the scores, the value scale as an exponent, the inverse of that (2^-kLift
 // times), and what is left of a value scale outside the exponent's range.
 constexpr int kBatch = 16;
@@ -569,7 +586,8 @@ __device__ __forceinline__ void finish(const ChunkArgs& a, const Piece& p, int k
 }
 
 // A piece, by the waves of a workgroup.  THIN: a row block of up to 32 rows, which the waves
-// share: each takes half of the keys and half of the channels.
+// share: each takes half of the keys and half of the channels (two of up to 700 tokens beside
+// 40 single ones 173 us, and 203 with the rows in one wave; 128 single ones 205 and 237).
 template <int D, bool THIN>
 __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh, uint16_t* k0, uint16_t* k1, uint16_t* v0, uint16_t* v1, Info& info) {
   constexpr int DT = D / 32, KK = D / 16, ST = kKeys / 32, OB = THIN ? DT / 2 : DT;
@@ -598,7 +616,7 @@ __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh,
   for (int d = 0; d < OB; ++d) o[d] = (f32x16)(0.0f);
 
   // a thin block's tile is done before the next one's codes can arrive; it has registers
-  // to spare
+  // to spare (7 of 17 to 900 tokens 224 us, and 247 a tile ahead)
   constexpr int DEPTH = THIN ? 2 : 1;
   typedef Tiles<D, DEPTH> T;
   T tiles(a, info, p, kvh, wave);
@@ -658,6 +676,8 @@ __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh,
         }
     };
     read_k(0);
+    // products before another wave's softmax, those with the values first (2048 on 14336
+    // 742 us, and 779 without an order; others took as long or longer)
     __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -739,7 +759,8 @@ __device__ __forceinline__ void run(const ChunkArgs& a, const Piece& p, int kvh,
     };
     if constexpr (!THIN) stay_in_accumulators<D>(o);
     if constexpr (D == 256 && !THIN) {
-      // the scores beside their weights do not fit the registers
+      // the scores beside their weights do not fit the registers (2048 on 6144 536 us, and
+      // 616 with the weights first)
       const float up = highest();
       if (__any(up > m + kSlack)) raise(up);
       weigh();

@@ -920,7 +920,7 @@ __global__ __launch_bounds__(kWave * kWaves) void kv8_chunk_join_kernel(ChunkArg
 }
 
 struct Plan {
-  int64_t workers, slots, grid;
+  int64_t workers, slots, blocks, grid;
   int joined;
   size_t scratch;
 };
@@ -936,7 +936,7 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv, i
   // no more pieces than all row blocks have of the smallest size
   const int64_t pieces = blocks * ((tiles + kMinTiles - 1) / kMinTiles);
   p.slots = !p.joined ? 0 : pieces < kPartRounds * p.workers ? pieces : kPartRounds * p.workers;
-  p.grid = blocks + p.slots;
+  p.blocks = blocks, p.grid = blocks + p.slots;
   p.scratch = p.slots ? (((size_t)p.slots * kRows * (head_dim + 2) * 4 + 255) & ~(size_t)255) + 256 : 0;
   return p;
 }
@@ -958,7 +958,7 @@ template <int D>
 void launch(const ChunkArgs& a, const Plan& p, hipStream_t st) {
   kv8_chunk_kernel<D><<<dim3((unsigned)p.grid), dim3(kWave * kWaves), 0, st>>>(a);
   if (!p.joined) return;
-  const int64_t units = p.workers * kWaves * (D / 32), most = 8 * (int64_t)lbh::device_cus();
+  const int64_t cut = p.blocks < p.workers ? p.blocks : p.workers, units = cut * kWaves * (D / 32), most = 8 * (int64_t)lbh::device_cus();
   kv8_chunk_join_kernel<D><<<dim3((unsigned)(units < most ? units : most)), dim3(kWave * kWaves), 0, st>>>(a);
 }
 

@@ -445,3 +445,27 @@ def test_forks_of_few_and_many_entries(dev, children, width):
     pool.free(named[::2])
     pool.fork(parents[::-1], named[::-1])
     pool.same("second")
+
+
+def test_rows_of_many_pages(dev):
+    """Tables wider than a workgroup's turn, and than a turn of all workgroups of a row: cut, forked, ended."""
+    import torch
+
+    from neurova_amd.pages import KV8Pages
+
+    print_case("pages-wide")
+    width = 256 * 4096 + 300
+    pages = KV8Pages(2 * width, 4, width * 16, page_size=16, device=dev)
+    row = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    assert int(pages.extend(row(2), row(width * 16))) == 0
+    want = torch.arange(width, dtype=torch.int32, device=dev)
+    assert torch.equal(pages.page_table[2], want) and int(pages.refs.sum()) == width
+    pages.fork(row(2), row(0), row(width * 16 - 20))
+    assert torch.equal(pages.page_table[0][:width - 1], want[:-1]) and int(pages.page_table[0][-1]) == -1
+    assert int(pages.refs.sum()) == 2 * width - 1
+    pages.free(row(2), row(16 * 300 + 1))
+    assert pages.seq_lens.tolist() == [width * 16 - 20, 0, 16 * 300 + 1, 0]
+    assert torch.equal(pages.page_table[2][:301], want[:301]) and int(pages.page_table[2][301:].max()) == -1
+    assert int(pages.refs.sum()) == width - 1 + 301 and int(pages.refs[width - 1]) == 0
+    pages.free(row(0, 2))
+    assert not pages.refs.any() and not pages.seq_lens.any() and int(pages.page_table.max()) == -1

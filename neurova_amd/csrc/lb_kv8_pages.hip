@@ -7,7 +7,7 @@
 // holders; everything stays on the GPU.
 //
 // Bound by latency: a few dependent loads (rows, lengths, holders, pages) and the
-// launches.  free takes 2 to 5 us, fork 3 to 5, extend 8 to 13 (200 rows, and 100000 tokens
+// launches.  free takes 2 to 5 us, fork 3 to 5, extend 8 to 11 (200 rows, and 100000 tokens
 // for each of six), the plan of compact 7 to 8.  One workgroup plans, since every count goes
 // by all rows before it.  Copies are bound by HBM (951 pages of 128 KB in each of four layers,
 // read and written: 190 us, 5.2 TB/s).

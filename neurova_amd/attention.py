@@ -138,11 +138,11 @@ class KV8Cache:
         queries are whose: pieces of prompts, whole ones and single tokens in one
         call.  Without it ``q`` holds the same number for every sequence, a token or
         a few, which for single tokens alone is the faster call.  Rows of tokens that
-        belong to no sequence are not written.  ``scale`` is ``head_dim ** -0.5`` by default.  ``workspace`` (only
-        without ``cu_seqlens``) int32, zeros, of tokens * heads entries, is left zero
-        and belongs to calls that run in order; without it the cache keeps one for
-        each stream, and a call captured into a graph clears one of its own in every
-        replay.
+        belong to no sequence are not written.  ``scale`` is ``head_dim ** -0.5`` by
+        default.  ``workspace`` (only without ``cu_seqlens``) int32, zeros, of tokens *
+        heads entries, is left zero and belongs to calls that run in order; without it
+        the cache keeps one for each stream, and a call captured into a graph clears
+        one of its own in every replay.
         """
         import torch
 

@@ -402,8 +402,10 @@ int lb_kv8_pages_fork(int32_t* page_table, int64_t rows, int64_t max_pages, int6
  * it.  (A copy has the whole page's codes and scales.)  A row's page comes before
  * its new ones.  All or nothing: *status is 0, or how many pages are missing, -1
  * where a row would pass the end of its table, -2 where a page would have to be
- * copied and no layers are given; nothing has changed then.  Of a row that is named
- * twice the first counts.  layers: host array, num_layers caches of num_pages pages
+ * copied and no layers are given; nothing has changed then, and the tokens must not be
+ * appended (lb_kv8_append by the old lengths overwrites the last tokens that the row
+ * holds, for every row that shares their page; by lengths of 0 it stores nothing).
+ * Of a row that is named twice the first counts.  layers: host array, num_layers caches of num_pages pages
  * of the same shape (0: none).  One launch, and one more for each 32 layers.
  * scratch: lb_kv8_pages_extend_scratch_bytes(), 16-byte aligned, no initialisation. */
 size_t lb_kv8_pages_extend_scratch_bytes(int64_t num_pages);

@@ -9,8 +9,16 @@ takes, and the number of rows that hold each page.  A prompt and eight answers:
     ... every layer appends the prompt's keys and values ...
     pages.fork(prompt.expand(8).contiguous(), answers)      # nothing is copied
     status = pages.extend(answers, 1)                       # pages for a token each; the prompt's last page is copied
-    cache.append(q, k, v, pages.page_table[answers], pages.seq_lens[answers], ...)
+    table = pages.page_table[answers]
+    lens = pages.seq_lens[answers] * (status == 0)          # refused: nothing has changed, and the new tokens are padding
+    cache.append(q, k, v, table, lens)                      # every layer
+    out = cache.attend(q, table, lens)
     pages.free(answers)
+
+A row's lengths do not change when :meth:`KV8Pages.extend` refuses, so tokens
+appended by them all the same would overwrite the last ones that the row holds,
+and those of every row that shares the page.  Lengths of zero instead store
+nothing, and nothing has to wait for the status.
 
 Free pages are handed out lowest first, :meth:`KV8Pages.compact` moves the
 pages in use to the front, and nothing waits for the device.  The operators
@@ -77,7 +85,8 @@ class KV8Pages:
 
         0: done.  Otherwise nothing has changed: the number of pages that are
         missing, -1 where a row would pass the end of the table, -2 where a shared
-        page would have to be copied and there are no caches.
+        page would have to be copied and there are no caches.  The tokens must not be
+        appended then; ``seq_lens[rows] * (status == 0)`` as the lengths makes padding of them.
         """
         import torch
 

@@ -60,3 +60,106 @@ def test_a_refused_step_as_documented_changes_nothing(dev, refused):
         pages.free(answers[:1], i32([40]))
     exec(documented_step(), got)
     assert int(got["status"]) == 0 and got["out"].any()
+
+
+# ------------------------------------------------- scales that lie far apart ---
+
+
+class Scaled:
+    """Sequences whose logits stay within some 2^4, beside value scales that lie as far apart as `spread` says.
+
+    Drawn on the CPU, so that :meth:`check` can be shown there to have power.  Of
+    each sequence (after the first) the value scales have a level of their own,
+    since an output shows only what is within 2^-11 of it.
+    """
+
+    LEVELS = (8.0, 0.0, -5.0, -9.0)
+
+    def __init__(self, d, p, spread, seed, kinds="plain", hq=4, hkv=2):
+        import torch
+
+        from tests.test_gpu_kv8_chunk import Chunks
+
+        self.c = c = Chunks("cpu", [70, 5, 40, 1], [500, 90, 200, 333], hq, hkv, d, p, seed=seed, sharp=2.0)
+        g = torch.Generator()
+        g.manual_seed(seed + 1000)
+        for b, level in enumerate(self.LEVELS):
+            pages = torch.from_numpy(c.table_np[b][c.table_np[b] >= 0]).long()
+            n = len(pages)
+            down = (torch.randn((n, hkv), generator=g).abs() * spread).exp2()
+            down[torch.randint(n, (hkv,), generator=g), torch.arange(hkv)] = 1.0   # one page at the level itself
+            down[0] = down[0].clamp(max=4.0)                                       # and one near it that every row sees
+            c.v_scale[pages] = 2.0 ** level / down * 0.9
+            c.k_scale[pages] *= (torch.randn((n, hkv), generator=g) * 0.5).exp2()
+            if kinds == "odd":  # of pages behind the first: no scale, negative ones, values below all that count
+                c.v_scale[pages[1::6]] = 0.0
+                c.v_scale[pages[2::6]] *= -1
+                c.k_scale[pages[3::6]] *= -1
+                c.k_scale[pages[4::6]] = 0.0
+                c.v_scale[pages[5::6], 0] = 2.0 ** -45
+
+    def to(self, dev):
+        import torch
+
+        for name, t in vars(self.c).items():
+            if isinstance(t, torch.Tensor):
+                setattr(self.c, name, t.to(dev))
+        self.c.dev = dev
+        return self
+
+    def wanted(self):
+        """For every sequence and head: where its rows are, the output in 64 bits and how far it may be off.
+
+        A weight p_j (times its value scale) is off by the error of its score, (d + 3)
+        roundings of fp32 of scale |q| |k_j|, by those of the exponential, the logarithm,
+        their argument below 2^7 and the sums (2^-16), by its rounding to fp16 (2^-11) or,
+        below fp16's normal numbers, by 2^-32 of the row's largest; the sum of all that the
+        output is divided by is off by the mean of the first two.
+        """
+        import torch
+
+        c, at = self.c, 0
+        for b, (n, length) in enumerate(zip(c.news, c.lens)):
+            pages = torch.from_numpy(c.table_np[b][c.table_np[b] >= 0]).to(c.dev).long()
+            sees = torch.arange(length - n, length, device=c.dev)[:, None] >= torch.arange(length, device=c.dev)
+            for h in range(c.hq):
+                kv = h // (c.hq // c.hkv)
+                ks, vs = (t[pages, kv].double().repeat_interleave(c.p)[:length] for t in (c.k_scale, c.v_scale))
+                k = c.k_cache[pages, kv].double().reshape(-1, c.d)[:length] * ks[:, None]
+                v = c.v_cache[pages, kv].double().transpose(1, 2).reshape(-1, c.d)[:length]
+                q = c.q[at:at + n, h].double()
+                p = torch.softmax(((q @ k.T) * c.d ** -0.5).masked_fill(~sees, -torch.inf), dim=-1)
+                w = p * vs
+                out = w @ v
+                off = (c.d + 3) * 2.0 ** -24 * c.d ** -0.5 * (q.abs() @ k.abs().T) + 2.0 ** -16
+                bound = 2.0 ** -11 * out.abs() + ((off + 2.0 ** -11) * w.abs()) @ v.abs() + (off * p).sum(-1, keepdim=True) * out.abs()
+                bound += 2.0 ** -32 * w.abs().amax(-1, keepdim=True) * (sees.double() @ v.abs()) + 2.0 ** -25
+                yield b, h, slice(at, at + n), out, bound
+            at += n
+
+    def check(self, got):
+        for b, h, rows, want, bound in self.wanted():
+            bad = ~((got[rows, h].double() - want).abs() <= bound)
+            assert not bad.any(), (b, h, int(bad.sum()), float((got[rows, h].double() - want).abs().max()))
+
+    def has_power(self):
+        """Outputs that are zeros, or that leave a page or its scale out, are far outside the bounds."""
+        for b, h, rows, want, bound in self.wanted():
+            assert float((want.abs() > 4 * bound).double().mean()) > 0.9, (b, h)
+            assert float(bound.median()) < 2.0 ** -5 * float(want.abs().median()), (b, h)
+            assert float(want.abs().max()) < 65504
+
+
+SCALED = [(d, p, spread, kinds) for d, p in ((64, 16), (128, 64), (256, 32)) for spread, kinds in ((3.0, "plain"), (9.0, "plain"), (9.0, "odd"))]
+
+
+@pytest.mark.parametrize("d,p,spread,kinds", SCALED)
+def test_value_scales_far_apart(dev, d, p, spread, kinds):
+    import torch
+
+    print_case("serving-scales", d, p, spread, kinds)
+    s = Scaled(d, p, spread, seed=d + int(spread), kinds=kinds)
+    s.has_power()
+    out = s.to(dev).c.run()
+    torch.cuda.synchronize()
+    s.check(out)

@@ -163,3 +163,107 @@ def test_value_scales_far_apart(dev, d, p, spread, kinds):
     out = s.to(dev).c.run()
     torch.cuda.synchronize()
     s.check(out)
+
+
+# ------------------------------------------------------ any order of calls ---
+
+
+class Calls:
+    """Calls that a state of the table makes worth making, and how often each thing came of them.
+
+    The pool has about as many pages as the rows come to hold, requests are drawn
+    from what the rows hold, and some are refused on purpose.
+    """
+
+    KINDS = ("copied", "moved", "branched", "cut", "done", "missing", "row full")
+
+    def __init__(self, seed, page):
+        import random
+
+        self.rng = random.Random(seed * 100 + page)
+        self.page, self.rows, self.width = page, *self.rng.choice([(12, 6), (24, 5), (90, 4)])
+        self.pages = int(self.rows * self.width * self.rng.uniform(0.45, 0.6))
+        self.came = dict.fromkeys(self.KINDS, 0)
+
+    def next(self, model):
+        """The name and the arguments of a call, for a table as `model` says."""
+        rng, p = self.rng, self.page
+        full = [r for r in range(self.rows) if model.lens[r] > 0]
+        empty = [r for r in range(self.rows) if model.lens[r] <= 0]
+        free = sum(x <= 0 for x in model.refs)
+        few = lambda rows, most: rng.sample(rows, min(len(rows), rng.randint(1, most)))  # noqa: E731
+        what = rng.choice(["extend", "extend", "extend", "fork", "cut", "end", "compact", "bad"])
+        if len(full) < 2:
+            what = "extend"
+        elif free < self.width or not empty:
+            what = rng.choice(["end", "end", "cut", "extend", "bad"])
+        if what == "extend":
+            # half the time rows whose last page others hold too
+            share = [r for r in full if model.lens[r] % p and model.refs[model.table[r][model.lens[r] // p]] > 1]
+            rows = few(share if share and rng.random() < 0.5 else range(self.rows), 6)
+            # within the row, one token, to the end of a page, or some pages
+            add = [min(rng.choice([1, 1, 3, p - model.lens[r] % p, rng.randint(1, 2 * p)]), self.width * p - model.lens[r]) for r in rows]
+            return "extend", (rows + rows[:1], add + [5])          # a row named again changes nothing
+        if what == "fork":
+            parents = few(full, 2) * 3
+            children = few(empty, 5) + [full[0]]                    # and one that holds tokens
+            parents = [rng.choice(parents) for _ in children]
+            # of a half all, of others a part that ends inside a page or at its end
+            lens = None if rng.random() < 0.5 else [rng.choice([model.lens[r], rng.randint(1, model.lens[r]), p]) for r in parents]
+            return "fork", (parents, children, lens)
+        if what in ("cut", "end"):
+            rows = few(full, 4)
+            return "free", (rows + rows[:1], [0 if what == "end" else max(model.lens[r] - rng.choice([1, 2, p]), 0) for r in rows + rows[:1]])
+        if what == "bad":
+            if rng.random() < 0.5:                                  # a row past its end, beside one that would do
+                return "extend", ([full[0], full[1]], [1, self.width * p - model.lens[full[1]] + 1])
+            rows, add, left = [], [], free                          # more pages than there are
+            for r in rng.sample(range(self.rows), self.rows):
+                room = self.width * p - model.lens[r]
+                if room > 0:
+                    rows.append(r), add.append(room)
+                    left -= room // p
+                if left < 0:
+                    break
+            return "extend", (rows, add)
+        return "compact", ()
+
+    def count(self, what, args, result, before, model):
+        came = self.came
+        if what == "extend":
+            came["done" if result == 0 else "row full" if result < 0 else "missing"] += 1
+            came["copied"] += sum(a != b for a, b in zip(before, model.was))
+        elif what == "compact":
+            came["moved"] += sum(a != b for a, b in zip(before, model.was))
+        elif what == "fork":
+            came["branched"] += sum(result)
+        else:
+            came["cut"] += len(args[0])
+
+    def enough(self):
+        """Everything that can come of a call came of some, and most went through."""
+        least = {"copied": 5, "moved": 5, "branched": 5, "cut": 5, "done": 12, "missing": 1, "row full": 1}
+        assert all(self.came[k] >= n for k, n in least.items()), self.came
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("seed", range(3))
+def test_any_order_of_calls_that_a_server_makes(dev, page, seed):
+    from tests.test_gpu_kv8_pages import Pool
+
+    calls = Calls(seed, page)
+    print_case("serving-any", page, seed, calls.rows, calls.width, calls.pages)
+    pool = Pool(dev, calls.pages, calls.rows, calls.width, page, layers=1 + seed, heads=1 + 2 * (seed % 2), dim=(64, 128, 256)[seed], seed=seed)
+    for step in range(80):
+        what, args = calls.next(pool.model)
+        before = list(pool.model.was)
+        if what == "fork":
+            done = pool.i32([7] * len(args[0]))
+            pool.pages.fork(*map(pool.i32, args), done)
+            result = pool.model.fork(*args)
+            assert done.tolist() == result, (step, args)
+        else:
+            result = getattr(pool, what)(*args)
+        pool.same((step, what, args))
+        calls.count(what, args, result, before, pool.model)
+    calls.enough()

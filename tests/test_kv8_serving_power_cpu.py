@@ -1,9 +1,10 @@
-"""What the GPU tests of serving would notice, shown on the CPU by mistakes planted in the expected values."""
+"""What the GPU tests of serving would notice, shown on the CPU: mistakes planted in the expected values, and which calls their draws make."""
 from __future__ import annotations
 
 import pytest
 
-from tests.test_gpu_kv8_serving_edges import SCALED, Scaled
+from tests.test_gpu_kv8_pages import Model
+from tests.test_gpu_kv8_serving_edges import SCALED, Calls, Scaled
 
 
 @pytest.mark.parametrize("d,p,spread,kinds", SCALED)
@@ -28,3 +29,15 @@ def test_a_wrong_scale_is_noticed(d, p, spread, kinds):
             got[rows, h] = want
         with pytest.raises(AssertionError):
             s.check(got.half())
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("seed", range(3))
+def test_the_calls_drawn_make_everything_happen(page, seed):
+    calls = Calls(seed, page)
+    model = Model(calls.pages, calls.rows, calls.width, page)
+    for _ in range(80):
+        what, args = calls.next(model)
+        before = list(model.was)
+        calls.count(what, args, getattr(model, what)(*args), before, model)
+    calls.enough()

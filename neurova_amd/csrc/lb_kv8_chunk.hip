@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "attn_common.hpp"
+#include "chunk_pieces.hpp"
 
 namespace lb {
 namespace {
@@ -53,14 +54,14 @@ struct ChunkArgs {
   float* parts;
   struct Work* plan;  // behind the parts: how the keys were cut
   int64_t table_stride;
-  int num_pages, page_shift, max_tokens;
+  int num_pages, page_shift, max_tokens, unit_shift;
   int batch, tokens;
   Divisor heads_kv, group;
   int workers, slots;  // workgroups that run at once; parts that the scratch holds
   float scale;         // softmax scale * log2(e)
 };
 
-constexpr int kRows = 128, kKeys = 64, kWaves = 4;
+constexpr int kRows = 128, kKeys = 1 << kTileShift, kWaves = 4;
 constexpr float kNoMax = -1e30f;
 // The running maximum is that of weight times value scale.  It moves only when
 // exceeded by 2^kSlack, and the weights carry 2^kLift more: at most 2^15, inside
@@ -103,12 +104,8 @@ __device__ __forceinline__ Seq seq_of(const ChunkArgs& a, int b) {
   return s;
 }
 __device__ __forceinline__ int blocks_of(const ChunkArgs& a, const Seq& s) { return (s.n * a.group.d + kRows - 1) / kRows; }
-__device__ __forceinline__ int tiles_of(const Seq& s) { return max((s.len + kKeys - 1) / kKeys, 1); }
-// Pieces of each of a sequence's row blocks.  The float quotient is exact enough:
-// (x + 1/2) / most is 1 / (2 most) away from an integer, more than its error.
-__device__ __forceinline__ int pieces_in(int tiles, int most, float inverse) {
-  return (int)(((float)(tiles + most - 1) + 0.5f) * inverse);
-}
+// What the keys of a sequence are cut by: tiles, or units of a few in the longest tables.
+__device__ __forceinline__ int tiles_of(const ChunkArgs& a, const Seq& s) { return max(units_of(s.len, a.unit_shift), 1); }
 // Up to kSorted sequences' row blocks and tiles stay in registers, lane l those of sequence
 // 64 c + l.
 constexpr int kChunks = 4, kSorted = kChunks * kWave;
@@ -119,13 +116,13 @@ struct Sizes {
 __device__ __forceinline__ Sizes sizes_of(const ChunkArgs& a) {
   Sizes z;
   z.own = seq_of(a, lane_id());
-  z.blocks[0] = blocks_of(a, z.own), z.tiles[0] = tiles_of(z.own);
+  z.blocks[0] = blocks_of(a, z.own), z.tiles[0] = tiles_of(a, z.own);
 #pragma unroll
   for (int c = 1; c < kChunks; ++c) {
     z.blocks[c] = 0, z.tiles[c] = 1;
     if (c * kWave >= a.batch || a.batch > kSorted) continue;
     const Seq s = seq_of(a, c * kWave + lane_id());
-    z.blocks[c] = blocks_of(a, s), z.tiles[c] = tiles_of(s);
+    z.blocks[c] = blocks_of(a, s), z.tiles[c] = tiles_of(a, s);
   }
   return z;
 }
@@ -160,7 +157,7 @@ __device__ __forceinline__ Work work_of(const ChunkArgs& a, const Sizes& z) {
     int all = 0, n = 0;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) all += z.blocks[c] * z.tiles[c];
-    const int most = max((int)((float)wave_total(all) * heads * slots) + 1, kMinTiles);
+    const int most = max(min((int)((float)wave_total(all) * heads * slots) + 1, kMostUnits), kMinTiles);
     const float inverse = __builtin_amdgcn_rcpf((float)most);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) n += z.blocks[c] * pieces_in(z.tiles[c], most, inverse);
@@ -170,14 +167,14 @@ __device__ __forceinline__ Work work_of(const ChunkArgs& a, const Sizes& z) {
     int all = wave_total(blocks * tiles);
     for (int c = kWave; c < a.batch; c += kWave) {
       const Seq s = seq_of(a, c + lane);
-      all += wave_total(blocks_of(a, s) * tiles_of(s));
+      all += wave_total(blocks_of(a, s) * tiles_of(a, s));
     }
-    const int most = max((int)((float)all * heads * slots) + 1, kMinTiles);
+    const int most = max(min((int)((float)all * heads * slots) + 1, kMostUnits), kMinTiles);
     const float inverse = __builtin_amdgcn_rcpf((float)most);
     int n = wave_total(blocks * pieces_in(tiles, most, inverse));
     for (int c = kWave; c < a.batch; c += kWave) {
       const Seq s = seq_of(a, c + lane);
-      n += wave_total(blocks_of(a, s) * pieces_in(tiles_of(s), most, inverse));
+      n += wave_total(blocks_of(a, s) * pieces_in(tiles_of(a, s), most, inverse));
     }
     return {most, n, 0, 1};
   }
@@ -318,7 +315,7 @@ __device__ __forceinline__ bool piece_of(const ChunkArgs& a, const Sizes& z, con
   int base = 0;
   for (int c = 0; c < a.batch; c += kWave) {
     const Seq s = c ? seq_of(a, c + lane) : own;
-    const int blocks = blocks_of(a, s), pieces = pieces_in(tiles_of(s), w.most, inverse);
+    const int blocks = blocks_of(a, s), pieces = pieces_in(tiles_of(a, s), w.most, inverse);
     const int split = pieces > 1 ? blocks * pieces : 0;
     const int size = JOIN ? (pieces > 1 ? blocks : 0) : blocks * pieces;
     const int upto = wave_scan(size), all = __builtin_amdgcn_readlane(upto, kWave - 1);
@@ -1004,7 +1001,7 @@ extern "C" int lb_kv8_chunk_attention(const uint16_t* q, int64_t q_token_stride,
   a.parts = static_cast<float*>(scratch), a.plan = p.slots ? reinterpret_cast<Work*>(static_cast<char*>(scratch) + p.scratch - 256) : nullptr;
   a.table_stride = table_stride;
   a.num_pages = (int)num_pages, a.page_shift = __builtin_ctzll((unsigned long long)page_size);
-  a.max_tokens = (int)max_tokens;
+  a.max_tokens = (int)max_tokens, a.unit_shift = unit_shift((int)max_tokens);
   a.batch = (int)batch, a.tokens = (int)tokens, a.heads_kv = Divisor((int)heads_kv), a.group = Divisor((int)(heads_q / heads_kv));
   a.workers = (int)p.workers, a.slots = (int)p.slots;
   a.scale = softmax_scale * kLog2e;

@@ -267,3 +267,32 @@ def test_any_order_of_calls_that_a_server_makes(dev, page, seed):
         pool.same((step, what, args))
         calls.count(what, args, result, before, pool.model)
     calls.enough()
+
+
+def test_a_hundred_million_tokens(dev):
+    """More tiles of keys than a rounded quotient counts exactly.  Every entry of the table is the same page, so the softmax is that over one page.
+
+    Tolerance: as everywhere, and for the fp32 sums of a piece's tiles, of which 512 workgroups
+    have 3100 each: a term of the sum of the weights and four of an output's sum a tile, 2^-24 each.
+    """
+    import torch
+
+    from tests.test_gpu_kv8_chunk import Chunks
+
+    print_case("serving-long")
+    c = Chunks(dev, [1], [127], 4, 2, 64, 128, seed=21)
+    page = c.table[0, 0].clone()
+    c.check(c.run())
+    p = c.run().double()
+    k = c.k_cache[page].double() * c.k_scale[page].double()[:, None, None]
+    v = c.v_cache[page].double().transpose(1, 2) * c.v_scale[page].double()[:, None, None]
+    c.table = page.expand(1, 100_000_000 // 128).contiguous()
+    c.seq_lens.fill_(100_000_000)
+    out = c.run()
+    torch.cuda.synchronize()
+    for h in range(4):
+        w = torch.softmax(c.q[0, h].double() @ k[h // 2].T * 64 ** -0.5, dim=-1)
+        want, spread = w @ v[h // 2], w @ v[h // 2].abs()
+        bound = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -16 + 5 * 3100 * 2.0 ** -24) * spread + 2.0 ** -25
+        assert float(want.abs().median()) > 8 * float(bound.median())
+        assert ((out[0, h].double() - want).abs() <= bound).all(), (h, float((out[0, h].double() - want).abs().max()), float((out[0, h] - p[0, h]).abs().max()))

@@ -30,6 +30,8 @@ counterpart in the reference's projection path.
 """
 from __future__ import annotations
 
+import operator
+
 from .attention import PAGE_SIZES
 from .store import _ops, _require_device
 
@@ -53,9 +55,9 @@ def copy_pages(layers, src, dst):
 class KV8Pages:
     """Rows of pages: ``page_table`` int32 ``[rows, max_pages]``, ``seq_lens`` int32 ``[rows]``, ``refs`` int32 ``[num_pages]``.
 
-    ``caches``: one :class:`KV8Cache` of ``num_pages`` pages for each layer.
-    Without them, pages are counted but nothing is copied or moved, and
-    :meth:`extend` refuses rows whose last page would have to be copied.
+    ``caches``: one :class:`KV8Cache` of ``num_pages`` pages of ``page_size`` tokens
+    for each layer.  Without them the tables alone change: nothing is copied or moved,
+    and :meth:`extend` refuses rows whose last page would have to be copied.
     ``rows`` arguments are int32 tensors on the GPU, of at most 4096 rows.
     """
 
@@ -66,11 +68,16 @@ class KV8Pages:
             raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
         if num_pages < 0 or rows < 0 or max_tokens < 0:
             raise ValueError("num_pages, rows and max_tokens must not be negative")
+        caches = list(caches)
+        for i, c in enumerate(caches):
+            if (c.k_cache.shape[0], c.k_cache.shape[2]) != (num_pages, page_size):
+                raise ValueError(f"the caches must have {num_pages} pages of {page_size} tokens, "
+                                 f"got {c.k_cache.shape[0]} of {c.k_cache.shape[2]} in layer {i}")
         self.page_size = int(page_size)
         self.page_table = torch.full((rows, -(-max_tokens // page_size)), -1, dtype=torch.int32, device=device)
         self.seq_lens = torch.zeros((rows,), dtype=torch.int32, device=device)
         self.refs = torch.zeros((num_pages,), dtype=torch.int32, device=device)
-        self.layers = kv8_layers(caches) if len(caches) else None
+        self.layers = kv8_layers(caches) if caches else None
 
     def _state(self):
         return self.page_table, self.seq_lens, self.refs, self.page_size
@@ -78,7 +85,9 @@ class KV8Pages:
     def _counts(self, n, rows):
         import torch
 
-        return torch.full(rows.shape, n, dtype=torch.int32, device=rows.device) if isinstance(n, int) else n
+        if isinstance(n, torch.Tensor):
+            return n
+        return torch.full(rows.shape, operator.index(n), dtype=torch.int32, device=rows.device)
 
     def extend(self, rows, new, status=None):
         """Pages for ``new`` more tokens (a number, or int32 for each) of the rows, and their lengths; returns ``status`` int32 ``[1]``.

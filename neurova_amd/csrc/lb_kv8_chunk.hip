@@ -22,6 +22,7 @@
 // 407 us, 887 TFLOP/s).  128 sequences of one new token: 161 us, 4.5 TB/s, where the operator
 // for single tokens takes 122.  The smallest calls run instructions for the first time (24 on
 // 301: 20 us, about 8 of them before the second tile and 4 for the second launch).
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_common.hpp"
@@ -922,8 +923,11 @@ struct Plan {
   size_t scratch;
 };
 
-// Above 64 sequences the row blocks that are cut have more than `most` tiles each, of
-// workers * most in all: at most as many as the workers, and their pieces twice that.
+// Of the lengths that work_of tries, those that cut the longest row block into up to kCuts leave
+// each of the others with no more; those that share out what all have in all are at least
+// work / workers long, so that the pieces are at most the workers and one for each row block (and
+// one, for the share in fp32).  No plan has more parts (24 new tokens, 24 / 4 heads of 256, with a
+// table of 32768: 264 of 130 KB, where four for each worker would be 1024).
 Plan plan_of(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv, int64_t head_dim, int64_t max_tokens) {
   Plan p;
   p.workers = (head_dim == 64 ? kPerSimd<64> : head_dim == 128 ? kPerSimd<128> : kPerSimd<256>) * (int64_t)lbh::device_cus();
@@ -932,7 +936,8 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads_q, int64_t heads_kv, i
   p.joined = tiles > kMinTiles;
   // no more pieces than all row blocks have of the smallest size
   const int64_t pieces = blocks * ((tiles + kMinTiles - 1) / kMinTiles);
-  p.slots = !p.joined ? 0 : pieces < kPartRounds * p.workers ? pieces : kPartRounds * p.workers;
+  const int64_t cuts = (kCuts + 1) * blocks, shares = p.workers + blocks + 1;
+  p.slots = !p.joined ? 0 : std::min({pieces, kPartRounds * p.workers, std::max(cuts, shares)});
   p.blocks = blocks, p.grid = blocks + p.slots;
   p.scratch = p.slots ? (((size_t)p.slots * kRows * (head_dim + 2) * 4 + 255) & ~(size_t)255) + 256 : 0;
   return p;

@@ -296,3 +296,24 @@ def test_a_hundred_million_tokens(dev):
         bound = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -16 + 5 * 3100 * 2.0 ** -24) * spread + 2.0 ** -25
         assert float(want.abs().median()) > 8 * float(bound.median())
         assert ((out[0, h].double() - want).abs() <= bound).all(), (h, float((out[0, h].double() - want).abs().max()), float((out[0, h] - p[0, h]).abs().max()))
+
+
+@pytest.mark.parametrize("news,held,hq,hkv,d,p", [([24], [9000], 24, 4, 256, 64), ([1], [20000], 1, 1, 64, 16), ([1] * 70, [3000] * 70, 2, 1, 128, 32),
+                                                  ([3] * 5 + [700], [6000] * 6, 8, 2, 128, 16), ([40] + [1] * 280, [9000] + [64] * 280, 3, 3, 64, 32),
+                                                  ([130, 1, 1], [4000, 12000, 3], 4, 1, 256, 128), ([900], [2500], 40, 8, 128, 64)])
+def test_parts_stay_in_the_scratch_that_is_asked_for(dev, news, held, hq, hkv, d, p):
+    import torch
+
+    from neurova_amd import capi
+    from tests.test_gpu_kv8_chunk import Chunks
+
+    print_case("serving-scratch", len(news), hq, hkv, d, p)
+    c = Chunks(dev, news, held, hq, hkv, d, p, seed=31, wide=1 + 20000 // p)   # tables of more than any sequence holds
+    need = capi.kv8_chunk_attention_scratch_bytes(len(news), sum(news), hq, hkv, d, p, c.table.shape[1])
+    whole = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device=dev)
+    out = torch.full(c.q.shape, 7.0, dtype=torch.float16, device=dev)
+    assert capi.kv8_chunk_attention(c.q, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.table, c.seq_lens, c.starts, out, whole[:need],
+                                    d ** -0.5) == capi.LB_OK
+    torch.cuda.synchronize()
+    c.check(out, heads=(0, hq - 1), most=60)
+    assert (whole[need:] == 0x5A).all()

@@ -324,8 +324,8 @@ int lb_kv8_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_s
  * call.  Row i of n sees the keys 0 to seq_lens[b] - n + i that the table holds;
  * one that sees none (padding before position 0) is zero, and rows of tokens that
  * belong to no sequence are left as they are.  Scores, softmax and sums are fp32;
- * a weight times its value scale enters the second product as one fp16 number
- * (2^-11, and 2^-32 of the row's largest; value scales of any size up to 2^32, and
+ * a weight times its value scale enters the second product as one fp16 number, where
+ * lb_kv8_attention takes two (2^-11, and 2^-32 of the row's largest; value scales of any size up to 2^32, and
  * fp16 values give 2^9 at most).  A page's scale that is not finite reaches the rows
  * that see a token of the page.
  * One launch, or with tables of more than 128 tokens a second one, which joins the

@@ -149,8 +149,7 @@ struct Work {
 // A lane tries one length of the pieces: the longest row block's keys cut into one to
 // kCuts, or what all workers have in all and somewhat more, so that all run at once.  What
 // has the least rounds of pieces times their mean length, and the time that a piece takes
-// besides, is taken.  (Above 64 sequences: what
-// the workers have in all.)
+// besides, is taken.  (Above 64 sequences: what the workers have in all.)
 __device__ __forceinline__ Work work_of(const ChunkArgs& a, const Sizes& z) {
   const int lane = lane_id(), blocks = z.blocks[0], tiles = z.tiles[0];
   const float heads = (float)a.heads_kv.d, slots = __builtin_amdgcn_rcpf((float)a.workers);
@@ -348,9 +347,10 @@ __device__ __forceinline__ int k_swizzle(int key) {
 }
 
 // Sixteen tiles' pages and scales are looked up together (4096 on 12288 1267 us, and 1300 with
-// a tile's at a time), lane l those of the 16 tokens l % 4 of tile l / 4, and what the products need of them lies in LDS for all waves: the
-// factor of the scores, the value scale as an exponent, the inverse of that (2^-kLift
-// times), and what is left of a value scale outside the exponent's range.
+// a tile's at a time), lane l those of the 16 tokens l % 4 of tile l / 4, and what the products
+// need of them lies in LDS for all waves: the factor of the scores, the value scale as an
+// exponent, the inverse of that (2^-kLift times), and what is left of a value scale outside
+// the exponent's range.
 constexpr int kBatch = 16;
 typedef f32x4 Info[2][kBatch * 4];
 

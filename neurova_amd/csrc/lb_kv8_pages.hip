@@ -8,9 +8,10 @@
 //
 // Bound by latency: a few dependent loads (rows, lengths, holders, pages) and the
 // launches.  free takes 2 to 5 us, fork 3 to 5, extend 8 to 11 (200 rows, and 100000 tokens
-// for each of six), the plan of compact 7 to 8.  One workgroup plans, since every count goes
-// by all rows before it.  Copies are bound by HBM (951 pages of 128 KB in each of four layers,
-// read and written: 190 us, 5.2 TB/s).
+// for each of six; 200 rows with caches of 1, 32 and 64 layers and nothing to copy 9.7, 10.2
+// and 11.4), the plan of compact 7 to 8.  One workgroup plans, since every count goes by all
+// rows before it.  Copies are bound by HBM (951 pages of 128 KB in each of four layers, read
+// and written: 190 us, 5.2 TB/s).
 #include "attn_common.hpp"
 
 namespace lb {
@@ -26,7 +27,9 @@ struct Pages {
 constexpr int kMaxRows = 4096;
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / kWave;
 constexpr int kEach = kMaxRows / kPlanThreads;
-constexpr int kClaims = 8192;  // rows of a table in which a row's first mention is found by its number, not by a search
+// Rows of a table in which a row's first mention is found by its number, not by a search (extend
+// of 4096 rows, of 4096 and of 9000: 16 and 296 us).
+constexpr int kClaims = 8192;
 
 // Pages of `tokens` (not below 0).
 __device__ __forceinline__ int pages_of(int tokens, const Pages& p) { return (int)(((uint32_t)tokens + (1u << p.shift) - 1) >> p.shift); }
@@ -246,7 +249,7 @@ __global__ __launch_bounds__(kPlanThreads) void extend_kernel(Pages p, const int
   any_shared = __syncthreads_or(any_shared);
   int copied = 0;  // bit e
   if (any_shared) {
-    // all but the last of a page's holders take a copy
+    // all but the last of a page's holders take a copy (1024 rows that share one page 42 us, 4096 326)
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int i = i0 + e;

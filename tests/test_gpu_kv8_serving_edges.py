@@ -317,3 +317,55 @@ def test_parts_stay_in_the_scratch_that_is_asked_for(dev, news, held, hq, hkv, d
     torch.cuda.synchronize()
     c.check(out, heads=(0, hq - 1), most=60)
     assert (whole[need:] == 0x5A).all()
+
+
+def test_nothing_to_do(dev):
+    """No rows in a call, in a table, no pages, no tokens, no sequences: nothing changes, and extend says that it is done."""
+    import torch
+
+    from neurova_amd.attention import KV8Cache
+    from neurova_amd.pages import KV8Pages, copy_pages
+    from tests.test_gpu_kv8_chunk import Chunks
+
+    print_case("serving-nothing")
+    none, one = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([], [0]))
+    for num, rows, tokens in ((6, 3, 100), (6, 0, 100), (6, 3, 0), (0, 3, 100), (0, 0, 0)):
+        caches = [KV8Cache(num, 2, 64, page_size=16, device=dev) for _ in range(2)]
+        for own in ((), caches):
+            pages = KV8Pages(num, rows, tokens, page_size=16, caches=own, device=dev)
+            assert int(pages.extend(none, 5)) == 0 and int(pages.extend(one, 0)) == 0 and int(pages.extend(none, none)) == 0
+            pages.fork(none, none)
+            pages.fork(one, one, 5)
+            pages.free(none)
+            pages.free(one, 3)
+            assert int(pages.compact()) == 0
+            assert not pages.refs.any() and not pages.seq_lens.any() and (pages.page_table == -1).all()
+        copy_pages(caches, none, none)
+    c = Chunks(dev, [4, 0, 9], [30, 7, 0], 4, 2, 64, 16, seed=41, extra=2)
+    want = c.run()
+    c.check(want)
+    assert c.run(q=c.q[:0]).shape == (0, 4, 64)
+    c.starts, c.seq_lens, c.table = c.starts[:1], c.seq_lens[:0], c.table[:0]
+    assert (c.run() == 7).all()
+
+
+def test_two_streams_at_once(dev):
+    """Calls that cut their keys, on two streams without any order between them: each has a scratch of its own."""
+    import torch
+
+    from tests.test_gpu_kv8_chunk import Chunks
+
+    print_case("serving-streams")
+    a, b = Chunks(dev, [40, 1, 1], [9000, 700, 2], 8, 2, 128, 16, seed=42), Chunks(dev, [70], [12000], 6, 1, 256, 64, seed=43)
+    wants = [a.run(), b.run()]
+    a.check(wants[0], heads=(0, 7), most=30)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [[torch.empty_like(w) for _ in range(20)] for w in wants]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for c, o, st in zip((a, b), outs, streams):
+            with torch.cuda.stream(st):
+                c.run(out=o[i])
+    torch.cuda.synchronize()
+    for want, got in zip(wants, outs):
+        assert all(torch.equal(want, o) for o in got)
